@@ -43,7 +43,13 @@ typedef enum {
 typedef enum { SVSX_L2 = 0, SVSX_IP = 1, SVSX_COSINE = 2 } svsx_metric;
 
 /* svs::DataType subset with AVX-512 kernels (lib/datatype.h): float32, float16, int8, uint8 */
-typedef enum { SVSX_F32 = 0, SVSX_F16 = 1, SVSX_I8 = 2, SVSX_U8 = 3 } svsx_dtype;
+typedef enum {
+    SVSX_F32 = 0,
+    SVSX_F16 = 1,
+    SVSX_I8 = 2,
+    SVSX_U8 = 3,
+    SVSX_BF16 = 4 /* rows of the paged cache and of attention only (svsx_cache_*, svsx_*attention*): an index refuses it */
+} svsx_dtype;
 
 typedef struct svsx_index svsx_index;
 
@@ -394,6 +400,121 @@ int svsx_get_distance(const svsx_index* index, uint64_t id, const void* query, i
  *   mode 0        frees either.
  * SVSX_NOT_IMPLEMENTED for other row types.  Call while no search is in flight on this index. */
 int svsx_index_build_bound_codes(svsx_index* index, int mode);
+
+/* ---- paged cache of rows ----------------------------------------------------------------------------------------------------------------
+ * Rows that a model stores token by token (keys and values of attention; no reference counterpart), in pages that sequences take, share and give back.
+ * The cache is the caller's arrays, all resident in HBM on `device`; a call reads and changes them in stream order, never waits, allocates nothing and may be captured
+ * into a graph.  Calls that change one cache must be ordered among each other and with the calls that read it (one stream, or events).
+ *   d_keys     [n_layers][n_pages][n_heads][page_size][key_dim]    of `dtype` (SVSX_F32, SVSX_F16, SVSX_BF16)
+ *   d_values   [n_layers][n_pages][n_heads][page_size][value_dim]  NULL with value_dim = 0: the rows are keys and values at once (latent rows)
+ *   d_table    [n_sequences][max_pages]  row r of a sequence is row r % page_size of page table[r / page_size]; -1 behind the sequence's last page
+ *   d_lengths  [n_sequences]             rows of each sequence (0: empty)
+ *   d_refs     [n_pages]                 how many sequences hold the page (0: free)
+ *   d_failures [1]                       counts the entries of all calls that were refused ON THE DEVICE (below); the caller zeroes and reads it
+ * A new cache is: table all -1, everything else 0.  Limits: n_sequences <= 4096; max_pages * page_size and max_pages * n_sequences < 2^31.
+ * Lists of sequences are device arrays of int32, at most 4096 a call.  An entry is refused -- it changes nothing and is counted in d_failures -- when
+ * its sequence does not exist, when the call named the same sequence in an earlier entry (sequences that grow, targets), or when there is no room.  Pages are
+ * taken lowest first, in the order of the entries; the first entry that the free pages do not suffice for is refused, and every later one that needs pages.
+ *   _extend   sequence i grows by d_offsets[i + 1] - d_offsets[i] rows (d_offsets: n + 1 device int32, rising, within [0, n_tokens]; otherwise every
+ *             entry is refused).  d_slots [n_tokens]: where new row t goes (page * page_size + row in the page); -1 for the rows of refused entries and for
+ *             rows that no entry has.  Also refused: more pages than a table row has.
+ *   _write    rows of one layer to their slots: row t of head h at d_keys + t * key_token_stride + h * key_head_stride (elements; values alike), contiguous
+ *             within the row.  Slots outside the cache are skipped.  The slots of one call differ from each other.
+ *   _copy     target i, an empty sequence, becomes a copy of source i.  share = 0: in pages of its own.  share != 0 (fork): full pages are held by
+ *             both, a partly filled last page is copied -- so pages held twice are full, and no row is ever written to one.  Also refused: a
+ *             target that holds rows or is its own source, a source that is a target of the same call.  Rows of a page behind the sequence's last one stay as they were.
+ *   _free     the sequences become empty; a page nobody holds any more is free.  Naming a sequence twice frees it once.
+ *   _compact  with U pages in use, the used pages from U on move, in order, to the free pages below U, in order; tables follow.
+ *             d_moved [n_pages]: the page's new place, -1 for a page that was free.
+ * d_workspace: svsx_cache_workspace bytes (for a call with n entries), used by this call alone until it has run. */
+typedef struct {
+    size_t struct_size; /* sizeof(svsx_cache_desc) */
+    int device;
+    int dtype;
+    size_t n_layers, n_pages, n_heads, page_size, key_dim, value_dim;
+    size_t n_sequences, max_pages;
+    void* d_keys;
+    void* d_values;
+    int32_t* d_table;
+    int32_t* d_lengths;
+    int32_t* d_refs;
+    int32_t* d_failures;
+} svsx_cache_desc;
+int svsx_cache_workspace(const svsx_cache_desc* desc, size_t n, size_t* bytes);
+int svsx_cache_extend_device(
+    const svsx_cache_desc* desc, const int32_t* d_sequences, const int32_t* d_offsets, size_t n, size_t n_tokens, int64_t* d_slots, void* d_workspace,
+    size_t workspace_bytes, void* hip_stream
+);
+int svsx_cache_write_device(
+    const svsx_cache_desc* desc, size_t layer, const int64_t* d_slots, size_t n_tokens, const void* d_keys, size_t key_token_stride, size_t key_head_stride,
+    const void* d_values, size_t value_token_stride, size_t value_head_stride, void* hip_stream
+);
+int svsx_cache_copy_device(
+    const svsx_cache_desc* desc, const int32_t* d_sources, const int32_t* d_targets, size_t n, int share, void* d_workspace, size_t workspace_bytes, void* hip_stream
+);
+int svsx_cache_free_device(const svsx_cache_desc* desc, const int32_t* d_sequences, size_t n, void* hip_stream);
+int svsx_cache_compact_device(const svsx_cache_desc* desc, int32_t* d_moved, void* d_workspace, size_t workspace_bytes, void* hip_stream);
+
+/* ---- attention over rows in HBM ---------------------------------------------------------------------------------------------------------------
+ * out[i][h] = sum_r p_r v_r / sum_r p_r with p_r = exp(scale * <q[i][h], k_r>): one new token's attention (no reference counterpart; svsx_flat_search's
+ * exhaustive inner products with a softmax in the place of the k best).  Sums and the softmax are kept in float32.
+ *   rows      query i attends to rows 0 .. d_lengths[s] - 1 of sequence s = d_sequences[i] (NULL: s = i); row r is row r % page_size of page
+ *             d_table[s * table_stride + r / page_size], at most max_pages of them.  An entry outside [0, n_pages) is a hole: its rows are left out (page_size 1: the
+ *             table may be the ids32 of svsx_search_device over the same rows).  A sequence outside [0, n_sequences) has no rows.
+ *   heads     n_heads is a multiple of n_key_heads; head h reads key head h / (n_heads / n_key_heads).
+ *   values    d_values = NULL: the first value_dim (<= key_dim) columns of a key row are its value (latent attention, absorbed: n_key_heads = 1).
+ *   d_out     [n_queries][n_heads][value_dim] of dtype; a query without rows (or all of whose products are -inf) gives zeros
+ *   d_lse     [n_queries][n_heads] float32 or NULL: log sum_r p_r; -inf where there is nothing
+ * Strides are in elements; rows are contiguous.  key_dim and value_dim are at most 1024.
+ * The workspace (svsx_paged_attention_workspace bytes, possibly 0) belongs to the call until it has run.  Device pointers, enqueued on hip_stream, no waiting. */
+typedef struct {
+    size_t struct_size; /* sizeof(svsx_attention_desc) */
+    int device;
+    int dtype;          /* SVSX_F32, SVSX_F16, SVSX_BF16: queries, rows and out */
+    size_t n_queries, n_heads, n_key_heads, key_dim, value_dim;
+    size_t n_pages, page_size, n_sequences, max_pages, table_stride;
+    const void* d_queries;
+    size_t query_stride, query_head_stride;
+    const void* d_keys;
+    size_t key_page_stride, key_head_stride, key_row_stride;
+    const void* d_values;
+    size_t value_page_stride, value_head_stride, value_row_stride;
+    const int32_t* d_table;
+    const int32_t* d_lengths;
+    const int32_t* d_sequences;
+    float scale;
+    void* d_out;
+    float* d_lse;
+} svsx_attention_desc;
+int svsx_paged_attention_workspace(const svsx_attention_desc* desc, size_t* bytes);
+int svsx_paged_attention_device(const svsx_attention_desc* desc, void* d_workspace, size_t workspace_bytes, void* hip_stream);
+
+/* Latent attention in its expanded form, for prompts: row r's key for head h is (w_key[h] c_r, rotary part of row r), its value w_value[h] c_r, with c_r the
+ * first `rank` columns of the row.  Sequence i has queries d_query_offsets[i] .. d_query_offsets[i + 1] - 1 and rows d_row_offsets[i] .. (rising device int32,
+ * n_sequences + 1 each; parts outside the arrays are left out); its last query is aligned with its last row, and with `causal` a query sees the rows up to its own.
+ *   d_queries  [n_tokens][n_heads][nope_dim + rope_dim]     d_rows     [n_rows][rank + rope_dim]
+ *   d_w_key    [n_heads][nope_dim][rank], contiguous        d_w_value  [n_heads][value_dim][rank], contiguous
+ *   d_out      [n_tokens][n_heads][value_dim], contiguous; a query that sees no row gives zeros.  Queries in no sequence: zeros, or with keep_rest left alone.
+ * nope_dim + rope_dim <= 1024, value_dim <= 1024, rank + rope_dim <= 1024.  For the 16-bit types the expanded keys and values are rounded to dtype. */
+typedef struct {
+    size_t struct_size; /* sizeof(svsx_expanded_desc) */
+    int device;
+    int dtype;
+    size_t n_sequences, n_tokens, n_rows, n_heads, nope_dim, rope_dim, rank, value_dim;
+    const void* d_queries;
+    size_t query_stride, query_head_stride;
+    const void* d_rows;
+    size_t row_stride;
+    const void* d_w_key;
+    const void* d_w_value;
+    const int32_t* d_query_offsets;
+    const int32_t* d_row_offsets;
+    float scale;
+    int causal, keep_rest;
+    void* d_out;
+} svsx_expanded_desc;
+int svsx_latent_expanded_workspace(const svsx_expanded_desc* desc, size_t* bytes);
+int svsx_latent_expanded_device(const svsx_expanded_desc* desc, void* d_workspace, size_t workspace_bytes, void* hip_stream);
 
 /* Index facts: info[0]=n, [1]=d, [2]=data bytes in HBM, [3]=graph bytes in HBM, [4]=graph row stride (u32),
  * [5]=data row stride (bytes). */

@@ -85,6 +85,44 @@ class BuildParams(C.Structure):
     ]
 
 
+class CacheDesc(C.Structure):
+    """svsx_cache_desc."""
+
+    _fields_ = [
+        ("struct_size", C.c_size_t), ("device", C.c_int), ("dtype", C.c_int),
+        ("n_layers", C.c_size_t), ("n_pages", C.c_size_t), ("n_heads", C.c_size_t), ("page_size", C.c_size_t), ("key_dim", C.c_size_t), ("value_dim", C.c_size_t),
+        ("n_sequences", C.c_size_t), ("max_pages", C.c_size_t),
+        ("d_keys", C.c_void_p), ("d_values", C.c_void_p), ("d_table", C.c_void_p), ("d_lengths", C.c_void_p), ("d_refs", C.c_void_p), ("d_failures", C.c_void_p),
+    ]
+
+
+class AttentionDesc(C.Structure):
+    """svsx_attention_desc."""
+
+    _fields_ = [
+        ("struct_size", C.c_size_t), ("device", C.c_int), ("dtype", C.c_int),
+        ("n_queries", C.c_size_t), ("n_heads", C.c_size_t), ("n_key_heads", C.c_size_t), ("key_dim", C.c_size_t), ("value_dim", C.c_size_t),
+        ("n_pages", C.c_size_t), ("page_size", C.c_size_t), ("n_sequences", C.c_size_t), ("max_pages", C.c_size_t), ("table_stride", C.c_size_t),
+        ("d_queries", C.c_void_p), ("query_stride", C.c_size_t), ("query_head_stride", C.c_size_t),
+        ("d_keys", C.c_void_p), ("key_page_stride", C.c_size_t), ("key_head_stride", C.c_size_t), ("key_row_stride", C.c_size_t),
+        ("d_values", C.c_void_p), ("value_page_stride", C.c_size_t), ("value_head_stride", C.c_size_t), ("value_row_stride", C.c_size_t),
+        ("d_table", C.c_void_p), ("d_lengths", C.c_void_p), ("d_sequences", C.c_void_p), ("scale", C.c_float), ("d_out", C.c_void_p), ("d_lse", C.c_void_p),
+    ]
+
+
+class ExpandedDesc(C.Structure):
+    """svsx_expanded_desc."""
+
+    _fields_ = [
+        ("struct_size", C.c_size_t), ("device", C.c_int), ("dtype", C.c_int),
+        ("n_sequences", C.c_size_t), ("n_tokens", C.c_size_t), ("n_rows", C.c_size_t), ("n_heads", C.c_size_t), ("nope_dim", C.c_size_t), ("rope_dim", C.c_size_t),
+        ("rank", C.c_size_t), ("value_dim", C.c_size_t),
+        ("d_queries", C.c_void_p), ("query_stride", C.c_size_t), ("query_head_stride", C.c_size_t), ("d_rows", C.c_void_p), ("row_stride", C.c_size_t),
+        ("d_w_key", C.c_void_p), ("d_w_value", C.c_void_p), ("d_query_offsets", C.c_void_p), ("d_row_offsets", C.c_void_p),
+        ("scale", C.c_float), ("causal", C.c_int), ("keep_rest", C.c_int), ("d_out", C.c_void_p),
+    ]
+
+
 EXPORTS = [
     "svsx_index_create", "svsx_index_create_device_view", "svsx_index_destroy", "svsx_search", "svsx_search_device",
     "svsx_distance_batch", "svsx_merge_topk_device", "svsx_prune_device", "svsx_flat_search_device", "svsx_index_info", "svsx_last_error", "svsx_version",
@@ -95,6 +133,8 @@ EXPORTS = [
     "svsx_sharded_search_device", "svsx_abi_version", "svsx_flat_search_device_counted", "svsx_flat_search",
     "svsx_index_refresh_row_norms", "svsx_index_drop_row_norms", "svsx_range_search", "svsx_get_distance", "svsx_index_memory",
     "svsx_sharded_plan", "svsx_sharded_set_timing", "svsx_sharded_phase_times",
+    "svsx_cache_workspace", "svsx_cache_extend_device", "svsx_cache_write_device", "svsx_cache_copy_device", "svsx_cache_free_device", "svsx_cache_compact_device",
+    "svsx_paged_attention_workspace", "svsx_paged_attention_device", "svsx_latent_expanded_workspace", "svsx_latent_expanded_device",
 ]
 
 _lib = None
@@ -168,6 +208,21 @@ def lib() -> C.CDLL:
             L.svsx_index_drop_row_norms.argtypes = [C.c_void_p]
             L.svsx_range_search.argtypes = [C.c_void_p, C.c_void_p, C.c_int, C.c_size_t, C.c_float, C.POINTER(SearchParams), C.c_void_p, RESULTS_ALLOCATOR, C.c_void_p]
             L.svsx_get_distance.argtypes = [C.c_void_p, C.c_uint64, C.c_void_p, C.c_int, C.POINTER(C.c_double)]
+        except AttributeError:
+            if not os.environ.get("SVSX_LIB"):
+                raise
+        try:  # operators over paged rows: likewise absent from an older build
+            L.svsx_cache_workspace.argtypes = [C.POINTER(CacheDesc), C.c_size_t, C.POINTER(C.c_size_t)]
+            L.svsx_cache_extend_device.argtypes = [C.POINTER(CacheDesc), C.c_void_p, C.c_void_p, C.c_size_t, C.c_size_t, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]
+            L.svsx_cache_write_device.argtypes = [C.POINTER(CacheDesc), C.c_size_t, C.c_void_p, C.c_size_t, C.c_void_p, C.c_size_t, C.c_size_t, C.c_void_p, C.c_size_t,
+                                                  C.c_size_t, C.c_void_p]
+            L.svsx_cache_copy_device.argtypes = [C.POINTER(CacheDesc), C.c_void_p, C.c_void_p, C.c_size_t, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p]
+            L.svsx_cache_free_device.argtypes = [C.POINTER(CacheDesc), C.c_void_p, C.c_size_t, C.c_void_p]
+            L.svsx_cache_compact_device.argtypes = [C.POINTER(CacheDesc), C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]
+            L.svsx_paged_attention_workspace.argtypes = [C.POINTER(AttentionDesc), C.POINTER(C.c_size_t)]
+            L.svsx_paged_attention_device.argtypes = [C.POINTER(AttentionDesc), C.c_void_p, C.c_size_t, C.c_void_p]
+            L.svsx_latent_expanded_workspace.argtypes = [C.POINTER(ExpandedDesc), C.POINTER(C.c_size_t)]
+            L.svsx_latent_expanded_device.argtypes = [C.POINTER(ExpandedDesc), C.c_void_p, C.c_size_t, C.c_void_p]
         except AttributeError:
             if not os.environ.get("SVSX_LIB"):
                 raise

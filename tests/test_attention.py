@@ -1,0 +1,558 @@
+"""Attention over paged rows (paged_attention, latent_attention, latent_attention_expanded) against its formula in 64 bits.
+
+Tolerances, fixed before the first run.  u = half a step of the type (finfo.eps / 2).  With A = sum p |v| / sum p and o the exact result, in every
+column:
+  |error| <= u |o|                    the result rounded to the type
+           + u A                      p rounded to the type before it meets v (16-bit types; float32: u = 2^-24 covers exp's last bits)
+           + 2 d A                    d = error of a score: (32 + dk / 32) roundings of 2^-24 of sum |q k| scale (sums of 32 products in the matrix units,
+                                      one float32 addition per 32 columns; a chain of 32 as the worst a unit may do), and as many of |s| in exp's argument
+           + (64 + n / 32) 2^-24 A    n weighted values summed in float32, 32 at a time, 64 for the joins
+and for the logarithm of the sum: d + (64 + n / 32) 2^-24 + 2^-23 |lse|.
+The expanded form rounds keys and values to the type first: scores move by u sum |q| |K| scale, values by u A."""
+import ctypes as C
+import math
+
+import pytest
+
+from scalablevectorsearch_amd import _lib
+
+
+def _reference(q, keys, values, table, lengths, sequences, value_dim, scale):
+    """(out, lse, bound of out, bound of lse) of paged attention in float64 on the CPU, row by row as include/svsx.h says"""
+    import torch
+
+    u = torch.finfo(q.dtype).eps / 2
+    e = 2.0**-24
+    q, keys, table, lengths = q.cpu().double(), keys.cpu().double(), table.cpu(), lengths.cpu()
+    values = values.cpu().double() if values is not None else keys[..., :value_dim]
+    n, heads, dim = q.shape
+    pages, kv, page, _ = keys.shape
+    out, bound = torch.zeros(n, heads, value_dim, dtype=torch.float64), torch.zeros(n, heads, value_dim, dtype=torch.float64)
+    lse, lse_bound = torch.full((n, heads), -math.inf, dtype=torch.float64), torch.zeros(n, heads, dtype=torch.float64)
+    for i in range(n):
+        s = i if sequences is None else int(sequences[i])
+        if not 0 <= s < table.shape[0]:
+            continue
+        at = torch.arange(min(max(int(lengths[s]), 0), table.shape[1] * page))
+        of = table[s].long()[at // page]
+        there = (of >= 0) & (of < pages)
+        of, at = of[there], at[there] % page
+        if not len(at):
+            continue
+        for h in range(heads):
+            g = h // (heads // kv)
+            k, v = keys[of, g, at], values[of, g, at]
+            x = (k @ q[i, h]) * scale
+            top = x.max()
+            if top == -math.inf:
+                continue
+            p = torch.exp(x - top)
+            total = p.sum()
+            out[i, h] = (p[:, None] * v).sum(0) / total
+            lse[i, h] = top + torch.log(total)
+            a = (p[:, None] * v.abs()).sum(0) / total
+            some = x > -math.inf
+            d = (32 + dim / 32) * e * ((k[some].abs() @ q[i, h].abs()).max() * abs(scale) + x[some].abs().max())
+            sums = (64 + len(at) / 32) * e
+            bound[i, h] = u * out[i, h].abs() + (u + 2 * d + sums) * a
+            lse_bound[i, h] = d + sums + 2 * e * lse[i, h].abs()
+    return out, lse, bound, lse_bound
+
+
+def _check(got, lse, want):
+    out, lse64, bound, lse_bound = want
+    import torch
+
+    got, lse = got.cpu().double(), lse.cpu().double()
+    assert torch.equal(got.isnan(), out.isnan()) and torch.equal(lse.isinf(), lse64.isinf()) and torch.equal(lse.isnan(), lse64.isnan())
+    if not out.numel():
+        return
+    off = ((got - out).abs() - bound).nan_to_num(-1.0)
+    assert off.max() <= 0, f"worst excess {off.max().item()} at {off.argmax().item()} of {tuple(off.shape)}"
+    off = ((lse - lse64).abs() - lse_bound).nan_to_num(-1.0)
+    assert off.max() <= 0, f"lse: worst excess {off.max().item()}"
+
+
+def _case(dtype, lengths, heads, kv, dim, value_dim, page, seed=0, shared=False, spread=1.0):
+    """queries, rows in pages of no order with NaN behind every sequence's last row and in the pages nobody has, table, lengths"""
+    import torch
+
+    g = torch.Generator().manual_seed(seed)
+    n, t = len(lengths), getattr(torch, dtype)
+    taken = [-(-x // page) for x in lengths]
+    pages, columns = sum(taken) + 3, max(max(taken), 1)
+    order = torch.randperm(pages, generator=g)
+    table = torch.randint(-(2**31), 2**31 - 1, (n, columns), generator=g, dtype=torch.int64).to(torch.int32)  # what is behind a sequence's pages is not read
+    keys = torch.full((pages, kv, page, dim), math.nan)
+    values = None if shared else torch.full((pages, kv, page, value_dim), math.nan)
+    at = 0
+    for i, x in enumerate(lengths):
+        table[i, : taken[i]] = order[at:at + taken[i]].to(torch.int32)
+        for c in range(taken[i]):
+            r = min(page, x - c * page)
+            keys[order[at + c], :, :r] = torch.randn(kv, r, dim, generator=g) * spread
+            if not shared:
+                values[order[at + c], :, :r] = torch.randn(kv, r, value_dim, generator=g)
+        at += taken[i]
+    q = torch.randn(n, heads, dim, generator=g)
+    return [x if x is None else x.cuda() for x in (q.to(t), keys.to(t), None if shared else values.to(t), table, torch.tensor(lengths, dtype=torch.int32))]
+
+
+def _run(q, keys, values, table, lengths, sequences=None, value_dim=None, scale=None):
+    import scalablevectorsearch_amd as svs
+
+    value_dim = value_dim or (values.shape[3] if values is not None else keys.shape[3])
+    out, lse = svs.paged_attention(q, keys, values, table, lengths, sequences=sequences, value_dim=value_dim, scale=scale, return_lse=True)
+    assert out.dtype == q.dtype and out.shape == (*q.shape[:2], value_dim) and lse.shape == q.shape[:2]
+    _check(out, lse, _reference(q, keys, values, table, lengths, sequences, value_dim, q.shape[2]**-0.5 if scale is None else scale))
+    return out, lse
+
+
+DTYPES = ["float32", "float16", "bfloat16"]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lengths, heads, kv, dim, value_dim, page", [
+    ([1], 1, 1, 1, 1, 1), ([0, 1, 2, 15, 16, 17, 31, 32, 33, 64, 65, 300], 8, 2, 128, 128, 16), ([5, 700, 129], 32, 8, 64, 64, 8),
+    ([40, 0, 1000], 6, 2, 96, 96, 32), ([70, 33], 14, 2, 80, 80, 5), ([500, 3], 16, 1, 100, 36, 7), ([257, 64], 34, 2, 256, 256, 64),
+    ([90, 1], 20, 1, 33, 128, 3), ([45], 5, 5, 192, 128, 128), ([130, 20], 3, 1, 200, 200, 1), ([77], 2, 1, 768, 768, 16), ([35], 4, 2, 1024, 1000, 4),
+    ([2100, 1500], 4, 4, 128, 128, 16), ([64, 200], 12, 1, 128, 64, 256),
+])
+def test_paged_attention_is_its_formula(dtype, lengths, heads, kv, dim, value_dim, page):
+    _run(*_case(dtype, lengths, heads, kv, dim, value_dim, page))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lengths, heads, dim, value_dim, page", [
+    ([1, 0, 63, 64, 65], 16, 576, 512, 16), ([400, 33], 128, 576, 512, 64), ([90], 20, 288, 256, 1), ([70, 5, 129], 8, 320, 256, 32), ([333], 64, 544, 512, 16),
+    ([100, 31], 40, 96, 64, 16), ([50], 3, 130, 129, 8), ([1030], 130, 576, 512, 16),
+])
+def test_latent_attention_is_its_formula(dtype, lengths, heads, dim, value_dim, page):
+    import torch
+
+    import scalablevectorsearch_amd as svs
+
+    q, rows, _, table, n = _case(dtype, lengths, heads, 1, dim, value_dim, page, shared=True)
+    out, lse = _run(q, rows, None, table, n, value_dim=value_dim, scale=0.07)
+    again, lse2 = svs.latent_attention(q, rows, table, n, value_dim, scale=0.07, return_lse=True)
+    assert torch.equal(out, again) and torch.equal(lse, lse2)  # and the same bits from the same call
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shared", [False, True])
+def test_long_sequences_beside_short_ones(dtype, shared):
+    """the work is split over the length: 9 000 rows beside one row and none"""
+    _run(*_case(dtype, [9000, 1, 0, 4100], 4, 1, 64, 64, 16, shared=shared))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("page, dim, heads, kv", [(1, 96, 1, 1), (1, 128, 8, 2), (4, 64, 4, 4), (16, 576, 16, 1), (1, 100, 3, 1)])
+def test_holes_are_left_out(dtype, page, dim, heads, kv):
+    """table entries that are no page, among them all of one query's; rows in pages that nobody names hold NaN"""
+    import torch
+
+    q, keys, values, table, lengths = _case(dtype, [100, 37, 64, 1, 80], heads, kv, dim, dim, page, seed=2)
+    g = torch.Generator().manual_seed(1)
+    holes = torch.rand(table.shape, generator=g).cuda() < 0.4
+    table[holes] = torch.where(torch.rand(int(holes.sum()), generator=g).cuda() < 0.5, -1, keys.shape[0] + 5).to(torch.int32)
+    table[2] = -1
+    table[4, -1] = 2**31 - 1
+    out, lse = _run(q, keys, values, table, lengths)
+    assert not out[2].any() and (lse[2] == -math.inf).all()
+    _run(q, keys, None, table, lengths, value_dim=max(1, dim - 7))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim, value_dim", [(128, 128), (576, 512), (100, 20)])
+def test_infinite_and_not_a_number_rows(dtype, dim, value_dim):
+    """a row of -inf products has no weight, all rows of -inf give nothing, a NaN that is attended to shows, one that is not does not"""
+    import torch
+
+    q, keys, values, table, lengths = _case(dtype, [50, 40, 40, 40], 4, 1, dim, value_dim, 8, seed=4, shared=dim == 576)
+    q[:, :, 0] = 1.0
+    q[1:] = q[1:].abs()
+    k = lambda b, r: keys[table[b, r // 8], 0, r % 8]  # noqa: E731
+    column = dim - 1  # no value column of the latent rows
+    q[:, :, column] = q[:, :, column].abs() + 0.5
+    for r in (0, 1, 33):
+        k(0, r)[column] = -math.inf
+    for r in range(40):
+        k(1, r)[column] = -math.inf
+    k(2, 7)[column] = math.nan
+    lowest = torch.finfo(keys.dtype).min / 4
+    for r in range(39):  # finite, and as low as the type allows without overflow of the product
+        k(3, r)[column] = lowest if dtype != "float32" else -1e30
+    q[3, :, column] = 1.0
+    out, lse = _run(q, keys, values, table, lengths, value_dim=value_dim)
+    assert not out[1].any() and (lse[1] == -math.inf).all() and out[2].isnan().all() and out[0].isfinite().all() and out[3].isfinite().all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_large_scores(dtype):
+    """scores of some hundreds, as peaked as a softmax gets; a negative scale"""
+    q, keys, values, table, lengths = _case(dtype, [300, 20], 4, 2, 64, 64, 16, spread=6.0)
+    _run(q, keys, values, table, lengths, scale=4.0)
+    _run(q, keys, values, table, lengths, scale=-1.0)
+    _run(q, keys, values, table, lengths, scale=0.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_strides_and_alignment(dtype):
+    """heads inside tokens, keys and values interleaved, rows that begin at odd elements, queries of a wider array, a table of a wider table"""
+    import torch
+
+    q, keys, values, table, lengths = _case(dtype, [70, 33, 5], 8, 2, 64, 64, 16, seed=7)
+    want = _run(q, keys, values, table, lengths)
+    inside = lambda x: x.transpose(1, 2).contiguous().transpose(1, 2)  # noqa: E731
+    kv = torch.stack([keys, values], 3)
+    wide = torch.zeros(*keys.shape[:3], 71, dtype=q.dtype, device="cuda")
+    wide[..., 3:67] = keys
+    qw = torch.cat([q, q], 2).repeat_interleave(2, 0)
+    tw = torch.cat([table, table.flip(1)], 1)
+    for a in ((q, inside(keys), inside(values), table), (q, kv[:, :, :, 0], kv[:, :, :, 1], table), (q, wide[..., 3:67], values, table),
+              (qw[::2, :, :64], keys, values, table), (q, keys, values, tw[:, : table.shape[1]]), (inside(q[None])[0], wide[..., 3:67], wide[..., 3:67], table)):
+        got = _run(*a, lengths)
+        if a[2].data_ptr() != a[1].data_ptr():  # not the last, whose values are its keys
+            assert (got[0].float() - want[0].float()).abs().max() < 0.05
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_queries_name_their_sequences(dtype):
+    """several queries of one sequence, sequences in any order, ones that do not exist, fewer queries than sequences; tables longer than lengths and shorter"""
+    import torch
+
+    q, keys, values, table, lengths = _case(dtype, [70, 33, 5, 0], 4, 2, 64, 64, 16, seed=8)
+    sequences = torch.tensor([2, 0, 0, 7, 1, -1, 3, 2], dtype=torch.int32).cuda()
+    out, _ = _run(torch.cat([q, q.flip(0)]), keys, values, table, lengths, sequences)
+    assert not out[3].any() and not out[5].any() and not out[6].any()
+    lengths[0], lengths[3] = 10**6, -5  # a length beyond the table ends with the table
+    table[0, 4] = -1
+    _run(q, keys, values, table, lengths)
+    _run(q[:0], keys, values, table, lengths, sequences[:0])
+    empty, lse = _run(q[:2], keys[:0], values[:0], table, lengths, sequences[:2])  # no pages at all
+    assert not empty.any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("metric_dim", [96, 128])
+def test_attention_over_the_answers_of_a_search(dtype, metric_dim):
+    """index.search_device -> its int32 ids are the table: attention over the rows that were found, rows and ids untouched in between"""
+    import numpy as np
+    import torch
+
+    import scalablevectorsearch_amd as svs
+
+    rng = np.random.default_rng(0)
+    x = rng.standard_normal((3000, metric_dim)).astype(np.float32)
+    rows = torch.from_numpy(x).cuda()
+    q = torch.from_numpy(rng.standard_normal((50, metric_dim)).astype(np.float32)).cuda()
+    graph = np.zeros((3000, 33), np.uint32)
+    graph[:, 0] = 32
+    graph[:, 1:] = rng.integers(0, 3000, (3000, 32))
+    index = svs.VamanaIndex(graph, x, svs.DistanceIP(), [0])
+    ids = torch.full((50, 40), -1, dtype=torch.int32, device="cuda")
+    index.search_device(q, 40, svs.VamanaSearchParameters(svs.SearchBufferConfig(64)), d_ids32=ids, d_dists=torch.empty(50, 40, device="cuda"))
+    t = getattr(torch, dtype)
+    pages = rows.to(t)[:, None, None]
+    n = torch.full((50,), 40, dtype=torch.int32, device="cuda")
+    _run(q.to(t)[:, None], pages, None, ids, n)
+
+
+@pytest.mark.gpu
+def test_another_stream_and_a_graph():
+    """the calling stream's work; two calls at once in one graph, replayed with other inputs between eager calls, equal the eager results bit for bit"""
+    import torch
+
+    import scalablevectorsearch_amd as svs
+
+    a = _case("float16", [900, 17, 0, 350], 8, 2, 128, 128, 16, seed=1)
+    b = _case("bfloat16", [700, 64], 16, 1, 576, 512, 16, seed=2, shared=True)
+
+    def both():
+        return (*svs.paged_attention(*a, return_lse=True), *svs.latent_attention(b[0], b[1], b[3], b[4], 512, return_lse=True))
+
+    want = both()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = both()
+        for x, y in zip(got, want):
+            assert torch.equal(x, y)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = both()
+    for k in range(4):
+        a[0].mul_(0.5)
+        b[0].mul_(-0.9)
+        a[4][1] = 17 - k  # lengths are read on the device
+        graph.replay()
+        want = both()
+        torch.randn(100, device="cuda").sum().item()
+        for x, y in zip(got, want):
+            assert torch.equal(x, y), k
+
+
+@pytest.mark.gpu
+def test_rows_beyond_two_to_the_31_elements():
+    import torch
+
+    pages = (1 << 31) // (16 * 128) + 9
+    keys = torch.zeros(pages, 1, 16, 128, dtype=torch.float16, device="cuda")
+    at = torch.tensor([[pages - 1, 3, pages - 4, pages - 2]], dtype=torch.int32, device="cuda")
+    keys[at[0].long()] = torch.randn(4, 1, 16, 128, device="cuda").half()
+    import scalablevectorsearch_amd as svs
+
+    q, n = torch.randn(1, 4, 128, device="cuda").half(), torch.tensor([61], dtype=torch.int32, device="cuda")
+    out, lse = svs.paged_attention(q, keys, keys, at, n, return_lse=True)
+    few = keys[at[0].long()]
+    _check(out, lse, _reference(q, few, few, torch.arange(4, dtype=torch.int32)[None], n, None, 128, 128**-0.5))
+
+
+@pytest.mark.gpu
+def test_a_run_of_the_operators_together():
+    """a prompt is attended in the expanded form and its rows go to the cache; two samples fork from it; each decodes tokens in the absorbed form, pages are
+    compacted on the way; every step's result is the formula's over the rows that the sample has seen"""
+    import torch
+
+    import scalablevectorsearch_amd as svs
+
+    g = torch.Generator().manual_seed(0)
+    heads, nope, rope, rank, dv = 4, 32, 16, 64, 32
+    new = lambda *s: torch.randn(*s, generator=g).bfloat16().cuda()  # noqa: E731
+    wk, wv = new(heads, nope, rank) / 8, new(heads, dv, rank) / 8
+    cache = svs.PagedCache(24, 8, 1, rank + rope, 0, dtype=torch.bfloat16, n_sequences=3, max_pages=6)
+    scale = (nope + rope) ** -0.5
+    off = torch.tensor([0, 21], dtype=torch.int32).cuda()
+    prompt = new(21, rank + rope)
+    cache.write(cache.extend([0], off, 21), prompt[:, None])
+    out = svs.latent_attention_expanded(new(21, heads, nope + rope), prompt, wk, wv, off, off)
+    assert out.shape == (21, heads, dv) and out.isfinite().all()
+    cache.fork([0, 0], [1, 2])
+    seen = [prompt, prompt, prompt]
+    two, ends = torch.tensor([2, 1], dtype=torch.int32).cuda(), torch.tensor([0, 1, 2], dtype=torch.int32).cuda()
+    for step in range(6):
+        rows, q = new(2, rank + rope), new(2, heads, nope + rope)
+        cache.write(cache.extend(two, ends, 2), rows[:, None])
+        seen = [seen[0], torch.cat([seen[1], rows[1:]]), torch.cat([seen[2], rows[:1]])]
+        if step == 2:
+            cache.free([0])
+            cache.compact()
+        absorbed = torch.cat([torch.matmul(q[:, :, None, :nope].float(), wk.float())[:, :, 0].bfloat16(), q[..., nope:]], -1)
+        latent, lse = cache.attend(absorbed, two, value_dim=rank, scale=scale, return_lse=True)
+        for i, s in enumerate((2, 1)):
+            n = len(seen[s])
+            _check(latent[i:i + 1], lse[i:i + 1], _reference(absorbed[i:i + 1], seen[s][:, None, None], None, torch.arange(n, dtype=torch.int32)[None],
+                                                             torch.tensor([n]), None, rank, scale))
+            whole = svs.latent_attention_expanded(q[i:i + 1], seen[s], wk, wv, torch.tensor([0, 1], dtype=torch.int32).cuda(), torch.tensor([0, n], dtype=torch.int32).cuda())
+            folded = torch.matmul(latent[i, :, None].float(), wv.float().transpose(1, 2))[:, 0]
+            assert (whole[0].float() - folded).abs().max() < 0.05  # both forms of one function; each is held to its formula elsewhere
+    assert cache.failures.item() == 0 and cache.lengths.tolist() == [0, 27, 27]
+
+
+# ---- the expanded form -----------------------------------------------------------------------------------------------------------------------------
+
+
+def _expanded(q, rows, wk, wv, qo, ro, scale, causal):
+    import torch
+
+    u, e = torch.finfo(q.dtype).eps / 2, 2.0**-24
+    q, rows, wk, wv = (x.cpu().double() for x in (q, rows, wk, wv))
+    t, heads, dim = q.shape
+    rank, nope, dv = wk.shape[2], wk.shape[1], wv.shape[1]
+    out, bound = torch.zeros(t, heads, dv, dtype=torch.float64), torch.zeros(t, heads, dv, dtype=torch.float64)
+    for i in range(len(qo) - 1):
+        c = rows[ro[i]:ro[i + 1]]
+        nq, nr = qo[i + 1] - qo[i], ro[i + 1] - ro[i]
+        for h in range(heads):
+            k, v = torch.cat([c[:, :rank] @ wk[h].T, c[:, rank:]], 1), c[:, :rank] @ wv[h].T
+            ka, va = torch.cat([c[:, :rank].abs() @ wk[h].abs().T, c[:, rank:].abs()], 1), c[:, :rank].abs() @ wv[h].abs().T  # bounds of the sums' roundings
+            for j in range(nq):
+                n = min(nr, max(0, nr - nq + j + 1)) if causal else nr
+                if n == 0:
+                    continue
+                x = (k[:n] @ q[qo[i] + j, h]) * scale
+                p = torch.softmax(x, 0)[:, None]
+                o, a = (p * v[:n]).sum(0), (p * v[:n].abs()).sum(0)
+                mag = q[qo[i] + j, h].abs()
+                chain = 64 + rank / 32 + dim / 32
+                d = abs(scale) * (u * (k[:n].abs() @ mag).max() + chain * e * (ka[:n] @ mag).max()) + 32 * e * x.abs().max()
+                out[qo[i] + j, h] = o
+                bound[qo[i] + j, h] = u * o.abs() + (2 * u + 2 * d + (64 + n / 32) * e) * a + chain * e * (p * va[:n]).sum(0)
+    return out, bound
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("counts, before, heads, nope, rope, rank, dv", [
+    ([1], [0], 1, 1, 0, 1, 1), ([1], [40], 16, 128, 64, 512, 128), ([33, 1, 0, 70], [0, 5, 3, 129], 2, 64, 32, 128, 64), ([200], [0], 2, 128, 64, 256, 128),
+    ([65, 130], [300, 0], 3, 64, 64, 96, 128), ([17, 3], [2, 90], 2, 100, 20, 60, 36), ([40], [7], 1, 33, 31, 65, 77), ([129], [128], 1, 192, 64, 512, 192),
+    ([5, 64, 63, 128], [0, 64, 1, 0], 4, 32, 16, 64, 32), ([3], [0], 2, 0, 64, 32, 16),
+])
+@pytest.mark.parametrize("causal", [True, False])
+def test_expanded_latent_attention_is_its_formula(dtype, counts, before, heads, nope, rope, rank, dv, causal):
+    import torch
+
+    import scalablevectorsearch_amd as svs
+
+    g = torch.Generator().manual_seed(3)
+    t = getattr(torch, dtype)
+    qo, ro = [0], [0]
+    for n, b in zip(counts, before):
+        qo.append(qo[-1] + n)
+        ro.append(ro[-1] + n + b)
+    q, rows = torch.randn(qo[-1], heads, nope + rope, generator=g).to(t).cuda(), torch.randn(ro[-1], rank + rope, generator=g).to(t).cuda()
+    wk, wv = (torch.randn(heads, nope, rank, generator=g) * rank**-0.5).to(t).cuda(), (torch.randn(heads, dv, rank, generator=g) * rank**-0.5).to(t).cuda()
+    off = [torch.tensor(x, dtype=torch.int32).cuda() for x in (qo, ro)]
+    got = svs.latent_attention_expanded(q, rows, wk, wv, *off, causal=causal)
+    out, bound = _expanded(q, rows, wk, wv, qo, ro, (nope + rope) ** -0.5, causal)
+    off64 = (got.cpu().double() - out).abs() - bound
+    assert off64.max() <= 0, f"worst excess {off64.max().item()} at {off64.argmax().item()} of {tuple(off64.shape)}"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_expanded_prompts_with_ragged_edges(dtype):
+    """fewer rows than queries, queries behind the last sequence and before the first (left as they were, or zero), NaN in rows of no sequence, strided inputs"""
+    import torch
+
+    import scalablevectorsearch_amd as svs
+
+    g = torch.Generator().manual_seed(6)
+    t = getattr(torch, dtype)
+    qo, ro = [3, 43, 43, 160], [2, 22, 30, 150]  # 40 queries on 20 rows, none on 8, 117 on 120
+    base = torch.randn(170, 2, 200, generator=g).to(t).cuda()
+    q = base[:, :, 5:101]
+    rows = torch.full((160, 140), math.nan, dtype=t, device="cuda")
+    rows[2:150, :128 + 1] = torch.randn(148, 129, generator=g).to(t).cuda()
+    rows = rows[:, 1:129]
+    wk, wv = (torch.randn(2, 64, 96, generator=g) / 8).to(t).cuda(), (torch.randn(2, 40, 96, generator=g) / 8).to(t).cuda()
+    off = [torch.tensor(x, dtype=torch.int32).cuda() for x in (qo, ro)]
+    out, bound = _expanded(q, rows, wk, wv, qo, ro, 96**-0.5, True)
+    got = svs.latent_attention_expanded(q, rows, wk, wv, *off)
+    assert ((got.cpu().double() - out).abs() - bound).max() <= 0
+    assert not got[:23].any() and not got[160:].any()  # the first 20 of 40 queries see no row
+    mine = torch.full((170, 2, 40), 7.0, dtype=t, device="cuda")
+    assert svs.latent_attention_expanded(q, rows, wk, wv, *off, out=mine) is mine
+    assert (mine[:3] == 7).all() and (mine[160:] == 7).all() and torch.equal(mine[3:160], got[3:160])
+    none = svs.latent_attention_expanded(q[:9], rows, wk, wv, off[0][:1], off[1][:1])  # no sequence
+    assert not none.any() and svs.latent_attention_expanded(q[:0], rows, wk, wv, off[0][:1], off[1][:1]).shape == (0, 2, 40)
+    wrong = torch.tensor([-5, 60, 43, 500], dtype=torch.int32).cuda()  # offsets outside the arrays and falling: no result is promised, no access leaves the arrays
+    svs.latent_attention_expanded(q, rows, wk, wv, wrong, off[1])
+    svs.latent_attention_expanded(q, rows, wk, wv, off[0], wrong * 4)
+    torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+def test_expanded_prompts_in_a_graph():
+    import torch
+
+    import scalablevectorsearch_amd as svs
+
+    q, rows = torch.randn(150, 4, 96, device="cuda").half(), torch.randn(200, 128, device="cuda").half()
+    wk, wv = torch.randn(4, 64, 96, device="cuda").half() / 8, torch.randn(4, 64, 96, device="cuda").half() / 8
+    off = [torch.tensor(x, dtype=torch.int32).cuda() for x in ([0, 50, 150], [0, 90, 200])]
+    svs.latent_attention_expanded(q, rows, wk, wv, *off)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        one = svs.latent_attention_expanded(q, rows, wk, wv, *off)
+        two = svs.latent_attention_expanded(q, rows * 2, wv, wk, *off)
+    for k in range(4):
+        q.mul_(0.7)
+        off[0][1] = 60 - k
+        graph.replay()
+        assert torch.equal(one, svs.latent_attention_expanded(q, rows, wk, wv, *off)) and torch.equal(two, svs.latent_attention_expanded(q, rows * 2, wv, wk, *off)), k
+        torch.randn(100, device="cuda").sum().item()
+
+
+# ---- refusals --------------------------------------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("changes, message", [
+    (dict(struct_size=4), "struct_size"), (dict(dtype=2), "row dtype"), (dict(n_heads=3), "multiple"), (dict(n_key_heads=0), "multiple"), (dict(n_heads=0), "multiple"),
+    (dict(key_dim=0), "key_dim"), (dict(key_dim=1025), "key_dim"), (dict(value_dim=1025), "value_dim"), (dict(d_values=None, value_dim=9), "value_dim"), (dict(page_size=0), "page_size"),
+    (dict(page_size=1 << 20, max_pages=1 << 20), "page_size"), (dict(n_queries=1 << 32), "queries"), (dict(d_queries=None), "null"), (dict(d_out=None), "null"),
+    (dict(d_table=None), "null"), (dict(d_lengths=None), "null"), (dict(d_keys=None), "null"),
+])
+def test_paged_attention_refuses_before_any_device_work(changes, message):
+    _lib.build()
+    L, one, size = _lib.lib(), 256, C.c_size_t()
+    d = _lib.AttentionDesc(C.sizeof(_lib.AttentionDesc), 0, 1, 2, 4, 2, 8, 8, 10, 4, 2, 3, 3, one, 32, 8, one, 64, 32, 8, one, 64, 32, 8, one, one, None, 0.5, one, None)
+    assert L.svsx_paged_attention_workspace(C.byref(d), C.byref(size)) == _lib.SUCCESS
+    for k, v in changes.items():
+        setattr(d, k, v)
+    assert L.svsx_paged_attention_workspace(C.byref(d), C.byref(size)) == _lib.INVALID_ARGUMENT
+    assert message in L.svsx_last_error().decode()
+    assert L.svsx_paged_attention_device(C.byref(d), 256, 1 << 40, None) == _lib.INVALID_ARGUMENT
+    assert L.svsx_paged_attention_device(None, None, 0, None) == _lib.INVALID_ARGUMENT
+
+
+@pytest.mark.parametrize("changes, message", [
+    (dict(struct_size=4), "struct_size"), (dict(dtype=3), "row dtype"), (dict(n_heads=0), "n_heads"), (dict(rank=0), "rank"), (dict(rank=1000), "rank"), (dict(value_dim=0), "value_dim"),
+    (dict(nope_dim=1000), "nope_dim"), (dict(n_rows=1 << 31), "too many"), (dict(n_tokens=1 << 31), "too many"), (dict(d_queries=None), "null"), (dict(d_w_key=None), "null"),
+    (dict(d_row_offsets=None), "null"), (dict(d_rows=None), "null"), (dict(d_out=None), "null"),
+])
+def test_expanded_attention_refuses_before_any_device_work(changes, message):
+    _lib.build()
+    L, one, size = _lib.lib(), 256, C.c_size_t()
+    d = _lib.ExpandedDesc(C.sizeof(_lib.ExpandedDesc), 0, 1, 2, 10, 20, 2, 64, 32, 128, 64, one, 192, 96, one, 160, one, one, one, one, 0.1, 1, 0, one)
+    assert L.svsx_latent_expanded_workspace(C.byref(d), C.byref(size)) == _lib.SUCCESS
+    for k, v in changes.items():
+        setattr(d, k, v)
+    assert L.svsx_latent_expanded_workspace(C.byref(d), C.byref(size)) == _lib.INVALID_ARGUMENT
+    assert message in L.svsx_last_error().decode()
+    assert L.svsx_latent_expanded_device(C.byref(d), 256, 1 << 40, None) == _lib.INVALID_ARGUMENT
+    assert L.svsx_latent_expanded_device(None, None, 0, None) == _lib.INVALID_ARGUMENT
+
+
+def test_arrays_on_the_host_are_refused():
+    import torch
+
+    import scalablevectorsearch_amd as svs
+
+    _lib.build()
+    q, k, table, n = torch.zeros(1, 2, 8), torch.zeros(3, 1, 4, 8), torch.zeros(1, 1, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    for call in (lambda: svs.paged_attention(q, k, k, table, n), lambda: svs.latent_attention(q, k, table, n, 4),
+                 lambda: svs.latent_attention_expanded(q, k[0, 0], torch.zeros(2, 4, 4), torch.zeros(2, 4, 4), n, n)):
+        with pytest.raises(svs.SvsxError) as e:
+            call()
+        assert e.value.code == _lib.INVALID_ARGUMENT and "GPU" in e.value.message
+
+
+@pytest.mark.gpu
+def test_wrong_arguments_are_refused():
+    import torch
+
+    import scalablevectorsearch_amd as svs
+
+    q, keys, values, table, n = _case("float16", [20, 3], 4, 2, 64, 64, 16)
+    rows, wk, wv, off = keys[0, 0, :, :], torch.zeros(4, 32, 48, device="cuda").half(), torch.zeros(4, 32, 48, device="cuda").half(), torch.tensor([0, 2], dtype=torch.int32).cuda()
+    qe = torch.zeros(2, 4, 48, device="cuda").half()
+    att, exp = svs.paged_attention, svs.latent_attention_expanded
+    assert exp(qe, rows, wk, wv, off, off).shape == (2, 4, 32)
+    bad = [
+        lambda: att(q.double(), keys, values, table, n), lambda: att(q, keys.float(), values, table, n), lambda: att(q, keys, values.bfloat16(), table, n),
+        lambda: att(q[..., :32], keys, values, table, n), lambda: att(q[:, :3], keys, values, table, n), lambda: att(q, keys, values[:, :1], table, n),
+        lambda: att(q, keys, values, table.long(), n), lambda: att(q, keys, values, table, n.long()), lambda: att(q, keys, values, table, n[:1]),
+        lambda: att(q[:1], keys, values, table, n), lambda: att(q, keys, values, table.cpu(), n), lambda: att(q, keys, values, table, n, sequences=n[:1]),
+        lambda: att(q, keys, values, table, n, value_dim=32), lambda: att(q, keys, None, table, n, value_dim=65), lambda: att(q, keys, None, table, n, value_dim=0),
+        lambda: att(q[0], keys, values, table, n), lambda: att(q, keys.transpose(2, 3).contiguous().transpose(2, 3), values, table, n),
+        lambda: att(torch.zeros(2, 2, 2000, device="cuda"), torch.zeros(3, 1, 4, 2000, device="cuda"), None, table, n),
+        lambda: exp(qe, rows.float(), wk, wv, off, off), lambda: exp(qe[:, :3], rows, wk, wv, off, off), lambda: exp(qe, rows[:, :60], wk, wv, off, off),
+        lambda: exp(qe, rows, wk, wv[:, :, :40], off, off), lambda: exp(qe, rows, wk, wv, off, off[:1]), lambda: exp(qe, rows, wk, wv, off.long(), off.long()),
+        lambda: exp(qe, rows, wk, wv, off, off, out=torch.zeros(2, 4, 31, device="cuda").half()), lambda: exp(qe, rows.cpu(), wk, wv, off, off),
+        lambda: exp(qe[..., :16], rows, wk, wv, off, off),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(svs.SvsxError) as e:
+            call()
+        assert e.value.code == _lib.INVALID_ARGUMENT, i
