@@ -1,6 +1,7 @@
 // svsx_attention.hip -- attention of one new token over paged rows (include/svsx.h: svsx_paged_attention_device).
 #include "svsx_host.h"
-#include "svsx_paged.h"
+#include "svsx_mfma.h"
+#include <initializer_list>
 
 namespace svsx {
 namespace {
@@ -22,7 +23,7 @@ struct AttentionArgs {
 // rows of query i: its table row and how many rows there are
 __device__ __forceinline__ uint32_t rows_of(const AttentionArgs& a, uint32_t i, const int32_t** table) {
     const int32_t s = a.sequences ? a.sequences[i] : static_cast<int32_t>(i);
-    if (s < 0 || static_cast<uint32_t>(s) >= a.n_sequences) return 0;
+    if (s < 0 || static_cast<uint32_t>(s) >= a.n_sequences || a.n_pages == 0) return 0; // rows of a hole are read from page 0, and masked: there has to be one
     *table = a.table + static_cast<size_t>(s) * a.table_stride;
     const int32_t len = a.lengths[s];
     const uint32_t most = a.max_pages * a.page_size;
@@ -49,6 +50,369 @@ template <typename T> __global__ __launch_bounds__(256) void attend_head_kernel(
     T* out = static_cast<T*>(a.out) + (static_cast<size_t>(i) * a.n_heads + h) * a.dv;
     for (uint32_t c = threadIdx.x; c < a.dv; c += 256) out[c] = from_f32<T>(sm.out[0][c]);
     if (a.lse && threadIdx.x == 0) a.lse[static_cast<size_t>(i) * a.n_heads + h] = lse;
+}
+
+// ---- heads that share a key head, on the matrix units --------------------------------------------------------------------------------------------
+//
+// One wave takes 32 rows of one key head at a time for up to 16 query heads that share it; what it needs of them goes from HBM to registers once and is never
+// staged:
+//   S = K Q^T      rows x heads.  Row m of the s-th 16 x 16 product is row (m / 4) * 8 + s * 4 + m % 4 of the 32, so that lane l gets the scores of the EIGHT
+//                  CONSECUTIVE rows 8 (l / 16) .. + 7 for head l % 16.
+//   O^T = V^T P^T  columns x heads.  The lane's eight probabilities are a fragment of P^T as they are; and since it owns eight consecutive rows, it loads 8 columns
+//                  (16 bytes) of each of them and transposes that 8 x 8 block in its registers: lane l's columns are 8 (l % 16) .. + 7, the d-th product
+//                  takes the d-th of them.
+// Bound by HBM: 16 heads' products are half the matrix units' time per byte, and 32 rows' keys (of the next 32) and values are in flight per wave, three waves per SIMD.
+// The running maximum of a head is raised only when a score exceeds it by more than 2^kSlack (the accumulators are rescaled then), so the usual 32 rows cost
+// no rescaling; sums are kept per lane and joined at the end.
+//
+// A workgroup is four waves that deal the tiles of one chunk of rows among themselves.  Chunks: see plan below.
+
+constexpr int kTile = 32, kChunkUnit = 4 * kTile; // rows of a wave's tile; rows that a workgroup takes at a time
+constexpr float kSlack = 4.0f;                    // in powers of two
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+
+// Probabilities are rounded to the row type before they meet the values; float16 gets them 2^8 up, so that small ones stay normal numbers (at most 2^12 with the slack).
+template <typename T> constexpr float kLift = 0.0f;
+template <> constexpr float kLift<_Float16> = 8.0f;
+
+struct Plan {
+    float* partial;  // [slot][head][dv] sums of p v
+    float2* stats;   // [slot][head] {maximum (powers of two), sum of p}
+    int2* chunks;    // [query] {first slot, chunks}
+    uint32_t target; // slots to aim at; 0: one chunk a query and no joining
+};
+
+// Which rows a workgroup has.  Lengths are known on the device only, so every workgroup derives the same plan from them: all queries' rows in units of kChunkUnit,
+// divided over `target` slots, give the chunk; slots are dealt out query by query (at most target + n_queries of them).  False: nothing to do.
+struct Chunk {
+    uint32_t query, begin, end, slot, count;
+    const int32_t* table;
+};
+__device__ __forceinline__ bool find_chunk(const AttentionArgs& a, const Plan& plan, Chunk* c, uint32_t (&sh)[260]) {
+    if (plan.target == 0) {
+        c->query = blockIdx.x;
+        c->table = nullptr;
+        c->begin = 0;
+        c->end = rows_of(a, c->query, &c->table);
+        c->slot = 0;
+        c->count = 1;
+        return true;
+    }
+    const uint32_t t = threadIdx.x, wave = t >> 6, lane = t & 63;
+    auto units = [&](uint32_t i) {
+        const int32_t* unused;
+        return i < a.n_queries ? (rows_of(a, i, &unused) + kChunkUnit - 1) / kChunkUnit : 0u;
+    };
+    uint32_t mine = 0;
+    for (uint32_t i = t; i < a.n_queries; i += 256) mine += units(i);
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) mine += __shfl_xor(mine, off);
+    if (lane == 0) sh[wave] = mine;
+    __syncthreads();
+    const uint32_t total = sh[0] + sh[1] + sh[2] + sh[3];
+    const uint32_t size = (total + plan.target - 1) / plan.target; // units in a chunk
+    if (threadIdx.x == 0) sh[256] = 0xFFFFFFFFu;
+    uint32_t base = 0;
+    for (uint32_t first = 0; first < a.n_queries; first += 256) { // which query has this slot
+        const uint32_t i = first + t, n = size ? (units(i) + size - 1) / size : 0;
+        uint32_t incl = n;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const uint32_t u = __shfl_up(incl, off);
+            if (lane >= static_cast<uint32_t>(off)) incl += u;
+        }
+        __syncthreads();
+        if (lane == 63) sh[4 + wave] = incl;
+        __syncthreads();
+        uint32_t before = base;
+        for (uint32_t w = 0; w < wave; ++w) before += sh[4 + w];
+        const uint32_t at = before + incl - n;
+        if (n > 0 && blockIdx.x >= at && blockIdx.x < at + n) {
+            sh[256] = i;
+            sh[257] = at;
+            sh[258] = n;
+        }
+        base += sh[4] + sh[5] + sh[6] + sh[7];
+        if (base > blockIdx.x) break; // base is the same for all
+    }
+    __syncthreads();
+    if (sh[256] == 0xFFFFFFFFu) return false;
+    c->query = sh[256];
+    c->slot = blockIdx.x;
+    c->count = sh[258];
+    c->table = nullptr;
+    const uint32_t rows = rows_of(a, c->query, &c->table), k = blockIdx.x - sh[257];
+    c->begin = k * size * kChunkUnit;
+    c->end = min(rows, (k + 1) * size * kChunkUnit);
+    if (k == 0 && threadIdx.x == 0 && blockIdx.y == 0) plan.chunks[c->query] = make_int2(static_cast<int>(blockIdx.x), static_cast<int>(c->count));
+    return true;
+}
+
+// 2^x; the hardware's instruction, denormal results are zero
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Where a lane's rows are: pages of the two key rows and the eight value rows.  Page8: page_size is a multiple of 8, so eight consecutive rows share a page.
+template <bool Page8> struct TileRows {
+    int32_t key[Page8 ? 1 : 2], value[Page8 ? 1 : 8];
+    uint32_t key_at[Page8 ? 1 : 2], value_at[Page8 ? 1 : 8]; // row within the page
+};
+
+template <typename T, int KS, int VB, bool Wide, bool Page8>
+__global__ __launch_bounds__(256) void attend_group_kernel(const AttentionArgs a, const Plan plan, const Divider by_page) {
+    __shared__ uint32_t sh[260];
+    __shared__ float join[2][VB * 32 + 2][64];
+    Chunk c;
+    if (!find_chunk(a, plan, &c, sh)) return;
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, quad = lane >> 4;
+    const uint32_t tiles = (a.group + 15) / 16, g = blockIdx.y / tiles, h0 = (blockIdx.y % tiles) * 16; // key head; first head within its group
+    const uint32_t heads = min(16u, a.group - h0), head = g * a.group + h0 + n;
+    const bool live = n < heads;
+
+    Frag<T> q[KS];
+    {
+        const T* row = static_cast<const T*>(a.queries) + c.query * a.query_stride + (live ? head : g * a.group) * a.query_head_stride;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            q[k] = load_frag<T, false>(row, k * 32 + quad * 8, a.dk);
+            if (!live) q[k] = Frag<T>{};
+        }
+    }
+    const T* keys = static_cast<const T*>(a.keys) + g * a.key_head_stride;
+    const T* values = static_cast<const T*>(a.values) + g * a.value_head_stride;
+    const float scale = a.scale * kLog2e;
+
+    f32x4 o[VB * 8];
+#pragma unroll
+    for (int i = 0; i < VB * 8; ++i) o[i] = f32x4{0, 0, 0, 0};
+    float top = -INFINITY, sum = 0.0f; // the maximum that probabilities are relative to, in powers of two; this lane's share of their sum
+
+    const uint32_t last = c.end - 1; // rows behind the end are looked up at the last one, and masked
+    auto find = [&](uint32_t base) {
+        TileRows<Page8> r;
+        if constexpr (Page8) {
+            r.key[0] = c.table[by_page(min(base + (n >> 2) * 8, last), &r.key_at[0])];
+            r.value[0] = c.table[by_page(min(base + quad * 8, last), &r.value_at[0])];
+            // the page's row of the block's first row: `last` may be in its middle
+            r.key_at[0] &= ~7u;
+            r.value_at[0] &= ~7u;
+        } else {
+#pragma unroll
+            for (int s = 0; s < 2; ++s) r.key[s] = c.table[by_page(min(base + (n >> 2) * 8 + s * 4 + (n & 3), last), &r.key_at[s])];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) r.value[j] = c.table[by_page(min(base + quad * 8 + j, last), &r.value_at[j])];
+        }
+        return r;
+    };
+    auto is_page = [&](int32_t p) { return static_cast<uint32_t>(p) < a.n_pages; }; // negative ones are large
+    auto load_keys = [&](const TileRows<Page8>& r, Frag<T> (&k)[2][KS]) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const int32_t p = Page8 ? r.key[0] : r.key[Page8 ? 0 : s];
+            const uint32_t at = Page8 ? r.key_at[0] + s * 4 + (n & 3) : r.key_at[Page8 ? 0 : s];
+            const T* row = keys + (is_page(p) ? static_cast<size_t>(p) : 0) * a.key_page_stride + at * a.key_row_stride;
+#pragma unroll
+            for (int i = 0; i < KS; ++i) k[s][i] = load_frag<T, Wide>(row, i * 32 + quad * 8, a.dk);
+        }
+    };
+
+    uint32_t base = c.begin + wave * kTile;
+    Frag<T> k[2][KS];
+    TileRows<Page8> here, next;
+    if (base < c.end) {
+        here = find(base);
+        load_keys(here, k);
+        next = find(base + kChunkUnit);
+    }
+    for (; base < c.end; base += kChunkUnit) {
+        Frag<T> v[VB][8];
+        uint32_t mask = 0; // which of the lane's eight rows are there
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int32_t p = Page8 ? here.value[0] : here.value[Page8 ? 0 : j];
+            const uint32_t at = Page8 ? here.value_at[0] + j : here.value_at[Page8 ? 0 : j];
+            if (base + quad * 8 + j < c.end && is_page(p)) mask |= 1u << j;
+            const T* row = values + (is_page(p) ? static_cast<size_t>(p) : 0) * a.value_page_stride + at * a.value_row_stride;
+#pragma unroll
+            for (int b = 0; b < VB; ++b) v[b][j] = load_frag<T, Wide>(row, b * 128 + n * 8, a.dv);
+        }
+        f32x4 s[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+            s[0] = product16(k[0][i], q[i], s[0]);
+            s[1] = product16(k[1][i], q[i], s[1]);
+        }
+        if (base + kChunkUnit < c.end) {
+            here = next;
+            load_keys(here, k);
+            next = find(base + 2 * kChunkUnit);
+        }
+        float p[8], most = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) p[j] = s[j >> 2][j & 3] * scale;
+        if (!__all(mask == 0xFFu)) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const bool there = mask >> j & 1;
+                p[j] = there ? p[j] : -INFINITY;
+#pragma unroll
+                for (int b = 0; b < VB; ++b) // what a page holds behind the last row is not defined: zero times it need not be zero
+                    if (!there) v[b][j] = Frag<T>{};
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) most = fmaxf(most, p[j]);
+        most = fmaxf(most, __shfl_xor(most, 16));
+        most = fmaxf(most, __shfl_xor(most, 32));
+        if (__any(most > top + kSlack)) { // also the first tile: top is -inf
+            const float raised = fmaxf(top, most), shrink = top == -INFINITY ? 0.0f : exp2_fast(top - raised);
+            top = raised;
+            sum *= shrink;
+#pragma unroll
+            for (int i = 0; i < VB * 8; ++i) o[i] *= shrink;
+        }
+        const float from = (top == -INFINITY ? 0.0f : top) - kLift<T>;
+        Frag<T> w;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            p[j] = exp2_fast(p[j] - from);
+            sum += p[j];
+            w[j] = from_f32<T>(p[j]);
+        }
+#pragma unroll
+        for (int b = 0; b < VB; ++b) {
+#pragma unroll
+            for (int d = 0; d < 8; ++d) {
+                Frag<T> column;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) column[j] = v[b][j][d];
+                o[b * 8 + d] = product16(column, w, o[b * 8 + d]);
+            }
+        }
+    }
+    sum += __shfl_xor(sum, 16);
+    sum += __shfl_xor(sum, 32);
+    top -= kLift<T>; // sums are of 2^(score - top)
+
+    // the four waves' results, two at a time: waves 2 and 3 into 0 and 1, then 1 into 0
+#pragma unroll
+    for (int half = 2; half >= 1; half >>= 1) {
+        __syncthreads();
+        if (wave >= static_cast<uint32_t>(half) && wave < 2u * half) {
+#pragma unroll
+            for (int i = 0; i < VB * 32; ++i) join[wave - half][i][lane] = o[i >> 2][i & 3];
+            join[wave - half][VB * 32][lane] = top;
+            join[wave - half][VB * 32 + 1][lane] = sum;
+        }
+        __syncthreads();
+        if (wave < static_cast<uint32_t>(half)) {
+            const float other = join[wave][VB * 32][lane], all = fmaxf(top, other);
+            const float wa = top == -INFINITY ? 0.0f : exp2_fast(top - all), wb = other == -INFINITY ? 0.0f : exp2_fast(other - all);
+            sum = sum * wa + join[wave][VB * 32 + 1][lane] * wb;
+            top = all;
+#pragma unroll
+            for (int i = 0; i < VB * 32; ++i) o[i >> 2][i & 3] = o[i >> 2][i & 3] * wa + join[wave][i][lane] * wb;
+        }
+    }
+    if (wave != 0 || !live) return;
+    // o[b * 8 + d][r]: column b * 128 + (quad * 4 + r) * 8 + d of head n
+    if (c.count > 1) {
+        const size_t at = static_cast<size_t>(c.slot) * a.n_heads + head;
+        if (quad == 0) plan.stats[at] = make_float2(top, sum);
+        float* out = plan.partial + at * a.dv;
+#pragma unroll
+        for (int b = 0; b < VB; ++b)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int d = 0; d < 8; ++d) {
+                    const uint32_t col = b * 128 + (quad * 4 + r) * 8 + d;
+                    if (col < a.dv) out[col] = o[b * 8 + d][r];
+                }
+        return;
+    }
+    const size_t at = static_cast<size_t>(c.query) * a.n_heads + head;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    T* out = static_cast<T*>(a.out) + at * a.dv;
+#pragma unroll
+    for (int b = 0; b < VB; ++b)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const uint32_t col = b * 128 + (quad * 4 + r) * 8;
+            Frag<T> f;
+#pragma unroll
+            for (int d = 0; d < 8; ++d) f[d] = from_f32<T>(o[b * 8 + d][r] * inv);
+            if (a.dv % 8 == 0) {
+                if (col < a.dv) *reinterpret_cast<Frag<T>*>(out + col) = f;
+            } else {
+#pragma unroll
+                for (uint32_t d = 0; d < 8; ++d)
+                    if (col + d < a.dv) out[col + d] = f[d];
+            }
+        }
+    if (a.lse && quad == 0) a.lse[at] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
+}
+
+// The chunks of a query joined: out = sum_k 2^(top_k - top) o_k / sum_k 2^(top_k - top) sum_k.  One workgroup per head and query; queries of one chunk are done already,
+// queries without rows (no slot is theirs) get their zeros here.
+template <typename T> __global__ __launch_bounds__(128) void join_kernel(const AttentionArgs a, const Plan plan) {
+    __shared__ float weight[128];
+    __shared__ float wide[2][2];
+    const uint32_t h = blockIdx.x, i = blockIdx.y, t = threadIdx.x;
+    const size_t at = static_cast<size_t>(i) * a.n_heads + h;
+    T* out = static_cast<T*>(a.out) + at * a.dv;
+    const int32_t* table;
+    if (rows_of(a, i, &table) == 0) {
+        for (uint32_t col = t; col < a.dv; col += 128) out[col] = from_f32<T>(0.0f);
+        if (a.lse && t == 0) a.lse[at] = -INFINITY;
+        return;
+    }
+    const int2 mine = plan.chunks[i];
+    if (mine.y == 1) return;
+    const uint32_t n = static_cast<uint32_t>(mine.y);
+    const float2* stats = plan.stats + static_cast<size_t>(mine.x) * a.n_heads + h;
+    float top = -INFINITY;
+    for (uint32_t k = t; k < n; k += 128) top = fmaxf(top, stats[static_cast<size_t>(k) * a.n_heads].x);
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
+    if ((t & 63) == 0) wide[0][t >> 6] = top;
+    __syncthreads();
+    top = fmaxf(wide[0][0], wide[0][1]);
+    float sum = 0.0f, acc[8] = {};
+    const float* partial = plan.partial + (static_cast<size_t>(mine.x) * a.n_heads + h) * a.dv;
+    const size_t step = static_cast<size_t>(a.n_heads) * a.dv;
+    for (uint32_t first = 0; first < n; first += 128) {
+        __syncthreads();
+        if (first + t < n) {
+            const float2 st = stats[static_cast<size_t>(first + t) * a.n_heads];
+            const float w = st.x == -INFINITY ? 0.0f : exp2_fast(st.x - top);
+            weight[t] = w;
+            sum += w * st.y;
+        }
+        __syncthreads();
+        const uint32_t some = min(128u, n - first);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            const uint32_t col = t + 128 * c;
+            if (col >= a.dv) break;
+            const float* from = partial + first * step + col;
+            float x = acc[c];
+#pragma unroll 4
+            for (uint32_t k = 0; k < some; ++k) x = fmaf(weight[k], from[k * step], x);
+            acc[c] = x;
+        }
+    }
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off);
+    if ((t & 63) == 0) wide[1][t >> 6] = sum;
+    __syncthreads();
+    sum = wide[1][0] + wide[1][1];
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+        const uint32_t col = t + 128 * c;
+        if (col < a.dv) out[col] = from_f32<T>(acc[c] * inv);
+    }
+    if (a.lse && t == 0) a.lse[at] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
 }
 
 int check_attention(const svsx_attention_desc* d, AttentionArgs* a) {
@@ -100,6 +464,81 @@ int check_attention(const svsx_attention_desc* d, AttentionArgs* a) {
     return SVSX_SUCCESS;
 }
 
+// How a call is answered; decided from sizes, types, strides and addresses alone.
+struct Route {
+    bool group;       // on the matrix units; else one workgroup per head (rows beyond 256 columns)
+    bool wide, page8;
+    int ks, vb;
+    uint32_t slots, target, y;
+    size_t stats_at, chunks_at, bytes;
+};
+
+// Four workgroups for every compute unit: enough to even out ragged batches.
+constexpr uint32_t kTargetGroups = 1024;
+
+Route route_of(const AttentionArgs& a, size_t es) {
+    Route r = {};
+    r.group = a.dk <= 256 && a.dv <= 256;
+    if (!r.group) return r;
+    auto aligned = [&](std::initializer_list<size_t> strides, const void* p) {
+        size_t all = reinterpret_cast<size_t>(p);
+        for (size_t x : strides) all |= x * es;
+        return all % 16 == 0;
+    };
+    r.wide = a.dk % 8 == 0 && a.dv % 8 == 0 && aligned({a.key_page_stride, a.key_head_stride, a.key_row_stride}, a.keys) &&
+             aligned({a.value_page_stride, a.value_head_stride, a.value_row_stride}, a.values);
+    r.page8 = a.page_size % 8 == 0;
+    r.vb = a.dv > 128 || a.dk > 128 ? 2 : 1;
+    r.ks = !r.wide ? (r.vb == 2 ? 8 : 4) : a.dk > 192 ? 8 : a.dk > 128 || r.vb == 2 ? 6 : a.dk > 96 ? 4 : a.dk > 64 ? 3 : 2;
+    r.y = a.n_key_heads * ((a.group + 15) / 16);
+    // one chunk a query where queries alone fill the machine, or where no query can have more rows than a few tiles
+    const uint64_t groups = static_cast<uint64_t>(a.n_queries) * r.y, most = static_cast<uint64_t>(a.max_pages) * a.page_size;
+    if (groups >= 4 * kTargetGroups || most <= kChunkUnit) {
+        r.slots = a.n_queries;
+        return r;
+    }
+    r.target = std::max(1u, kTargetGroups / r.y);
+    r.slots = static_cast<uint32_t>(std::min<uint64_t>(static_cast<uint64_t>(r.target) + a.n_queries, a.n_queries * ((most + kChunkUnit - 1) / kChunkUnit)));
+    const size_t parts = static_cast<size_t>(r.slots) * a.n_heads;
+    r.stats_at = (parts * a.dv * 4 + 15) / 16 * 16;
+    r.chunks_at = r.stats_at + parts * 8;
+    r.bytes = r.chunks_at + static_cast<size_t>(a.n_queries) * 8;
+    return r;
+}
+
+template <typename T> hipError_t launch_group(const AttentionArgs& a, const Route& r, void* workspace, hipStream_t stream) {
+    Plan plan = {};
+    plan.target = r.target;
+    if (r.target) {
+        char* base = static_cast<char*>(workspace);
+        plan.partial = reinterpret_cast<float*>(base);
+        plan.stats = reinterpret_cast<float2*>(base + r.stats_at);
+        plan.chunks = reinterpret_cast<int2*>(base + r.chunks_at);
+    }
+    typedef void (*Kernel)(const AttentionArgs, const Plan, const Divider);
+    Kernel kernel = nullptr;
+#define SVSX_GROUP(KS, VB, WIDE) \
+    if (r.ks == KS && r.vb == VB && r.wide == WIDE) kernel = r.page8 ? attend_group_kernel<T, KS, VB, WIDE, true> : attend_group_kernel<T, KS, VB, WIDE, false>;
+    SVSX_GROUP(2, 1, true)
+    SVSX_GROUP(3, 1, true)
+    SVSX_GROUP(4, 1, true)
+    SVSX_GROUP(6, 2, true)
+    SVSX_GROUP(8, 2, true)
+    SVSX_GROUP(4, 1, false)
+    SVSX_GROUP(8, 2, false)
+#undef SVSX_GROUP
+    if (!kernel) return hipErrorInvalidValue;
+    hipLaunchKernelGGL(kernel, dim3(r.slots, r.y), dim3(256), 0, stream, a, plan, divider(a.page_size));
+    if (r.target) hipLaunchKernelGGL(join_kernel<T>, dim3(a.n_heads, a.n_queries), dim3(128), 0, stream, a, plan);
+    return hipGetLastError();
+}
+
+template <typename T> hipError_t launch_attention(const AttentionArgs& a, const Route& r, void* workspace, hipStream_t stream) {
+    if (r.group) return launch_group<T>(a, r, workspace, stream);
+    hipLaunchKernelGGL(attend_head_kernel<T>, dim3(a.n_heads, a.n_queries), dim3(256), 0, stream, a);
+    return hipGetLastError();
+}
+
 } // namespace
 } // namespace svsx
 
@@ -109,21 +548,23 @@ int svsx_paged_attention_workspace(const svsx_attention_desc* desc, size_t* byte
     AttentionArgs a;
     if (const int rc = check_attention(desc, &a)) return rc;
     if (!bytes) return fail(SVSX_INVALID_ARGUMENT, "null argument");
-    *bytes = 0;
+    *bytes = a.n_queries ? route_of(a, paged_dtype_size(desc->dtype)).bytes : 0;
     return SVSX_SUCCESS;
 }
 
 int svsx_paged_attention_device(const svsx_attention_desc* desc, void* d_workspace, size_t workspace_bytes, void* hip_stream) {
-    (void)d_workspace;
-    (void)workspace_bytes;
     AttentionArgs a;
     if (const int rc = check_attention(desc, &a)) return rc;
     if (a.n_queries == 0) return SVSX_SUCCESS;
+    const Route r = route_of(a, paged_dtype_size(desc->dtype));
+    if (r.bytes > 0 && (!d_workspace || workspace_bytes < r.bytes || reinterpret_cast<uintptr_t>(d_workspace) % 16 != 0))
+        return fail(SVSX_INVALID_ARGUMENT, "a workspace of %zu bytes, aligned to 16, is needed", r.bytes);
     DeviceScope on(desc->device);
     if (on.error != hipSuccess) return fail(SVSX_RUNTIME_ERROR, "hipSetDevice(%d) failed: %s", desc->device, hipGetErrorString(on.error));
-    auto kernel = desc->dtype == SVSX_F32 ? attend_head_kernel<float> : desc->dtype == SVSX_F16 ? attend_head_kernel<_Float16> : attend_head_kernel<bf16_t>;
-    hipLaunchKernelGGL(kernel, dim3(a.n_heads, a.n_queries), dim3(256), 0, static_cast<hipStream_t>(hip_stream), a);
-    const hipError_t e = hipGetLastError();
+    const hipStream_t s = static_cast<hipStream_t>(hip_stream);
+    const hipError_t e = desc->dtype == SVSX_F32   ? launch_attention<float>(a, r, d_workspace, s)
+                         : desc->dtype == SVSX_F16 ? launch_attention<_Float16>(a, r, d_workspace, s)
+                                                   : launch_attention<bf16_t>(a, r, d_workspace, s);
     return e == hipSuccess ? SVSX_SUCCESS : fail(SVSX_RUNTIME_ERROR, "attention launch failed: %s", hipGetErrorString(e));
 }
 
