@@ -18,6 +18,7 @@ struct AttentionArgs {
     size_t query_stride, query_head_stride, key_page_stride, key_head_stride, key_row_stride, value_page_stride, value_head_stride, value_row_stride, table_stride;
     uint32_t n_queries, n_heads, group, n_key_heads, dk, dv, n_pages, page_size, n_sequences, max_pages;
     float scale;
+    int shared; // rows are keys and values at once
 };
 
 // rows of query i: its table row and how many rows there are
@@ -80,9 +81,10 @@ struct Plan {
     float2* stats;   // [slot][head] {maximum (powers of two), sum of p}
     int2* chunks;    // [query] {first slot, chunks}
     uint32_t target; // slots to aim at; 0: one chunk a query and no joining
+    uint32_t unit;   // rows that a workgroup takes at a time
 };
 
-// Which rows a workgroup has.  Lengths are known on the device only, so every workgroup derives the same plan from them: all queries' rows in units of kChunkUnit,
+// Which rows a workgroup has.  Lengths are known on the device only, so every workgroup derives the same plan from them: all queries' rows in units of plan.unit,
 // divided over `target` slots, give the chunk; slots are dealt out query by query (at most target + n_queries of them).  False: nothing to do.
 struct Chunk {
     uint32_t query, begin, end, slot, count;
@@ -93,7 +95,7 @@ __device__ __forceinline__ bool find_chunk(const AttentionArgs& a, const Plan& p
         c->query = blockIdx.x;
         c->table = nullptr;
         c->begin = 0;
-        c->end = rows_of(a, c->query, &c->table);
+        c->end = __builtin_amdgcn_readfirstlane(rows_of(a, c->query, &c->table));
         c->slot = 0;
         c->count = 1;
         return true;
@@ -101,7 +103,7 @@ __device__ __forceinline__ bool find_chunk(const AttentionArgs& a, const Plan& p
     const uint32_t t = threadIdx.x, wave = t >> 6, lane = t & 63;
     auto units = [&](uint32_t i) {
         const int32_t* unused;
-        return i < a.n_queries ? (rows_of(a, i, &unused) + kChunkUnit - 1) / kChunkUnit : 0u;
+        return i < a.n_queries ? (rows_of(a, i, &unused) + plan.unit - 1) / plan.unit : 0u;
     };
     uint32_t mine = 0;
     for (uint32_t i = t; i < a.n_queries; i += 256) mine += units(i);
@@ -137,13 +139,13 @@ __device__ __forceinline__ bool find_chunk(const AttentionArgs& a, const Plan& p
     }
     __syncthreads();
     if (sh[256] == 0xFFFFFFFFu) return false;
-    c->query = sh[256];
+    c->query = __builtin_amdgcn_readfirstlane(sh[256]); // the same for all: in scalar registers, so that loops over it are too
     c->slot = blockIdx.x;
-    c->count = sh[258];
+    c->count = __builtin_amdgcn_readfirstlane(sh[258]);
     c->table = nullptr;
-    const uint32_t rows = rows_of(a, c->query, &c->table), k = blockIdx.x - sh[257];
-    c->begin = k * size * kChunkUnit;
-    c->end = min(rows, (k + 1) * size * kChunkUnit);
+    const uint32_t rows = rows_of(a, c->query, &c->table), k = blockIdx.x - __builtin_amdgcn_readfirstlane(sh[257]);
+    c->begin = __builtin_amdgcn_readfirstlane(k * size * plan.unit);
+    c->end = __builtin_amdgcn_readfirstlane(min(rows, (k + 1) * size * plan.unit));
     if (k == 0 && threadIdx.x == 0 && blockIdx.y == 0) plan.chunks[c->query] = make_int2(static_cast<int>(blockIdx.x), static_cast<int>(c->count));
     return true;
 }
@@ -158,7 +160,7 @@ template <bool Page8> struct TileRows {
 };
 
 template <typename T, int KS, int VB, bool Wide, bool Page8>
-__global__ __launch_bounds__(256) void attend_group_kernel(const AttentionArgs a, const Plan plan, const Divider by_page) {
+__global__ __launch_bounds__(256, 2) void attend_group_kernel(const AttentionArgs a, const Plan plan, const Divider by_page) {
     __shared__ uint32_t sh[260];
     __shared__ float join[2][VB * 32 + 2][64];
     Chunk c;
@@ -352,6 +354,343 @@ __global__ __launch_bounds__(256) void attend_group_kernel(const AttentionArgs a
     if (a.lse && quad == 0) a.lse[at] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
 }
 
+// ---- rows that are key and value at once, for many heads ------------------------------------------------------------------------------------------
+//
+// Latent rows: every head reads the same row, as key and (its first columns) as value, so 64 heads make 240 operations of each byte and the rows have to be
+// read from HBM once for all of them.  A workgroup of four waves brings 64 rows into LDS (straight from HBM, two buffers: the next 64 arrive while these are worked on) and
+// takes up to 64 heads over them:
+//   S = K Q^T     wave w takes 16 or 32 of the rows for 16 or 32 of the heads; its queries stay in registers
+//   maximum of the 64 rows per head through LDS; P, rounded to the row type, through LDS
+//   O^T = V^T P^T wave w takes a quarter of the value columns for all rows and heads; the transposed fragments come from gfx950's transposing LDS reads
+// (float32 rows: single words).  No sums are joined between waves but that of the probabilities.
+// LDS holds a row as 16-byte words in planes of 64 words (1 KB a row) and a narrow plane for the rest, word j of row r at j ^ swizzle(r): neither the 16 rows of a key
+// fragment nor the 16 half-words of a transposed one meet in a bank.
+// LDS reads bound it at 64 heads (248 KB per 64 rows against 2176 cycles of products), HBM at 16.
+
+constexpr int kRowTile = 64;
+
+template <typename T, int KS, int HT, int DT> struct RowsLayout { // KS: 32-column steps of a key row; HT: 16-head tiles; DT: 16-column value tiles of a wave
+    static constexpr int kWords = KS * 32 * sizeof(T) / 16;                    // 16-byte words in a row
+    static constexpr int kPlanes = kWords < 64 ? 1 : kWords / 64, kTail = kWords < 64 ? 0 : kWords % 64;
+    static constexpr int kTileBytes = kRowTile * 16 * (kPlanes * 64 + kTail);
+    static constexpr int kBuffers = sizeof(T) == 2 ? 2 : 1;                    // float32 rows: one buffer is 144 KB
+    static constexpr int kProbBytes = HT * 16 * kRowTile * sizeof(T);
+    static constexpr int kHeadsPerWave = HT == 1 ? 1 : 2, kTilesPerWave = HT == 4 ? 2 : 1; // of 16 heads, of 16 rows
+    static constexpr int kParts = 4 / kTilesPerWave;                           // waves that share a head's rows
+    static constexpr int kStatBytes = kParts * HT * 16 * 4;
+    static constexpr int kBytes = kBuffers * kTileBytes + kProbBytes + kStatBytes + 64;
+    static_assert(kTail == 0 || kTail == 8 || kTail == 16, "a narrow plane of 8 or 16 words");
+    static_assert(kBytes <= 160 * 1024 - 1088, "LDS");
+    // byte of word j of row r
+    static __device__ __forceinline__ uint32_t at(uint32_t r, uint32_t j) {
+        if (kTail > 0 && j >= kPlanes * 64) return kRowTile * 1024 * kPlanes + r * (kTail * 16) + ((j - kPlanes * 64) ^ narrow(r)) * 16;
+        return (j >> 6) * (kRowTile * 1024) + r * 1024 + ((j & 63) ^ swizzle(r)) * 16;
+    }
+    // word `lane_part | j` of the row whose word `lane_part` is at byte `first` (j is a constant that shares no bit with lane_part, which is below 16 and in the first plane)
+    static __device__ __forceinline__ uint32_t wide(uint32_t first, uint32_t j) { return (first ^ (j & 15) << 4) + (j >> 4 & 3) * 256 + (j >> 6) * (kRowTile * 1024); }
+    // rows r and r + 8 of four consecutive ones land in different pairs of words, all 16 rows in different words
+    static __device__ __forceinline__ uint32_t swizzle(uint32_t r) { return (r & 3) << 1 | (r >> 3 & 1) << 3 | (r >> 2 & 1); }
+    static __device__ __forceinline__ uint32_t narrow(uint32_t r) { return kTail == 8 ? r >> 1 & 7 : r & 15; }
+};
+
+#pragma clang diagnostic ignored "-Winline-asm" // m0 is a reserved register; the compiler is told that it changes
+// 16 bytes per lane from base + offset to LDS at `to` + 16 * lane; not waited for (direct_wait).
+__device__ __forceinline__ void direct_load(const void* base, uint32_t offset, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory", "m0");
+}
+__device__ __forceinline__ void direct_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// a barrier for what went through LDS: loads from HBM stay in flight over it
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+typedef __attribute__((address_space(3))) unsigned char lds_byte;
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+template <typename T, int KS, int HT, int DT> __global__ __launch_bounds__(256, 1) void attend_rows_kernel(const AttentionArgs a, const Plan plan, const Divider by_page) {
+    typedef RowsLayout<T, KS, HT, DT> L;
+    extern __shared__ __align__(16) unsigned char lds[];
+    __shared__ uint32_t sh[260];
+    Chunk c;
+    if (!find_chunk(a, plan, &c, sh)) return;
+    constexpr int kElems = 16 / sizeof(T); // elements in a 16-byte word
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, quad = lane >> 4;
+    const uint32_t groups = (a.group + HT * 16 - 1) / (HT * 16), g = blockIdx.y / groups, h0 = (blockIdx.y % groups) * (HT * 16);
+    const uint32_t heads = min(static_cast<uint32_t>(HT * 16), a.group - h0);
+    unsigned char* probs = lds + L::kBuffers * L::kTileBytes;
+    float* parts = reinterpret_cast<float*>(probs + L::kProbBytes);
+    uint32_t* masks = reinterpret_cast<uint32_t*>(probs + L::kProbBytes + L::kStatBytes); // [buffer][wave]: which of the wave's 16 rows are there
+    const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_byte*)lds));
+
+    const uint32_t words = a.dk / kElems; // of a row in memory; what LDS holds beyond them has to be finite
+
+    // the wave's queries: heads of tiles ht0 .., rows of tiles rt0 ..; through LDS, zeros where there is no head or column
+    const uint32_t ht0 = HT == 4 ? (wave & 1) * 2 : 0, rt0 = HT == 4 ? (wave >> 1) * 2 : wave, part = HT == 4 ? wave >> 1 : wave;
+    static_assert(HT * 16 * KS * 32 * sizeof(T) <= L::kBuffers * L::kTileBytes, "LDS");
+    Frag<T> q[L::kHeadsPerWave][KS];
+    {
+        T* stage = reinterpret_cast<T*>(lds);
+        const T* from = static_cast<const T*>(a.queries) + c.query * a.query_stride + (g * a.group + h0) * a.query_head_stride;
+        for (uint32_t h = wave; h < HT * 16; h += 4)
+            for (uint32_t col = lane; col < KS * 32; col += 64) stage[h * (KS * 32) + col] = h < heads && col < a.dk ? from[h * a.query_head_stride + col] : from_f32<T>(0.0f);
+        __syncthreads();
+#pragma unroll
+        for (int x = 0; x < L::kHeadsPerWave; ++x)
+#pragma unroll
+            for (int k = 0; k < KS; ++k) q[x][k] = *reinterpret_cast<const Frag<T>*>(stage + ((ht0 + x) * 16 + n) * (KS * 32) + k * 32 + quad * 8);
+        __syncthreads();
+    }
+    if (words < static_cast<uint32_t>(L::kWords)) {
+        for (uint32_t i = threadIdx.x; i < L::kBuffers * L::kTileBytes / 16; i += 256) reinterpret_cast<uint4*>(lds)[i] = make_uint4(0, 0, 0, 0);
+        __syncthreads();
+    }
+    f32x4 o[HT][DT];
+#pragma unroll
+    for (int x = 0; x < HT; ++x)
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[x][d] = f32x4{0, 0, 0, 0};
+    float top[HT], sum[L::kHeadsPerWave] = {};
+#pragma unroll
+    for (int x = 0; x < HT; ++x) top[x] = -INFINITY;
+    const float scale = a.scale * kLog2e;
+    const T* keys = static_cast<const T*>(a.keys) + g * a.key_head_stride;
+
+    // rows that this wave brings in: 16 wave + n of a tile; one lane of four looks a row up
+    const T* row = keys;
+    uint32_t there = 0;
+    auto find = [&](uint32_t base) {
+        const uint32_t r = base + wave * 16 + n;
+        uint32_t at;
+        const int32_t p = c.table[by_page(min(r, c.end - 1), &at)];
+        const bool page = static_cast<uint32_t>(p) < a.n_pages;
+        row = keys + (page ? static_cast<size_t>(p) : 0) * a.key_page_stride + at * a.key_row_stride;
+        there = static_cast<uint32_t>(__ballot(page && r < c.end)) & 0xFFFFu;
+    };
+    auto bring = [&](uint32_t buffer) {
+        const uint32_t to = lds0 + buffer * L::kTileBytes;
+        const uint64_t addr = reinterpret_cast<uint64_t>(row);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const uint64_t base = static_cast<uint64_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(addr >> 32), r)) << 32 |
+                                  static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(addr), r));
+#pragma unroll
+            for (int plane = 0; plane < L::kPlanes; ++plane) { // LDS is written lane by lane: the swizzle is in which word a lane fetches
+                const uint32_t word = plane * 64 + (lane ^ L::swizzle(r));
+                if (words >= (plane + 1) * 64u || word < words) direct_load(reinterpret_cast<const void*>(base), word * 16, to + plane * (kRowTile * 1024) + (wave * 16 + r) * 1024);
+            }
+        }
+        if constexpr (L::kTail > 0) {
+            constexpr int kRows = 64 / L::kTail; // rows in one go
+#pragma unroll
+            for (int r = 0; r < 16; r += kRows) {
+                const uint32_t mine = r + lane / L::kTail;
+                const uint64_t base = static_cast<uint64_t>(__shfl(static_cast<uint32_t>(addr >> 32), mine)) << 32 | __shfl(static_cast<uint32_t>(addr), mine);
+                const uint32_t word = L::kPlanes * 64 + (lane % L::kTail ^ L::narrow(mine));
+                const void* from = reinterpret_cast<const unsigned char*>(base) + word * 16;
+                const uint32_t dst = to + kRowTile * 1024 * L::kPlanes + (wave * 16 + r) * (L::kTail * 16);
+                if (word < words) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"(from) : "memory", "m0");
+            }
+        }
+    };
+    // once the rows are there: rows that are not to be seen become zeros (a weight of zero times what a page holds behind the last row need not be zero)
+    auto settle = [&](uint32_t buffer, uint32_t mask) {
+        direct_wait();
+        if (mask != 0xFFFFu) {
+            unsigned char* tile = lds + buffer * L::kTileBytes;
+            for (uint32_t r = 0; r < 16; ++r)
+                if (!(mask >> r & 1))
+                    for (uint32_t j = lane; j < static_cast<uint32_t>(L::kWords); j += 64) *reinterpret_cast<uint4*>(tile + L::at(wave * 16 + r, j)) = make_uint4(0, 0, 0, 0);
+        }
+        if (lane == 0) masks[buffer * 4 + wave] = mask;
+    };
+
+    uint32_t now = 0, mask = 0;
+    if (c.begin < c.end) {
+        find(c.begin);
+        bring(0);
+        mask = there;
+        find(c.begin + kRowTile);
+        settle(0, mask);
+        lds_barrier();
+    }
+    for (uint32_t base = c.begin; base < c.end; base += kRowTile) {
+        const bool more = base + kRowTile < c.end;
+        if (L::kBuffers == 2 && more) {
+            bring(now ^ 1);
+            mask = there;
+            find(base + 2 * kRowTile);
+        }
+        const unsigned char* tile = lds + now * L::kTileBytes;
+        f32x4 s[L::kTilesPerWave][L::kHeadsPerWave];
+#pragma unroll
+        for (int t = 0; t < L::kTilesPerWave; ++t)
+#pragma unroll
+            for (int x = 0; x < L::kHeadsPerWave; ++x) s[t][x] = f32x4{0, 0, 0, 0};
+        uint32_t key_at[L::kTilesPerWave], tail_at[L::kTilesPerWave]; // this lane's first word of its rows
+        constexpr int kStep = 2 * sizeof(T);                          // words in 32 columns
+#pragma unroll
+        for (int t = 0; t < L::kTilesPerWave; ++t) {
+            key_at[t] = L::at((rt0 + t) * 16 + n, quad * (kStep / 4));
+            tail_at[t] = L::kTail ? L::at((rt0 + t) * 16 + n, L::kPlanes * 64 + quad * (kStep / 4)) : 0;
+        }
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int t = 0; t < L::kTilesPerWave; ++t) {
+                const bool tail = k * kStep >= L::kPlanes * 64;
+                auto word = [&](uint32_t j) { return tile + (tail ? tail_at[t] ^ (j - L::kPlanes * 64) << 4 : L::wide(key_at[t], j)); };
+                Frag<T> f;
+                if constexpr (sizeof(T) == 2) {
+                    f = *reinterpret_cast<const Frag<T>*>(word(k * kStep));
+                } else {
+                    *reinterpret_cast<f32x4*>(&f) = *reinterpret_cast<const f32x4*>(word(k * kStep));
+                    *(reinterpret_cast<f32x4*>(&f) + 1) = *reinterpret_cast<const f32x4*>(word(k * kStep + 1));
+                }
+#pragma unroll
+                for (int x = 0; x < L::kHeadsPerWave; ++x) s[t][x] = product16(f, q[x][k], s[t][x]);
+            }
+        // lane: head n of tile ht0 + x, rows (rt0 + t) * 16 + quad * 4 + r
+#pragma unroll
+        for (int x = 0; x < L::kHeadsPerWave; ++x) {
+            float most = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < L::kTilesPerWave; ++t) {
+                const uint32_t seen = masks[now * 4 + rt0 + t] >> (quad * 4);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    s[t][x][r] = seen >> r & 1 ? s[t][x][r] * scale : -INFINITY;
+                    most = fmaxf(most, s[t][x][r]);
+                }
+            }
+            most = fmaxf(most, __shfl_xor(most, 16));
+            most = fmaxf(most, __shfl_xor(most, 32));
+            if (quad == 0) parts[part * (HT * 16) + (ht0 + x) * 16 + n] = most;
+        }
+        lds_barrier();
+#pragma unroll
+        for (int x = 0; x < HT; ++x) { // every wave keeps every head's maximum, from the same numbers
+            float most = parts[x * 16 + n];
+#pragma unroll
+            for (int i = 1; i < L::kParts; ++i) most = fmaxf(most, parts[i * (HT * 16) + x * 16 + n]);
+            if (__any(most > top[x] + kSlack)) {
+                const float raised = fmaxf(top[x], most), shrink = top[x] == -INFINITY ? 0.0f : exp2_fast(top[x] - raised);
+                top[x] = raised;
+#pragma unroll
+                for (int y = 0; y < L::kHeadsPerWave; ++y)
+                    if (ht0 + y == static_cast<uint32_t>(x)) sum[y] *= shrink;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) o[x][d] *= shrink;
+            }
+        }
+#pragma unroll
+        for (int x = 0; x < L::kHeadsPerWave; ++x) {
+            float ref = top[x];
+            if constexpr (HT == 4) ref = ht0 ? top[2 + x] : top[x];
+            const float from = (ref == -INFINITY ? 0.0f : ref) - kLift<T>;
+            const uint32_t h = (ht0 + x) * 16 + n;
+#pragma unroll
+            for (int t = 0; t < L::kTilesPerWave; ++t) {
+                typedef T Four __attribute__((ext_vector_type(4)));
+                Four w;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float p = exp2_fast(s[t][x][r] - from);
+                    sum[x] += p;
+                    w[r] = from_f32<T>(p);
+                }
+                const uint32_t at = (rt0 + t) * 16 + quad * 4; // first of the four rows
+                if constexpr (sizeof(T) == 2) *reinterpret_cast<Four*>(probs + h * 128 + ((at >> 3) ^ (h >> 1 & 7)) * 16 + (at & 4) * 2) = w;
+                else *reinterpret_cast<Four*>(probs + h * 256 + ((at >> 2) ^ (h & 15)) * 16) = w;
+            }
+        }
+        lds_barrier();
+        uint32_t value_at[2]; // row of the first 32, the wave's first columns; columns 16 d further are 2 d words on, bits that the lane's word has not set
+#pragma unroll
+        for (int half = 0; half < 2; ++half) value_at[half] = L::at(quad * 8 + half * 4 + (n >> 2), wave * (DT * 2) + (n >> 1 & 1)) + (n & 1) * 8;
+#pragma unroll
+        for (int b = 0; b < kRowTile / 32; ++b) {
+            Frag<T> w[HT];
+#pragma unroll
+            for (int x = 0; x < HT; ++x) {
+                const uint32_t h = x * 16 + n;
+                if constexpr (sizeof(T) == 2) {
+                    w[x] = *reinterpret_cast<const Frag<T>*>(probs + h * 128 + ((b * 4 + quad) ^ (h >> 1 & 7)) * 16);
+                } else {
+                    *reinterpret_cast<f32x4*>(&w[x]) = *reinterpret_cast<const f32x4*>(probs + h * 256 + ((b * 8 + quad * 2) ^ (h & 15)) * 16);
+                    *(reinterpret_cast<f32x4*>(&w[x]) + 1) = *reinterpret_cast<const f32x4*>(probs + h * 256 + ((b * 8 + quad * 2 + 1) ^ (h & 15)) * 16);
+                }
+            }
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                const uint32_t col = wave * (DT * 16) + d * 16; // first of 16 columns
+                Frag<T> f;
+                if constexpr (sizeof(T) == 2) {
+                    // a transposing read: lane 4 i + j of 16 points at columns 4 j .. of row i; each lane gets its column's four rows
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        const uint32_t at = (value_at[half] ^ (d & 7) << 5) + b * (32 * 1024);
+                        const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds_byte*)(tile + at));
+                        *(reinterpret_cast<s16x4*>(&f) + half) = v;
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) f[i] = *reinterpret_cast<const float*>(tile + L::at(b * 32 + quad * 8 + i, (col + n) >> 2) + (n & 3) * 4);
+                }
+#pragma unroll
+                for (int x = 0; x < HT; ++x) o[x][d] = product16(f, w[x], o[x][d]);
+            }
+        }
+        if (more) {
+            if constexpr (L::kBuffers == 2) {
+                settle(now ^ 1, mask);
+                lds_barrier();
+                now ^= 1;
+            } else {
+                lds_barrier();
+                bring(0);
+                mask = there;
+                find(base + 2 * kRowTile);
+                settle(0, mask);
+                lds_barrier();
+            }
+        }
+    }
+    // the probabilities' sums over the waves that share a head
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < L::kHeadsPerWave; ++x) {
+        sum[x] += __shfl_xor(sum[x], 16);
+        sum[x] += __shfl_xor(sum[x], 32);
+        if (quad == 0) parts[part * (HT * 16) + (ht0 + x) * 16 + n] = sum[x];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < HT; ++x) {
+        const uint32_t h = x * 16 + n;
+        if (h >= heads) continue;
+        float total = 0.0f;
+#pragma unroll
+        for (int i = 0; i < L::kParts; ++i) total += parts[i * (HT * 16) + h];
+        const float ref = top[x] - kLift<T>; // sums are of 2^(score - ref)
+        const uint32_t head = g * a.group + h0 + h;
+        const bool whole = c.count == 1;
+        const size_t at = static_cast<size_t>(whole ? c.query : c.slot) * a.n_heads + head;
+        const float factor = !whole ? 1.0f : total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const uint32_t col = wave * (DT * 16) + d * 16 + quad * 4 + r;
+                if (col < a.dv) {
+                    if (whole) static_cast<T*>(a.out)[at * a.dv + col] = from_f32<T>(o[x][d][r] * factor);
+                    else plan.partial[at * a.dv + col] = o[x][d][r];
+                }
+            }
+        if (wave == 0 && quad == 0) {
+            if (!whole) plan.stats[at] = make_float2(ref, total);
+            else if (a.lse) a.lse[at] = total == 0.0f ? -INFINITY : (ref + log2f(total)) * kLn2;
+        }
+    }
+}
+
 // The chunks of a query joined: out = sum_k 2^(top_k - top) o_k / sum_k 2^(top_k - top) sum_k.  One workgroup per head and query; queries of one chunk are done already,
 // queries without rows (no slot is theirs) get their zeros here.
 template <typename T> __global__ __launch_bounds__(128) void join_kernel(const AttentionArgs a, const Plan plan) {
@@ -461,25 +800,24 @@ int check_attention(const svsx_attention_desc* d, AttentionArgs* a) {
     a->n_sequences = static_cast<uint32_t>(d->n_sequences);
     a->max_pages = static_cast<uint32_t>(d->max_pages);
     a->scale = d->scale;
+    a->shared = d->d_values == nullptr;
     return SVSX_SUCCESS;
 }
 
 // How a call is answered; decided from sizes, types, strides and addresses alone.
 struct Route {
-    bool group;       // on the matrix units; else one workgroup per head (rows beyond 256 columns)
+    bool rows, group; // many heads over shared rows, or heads that share a key head, on the matrix units; else one workgroup per head
     bool wide, page8;
-    int ks, vb;
-    uint32_t slots, target, y;
+    int ks, vb, ht;
+    uint32_t slots, target, unit, y;
     size_t stats_at, chunks_at, bytes;
 };
 
-// Four workgroups for every compute unit: enough to even out ragged batches.
-constexpr uint32_t kTargetGroups = 1024;
+// Slots to aim at are this many workgroups: four a compute unit even out ragged batches; where LDS holds one workgroup a compute unit, two.
+constexpr uint32_t kGroupTarget = 1024, kRowsTarget = 512;
 
 Route route_of(const AttentionArgs& a, size_t es) {
     Route r = {};
-    r.group = a.dk <= 256 && a.dv <= 256;
-    if (!r.group) return r;
     auto aligned = [&](std::initializer_list<size_t> strides, const void* p) {
         size_t all = reinterpret_cast<size_t>(p);
         for (size_t x : strides) all |= x * es;
@@ -487,18 +825,31 @@ Route route_of(const AttentionArgs& a, size_t es) {
     };
     r.wide = a.dk % 8 == 0 && a.dv % 8 == 0 && aligned({a.key_page_stride, a.key_head_stride, a.key_row_stride}, a.keys) &&
              aligned({a.value_page_stride, a.value_head_stride, a.value_row_stride}, a.values);
-    r.page8 = a.page_size % 8 == 0;
-    r.vb = a.dv > 128 || a.dk > 128 ? 2 : 1;
-    r.ks = !r.wide ? (r.vb == 2 ? 8 : 4) : a.dk > 192 ? 8 : a.dk > 128 || r.vb == 2 ? 6 : a.dk > 96 ? 4 : a.dk > 64 ? 3 : 2;
-    r.y = a.n_key_heads * ((a.group + 15) / 16);
-    // one chunk a query where queries alone fill the machine, or where no query can have more rows than a few tiles
-    const uint64_t groups = static_cast<uint64_t>(a.n_queries) * r.y, most = static_cast<uint64_t>(a.max_pages) * a.page_size;
-    if (groups >= 4 * kTargetGroups || most <= kChunkUnit) {
+    // Shared rows go through LDS where more than 16 heads read them, and where they are too long for the registers of the other kernel
+    r.rows = a.shared && r.wide && a.dk <= 576 && a.dv <= 512 && (a.group > 16 || a.dk > 256);
+    r.group = !r.rows && a.dk <= 256 && a.dv <= 256;
+    if (!r.rows && !r.group) return r;
+    if (r.rows) {
+        r.ks = a.dk <= 320 && a.dv <= 256 ? 10 : 18;
+        r.ht = a.group <= 16 || es == 4 ? 1 : a.group <= 32 ? 2 : 4; // float32 queries of 16 heads fill the registers
+        r.unit = kRowTile;
+        r.y = a.n_key_heads * ((a.group + r.ht * 16 - 1) / (r.ht * 16));
+    } else {
+        r.page8 = a.page_size % 8 == 0;
+        r.vb = a.dv > 128 || a.dk > 128 ? 2 : 1;
+        r.ks = !r.wide ? (r.vb == 2 ? 8 : 4) : a.dk > 192 ? 8 : a.dk > 128 || r.vb == 2 ? 6 : a.dk > 96 ? 4 : a.dk > 64 ? 3 : 2;
+        r.unit = kChunkUnit;
+        r.y = a.n_key_heads * ((a.group + 15) / 16);
+    }
+    // one chunk a query where queries alone fill the machine, where no query can have more rows than one unit, or where the sum of all units might not fit 32 bits
+    const uint32_t goal = r.rows ? kRowsTarget : kGroupTarget;
+    const uint64_t groups = static_cast<uint64_t>(a.n_queries) * r.y, units = (static_cast<uint64_t>(a.max_pages) * a.page_size + r.unit - 1) / r.unit;
+    if (groups >= 4 * goal || units <= 1 || units * a.n_queries >= (1ull << 32)) {
         r.slots = a.n_queries;
         return r;
     }
-    r.target = std::max(1u, kTargetGroups / r.y);
-    r.slots = static_cast<uint32_t>(std::min<uint64_t>(static_cast<uint64_t>(r.target) + a.n_queries, a.n_queries * ((most + kChunkUnit - 1) / kChunkUnit)));
+    r.target = std::max(1u, goal / r.y);
+    r.slots = static_cast<uint32_t>(std::min<uint64_t>(static_cast<uint64_t>(r.target) + a.n_queries, a.n_queries * units));
     const size_t parts = static_cast<size_t>(r.slots) * a.n_heads;
     r.stats_at = (parts * a.dv * 4 + 15) / 16 * 16;
     r.chunks_at = r.stats_at + parts * 8;
@@ -506,9 +857,30 @@ Route route_of(const AttentionArgs& a, size_t es) {
     return r;
 }
 
-template <typename T> hipError_t launch_group(const AttentionArgs& a, const Route& r, void* workspace, hipStream_t stream) {
+template <typename T, int KS, int HT, int DT> hipError_t launch_rows(const AttentionArgs& a, const Plan& plan, const Route& r, hipStream_t stream) {
+    typedef RowsLayout<T, KS, HT, DT> L;
+    // more than 64 KB of LDS has to be asked for; asking is cheap and the same every time
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(attend_rows_kernel<T, KS, HT, DT>), hipFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((attend_rows_kernel<T, KS, HT, DT>), dim3(r.slots, r.y), dim3(256), L::kBytes, stream, a, plan, divider(a.page_size));
+    return hipGetLastError();
+}
+
+template <typename T> hipError_t launch_rows(const AttentionArgs& a, const Plan& plan, const Route& r, hipStream_t stream) {
+    if (r.ks == 10) {
+        if (r.ht == 1) return launch_rows<T, 10, 1, 4>(a, plan, r, stream);
+        if constexpr (sizeof(T) == 2) return r.ht == 2 ? launch_rows<T, 10, 2, 4>(a, plan, r, stream) : launch_rows<T, 10, 4, 4>(a, plan, r, stream);
+    } else {
+        if (r.ht == 1) return launch_rows<T, 18, 1, 8>(a, plan, r, stream);
+        if constexpr (sizeof(T) == 2) return r.ht == 2 ? launch_rows<T, 18, 2, 8>(a, plan, r, stream) : launch_rows<T, 18, 4, 8>(a, plan, r, stream);
+    }
+    return hipErrorInvalidValue;
+}
+
+template <typename T> hipError_t launch_split(const AttentionArgs& a, const Route& r, void* workspace, hipStream_t stream) {
     Plan plan = {};
     plan.target = r.target;
+    plan.unit = r.unit;
     if (r.target) {
         char* base = static_cast<char*>(workspace);
         plan.partial = reinterpret_cast<float*>(base);
@@ -527,14 +899,19 @@ template <typename T> hipError_t launch_group(const AttentionArgs& a, const Rout
     SVSX_GROUP(4, 1, false)
     SVSX_GROUP(8, 2, false)
 #undef SVSX_GROUP
-    if (!kernel) return hipErrorInvalidValue;
-    hipLaunchKernelGGL(kernel, dim3(r.slots, r.y), dim3(256), 0, stream, a, plan, divider(a.page_size));
+    if (r.rows) {
+        const hipError_t e = launch_rows<T>(a, plan, r, stream);
+        if (e != hipSuccess) return e;
+    } else {
+        if (!kernel) return hipErrorInvalidValue;
+        hipLaunchKernelGGL(kernel, dim3(r.slots, r.y), dim3(256), 0, stream, a, plan, divider(a.page_size));
+    }
     if (r.target) hipLaunchKernelGGL(join_kernel<T>, dim3(a.n_heads, a.n_queries), dim3(128), 0, stream, a, plan);
     return hipGetLastError();
 }
 
 template <typename T> hipError_t launch_attention(const AttentionArgs& a, const Route& r, void* workspace, hipStream_t stream) {
-    if (r.group) return launch_group<T>(a, r, workspace, stream);
+    if (r.rows || r.group) return launch_split<T>(a, r, workspace, stream);
     hipLaunchKernelGGL(attend_head_kernel<T>, dim3(a.n_heads, a.n_queries), dim3(256), 0, stream, a);
     return hipGetLastError();
 }
