@@ -18,7 +18,8 @@ struct AttentionArgs {
     size_t query_stride, query_head_stride, key_page_stride, key_head_stride, key_row_stride, value_page_stride, value_head_stride, value_row_stride, table_stride;
     uint32_t n_queries, n_heads, group, n_key_heads, dk, dv, n_pages, page_size, n_sequences, max_pages;
     float scale;
-    int shared; // rows are keys and values at once
+    int shared;       // rows are keys and values at once
+    int wide_queries; // heads' queries begin at 16-byte boundaries and are whole 16-byte words
 };
 
 // rows of query i: its table row and how many rows there are
@@ -90,7 +91,8 @@ struct Chunk {
     uint32_t query, begin, end, slot, count;
     const int32_t* table;
 };
-__device__ __forceinline__ bool find_chunk(const AttentionArgs& a, const Plan& plan, Chunk* c, uint32_t (&sh)[260]) {
+template <uint32_t kThreads> __device__ __forceinline__ bool find_chunk(const AttentionArgs& a, const Plan& plan, Chunk* c, uint32_t (&sh)[24]) {
+    constexpr uint32_t kWaves = kThreads / 64;
     if (plan.target == 0) {
         c->query = blockIdx.x;
         c->table = nullptr;
@@ -106,16 +108,17 @@ __device__ __forceinline__ bool find_chunk(const AttentionArgs& a, const Plan& p
         return i < a.n_queries ? (rows_of(a, i, &unused) + plan.unit - 1) / plan.unit : 0u;
     };
     uint32_t mine = 0;
-    for (uint32_t i = t; i < a.n_queries; i += 256) mine += units(i);
+    for (uint32_t i = t; i < a.n_queries; i += kThreads) mine += units(i);
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) mine += __shfl_xor(mine, off);
     if (lane == 0) sh[wave] = mine;
     __syncthreads();
-    const uint32_t total = sh[0] + sh[1] + sh[2] + sh[3];
+    uint32_t total = 0;
+    for (uint32_t w = 0; w < kWaves; ++w) total += sh[w];
     const uint32_t size = (total + plan.target - 1) / plan.target; // units in a chunk
-    if (threadIdx.x == 0) sh[256] = 0xFFFFFFFFu;
+    if (threadIdx.x == 0) sh[16] = 0xFFFFFFFFu;
     uint32_t base = 0;
-    for (uint32_t first = 0; first < a.n_queries; first += 256) { // which query has this slot
+    for (uint32_t first = 0; first < a.n_queries; first += kThreads) { // which query has this slot
         const uint32_t i = first + t, n = size ? (units(i) + size - 1) / size : 0;
         uint32_t incl = n;
 #pragma unroll
@@ -124,26 +127,28 @@ __device__ __forceinline__ bool find_chunk(const AttentionArgs& a, const Plan& p
             if (lane >= static_cast<uint32_t>(off)) incl += u;
         }
         __syncthreads();
-        if (lane == 63) sh[4 + wave] = incl;
+        if (lane == 63) sh[8 + wave] = incl;
         __syncthreads();
         uint32_t before = base;
-        for (uint32_t w = 0; w < wave; ++w) before += sh[4 + w];
+        for (uint32_t w = 0; w < kWaves; ++w) {
+            before += w < wave ? sh[8 + w] : 0;
+            base += sh[8 + w];
+        }
         const uint32_t at = before + incl - n;
         if (n > 0 && blockIdx.x >= at && blockIdx.x < at + n) {
-            sh[256] = i;
-            sh[257] = at;
-            sh[258] = n;
+            sh[16] = i;
+            sh[17] = at;
+            sh[18] = n;
         }
-        base += sh[4] + sh[5] + sh[6] + sh[7];
         if (base > blockIdx.x) break; // base is the same for all
     }
     __syncthreads();
-    if (sh[256] == 0xFFFFFFFFu) return false;
-    c->query = __builtin_amdgcn_readfirstlane(sh[256]); // the same for all: in scalar registers, so that loops over it are too
+    if (sh[16] == 0xFFFFFFFFu) return false;
+    c->query = __builtin_amdgcn_readfirstlane(sh[16]); // the same for all: in scalar registers, so that loops over it are too
     c->slot = blockIdx.x;
-    c->count = __builtin_amdgcn_readfirstlane(sh[258]);
+    c->count = __builtin_amdgcn_readfirstlane(sh[18]);
     c->table = nullptr;
-    const uint32_t rows = rows_of(a, c->query, &c->table), k = blockIdx.x - __builtin_amdgcn_readfirstlane(sh[257]);
+    const uint32_t rows = rows_of(a, c->query, &c->table), k = blockIdx.x - __builtin_amdgcn_readfirstlane(sh[17]);
     c->begin = __builtin_amdgcn_readfirstlane(k * size * plan.unit);
     c->end = __builtin_amdgcn_readfirstlane(min(rows, (k + 1) * size * plan.unit));
     if (k == 0 && threadIdx.x == 0 && blockIdx.y == 0) plan.chunks[c->query] = make_int2(static_cast<int>(blockIdx.x), static_cast<int>(c->count));
@@ -161,10 +166,10 @@ template <bool Page8> struct TileRows {
 
 template <typename T, int KS, int VB, bool Wide, bool Page8>
 __global__ __launch_bounds__(256, 2) void attend_group_kernel(const AttentionArgs a, const Plan plan, const Divider by_page) {
-    __shared__ uint32_t sh[260];
+    __shared__ uint32_t sh[24];
     __shared__ float join[2][VB * 32 + 2][64];
     Chunk c;
-    if (!find_chunk(a, plan, &c, sh)) return;
+    if (!find_chunk<256>(a, plan, &c, sh)) return;
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, quad = lane >> 4;
     const uint32_t tiles = (a.group + 15) / 16, g = blockIdx.y / tiles, h0 = (blockIdx.y % tiles) * 16; // key head; first head within its group
     const uint32_t heads = min(16u, a.group - h0), head = g * a.group + h0 + n;
@@ -357,25 +362,30 @@ __global__ __launch_bounds__(256, 2) void attend_group_kernel(const AttentionArg
 // ---- rows that are key and value at once, for many heads ------------------------------------------------------------------------------------------
 //
 // Latent rows: every head reads the same row, as key and (its first columns) as value, so 64 heads make 240 operations of each byte and the rows have to be
-// read from HBM once for all of them.  A workgroup of four waves brings 64 rows into LDS (straight from HBM, two buffers: the next 64 arrive while these are worked on) and
-// takes up to 64 heads over them:
-//   S = K Q^T     wave w takes 16 or 32 of the rows for 16 or 32 of the heads; its queries stay in registers
+// read from HBM once for all of them.  A workgroup brings 64 rows into LDS (straight from HBM, two buffers: the next 64 arrive while these are worked on) and
+// takes up to 64 heads over them, with eight waves (four for 16 heads):
+//   S = K Q^T     a wave takes 16 or 32 of the rows for 16 of the heads; its queries stay in registers
 //   maximum of the 64 rows per head through LDS; P, rounded to the row type, through LDS
-//   O^T = V^T P^T wave w takes a quarter of the value columns for all rows and heads; the transposed fragments come from gfx950's transposing LDS reads
+//   O^T = V^T P^T a wave takes its share of the value columns for all rows and heads; the transposed fragments come from gfx950's transposing LDS reads
 // (float32 rows: single words).  No sums are joined between waves but that of the probabilities.
-// LDS holds a row as 16-byte words in planes of 64 words (1 KB a row) and a narrow plane for the rest, word j of row r at j ^ swizzle(r): neither the 16 rows of a key
-// fragment nor the 16 half-words of a transposed one meet in a bank.
-// LDS reads bound it at 64 heads (248 KB per 64 rows against 2176 cycles of products), HBM at 16.
+// LDS holds a row as 16-byte words in planes of 64 words, rows 32 bytes further apart than they are long, so that neither eight rows of a key fragment nor the 16
+// half-words of a transposed one meet in a bank; and a narrow plane for the rest, which is brought in several rows at a time and has its words exchanged in fours instead.
+// (Exchanging single words of the long rows as well, with no padding, was measured: the loads then cross each 64-byte line out of order and cost twice the time.)
+// LDS reads bound it at 64 heads (416 KB per 64 rows, 3250 cycles, against 2176 cycles of products), HBM at 16.
 
 constexpr int kRowTile = 64;
 
-template <typename T, int KS, int HT, int DT> struct RowsLayout { // KS: 32-column steps of a key row; HT: 16-head tiles; DT: 16-column value tiles of a wave
+template <typename T, int KS, int HT> struct RowsLayout { // KS: 32-column steps of a key row; HT: 16-head tiles
+    static constexpr int kWaves = HT == 1 ? 4 : 8, kThreads = kWaves * 64;
+    static constexpr int DT = (KS > 10 ? 32 : 16) / kWaves;                    // 16-column value tiles of a wave: 512 or 256 columns in all
+    static constexpr uint32_t kBring = kRowTile / kWaves;                      // rows that a wave brings in
     static constexpr int kWords = KS * 32 * sizeof(T) / 16;                    // 16-byte words in a row
     static constexpr int kPlanes = kWords < 64 ? 1 : kWords / 64, kTail = kWords < 64 ? 0 : kWords % 64;
-    static constexpr int kTileBytes = kRowTile * 16 * (kPlanes * 64 + kTail);
+    static constexpr uint32_t kPlaneRow = 1024 + 32, kPlaneBytes = kRowTile * kPlaneRow;
+    static constexpr int kTileBytes = kPlaneBytes * kPlanes + kRowTile * 16 * kTail;
     static constexpr int kBuffers = sizeof(T) == 2 ? 2 : 1;                    // float32 rows: one buffer is 144 KB
     static constexpr int kProbBytes = HT * 16 * kRowTile * sizeof(T);
-    static constexpr int kHeadsPerWave = HT == 1 ? 1 : 2, kTilesPerWave = HT == 4 ? 2 : 1; // of 16 heads, of 16 rows
+    static constexpr int kTilesPerWave = HT == 4 ? 2 : 1;                      // of 16 rows, for one tile of 16 heads
     static constexpr int kParts = 4 / kTilesPerWave;                           // waves that share a head's rows
     static constexpr int kStatBytes = kParts * HT * 16 * 4;
     static constexpr int kBytes = kBuffers * kTileBytes + kProbBytes + kStatBytes + 64;
@@ -383,14 +393,10 @@ template <typename T, int KS, int HT, int DT> struct RowsLayout { // KS: 32-colu
     static_assert(kBytes <= 160 * 1024 - 1088, "LDS");
     // byte of word j of row r
     static __device__ __forceinline__ uint32_t at(uint32_t r, uint32_t j) {
-        if (kTail > 0 && j >= kPlanes * 64) return kRowTile * 1024 * kPlanes + r * (kTail * 16) + ((j - kPlanes * 64) ^ narrow(r)) * 16;
-        return (j >> 6) * (kRowTile * 1024) + r * 1024 + ((j & 63) ^ swizzle(r)) * 16;
+        if (kTail > 0 && j >= kPlanes * 64) return kPlaneBytes * kPlanes + r * (kTail * 16) + ((j - kPlanes * 64) ^ narrow(r)) * 16;
+        return (j >> 6) * kPlaneBytes + r * kPlaneRow + (j & 63) * 16;
     }
-    // word `lane_part | j` of the row whose word `lane_part` is at byte `first` (j is a constant that shares no bit with lane_part, which is below 16 and in the first plane)
-    static __device__ __forceinline__ uint32_t wide(uint32_t first, uint32_t j) { return (first ^ (j & 15) << 4) + (j >> 4 & 3) * 256 + (j >> 6) * (kRowTile * 1024); }
-    // rows r and r + 8 of four consecutive ones land in different pairs of words, all 16 rows in different words
-    static __device__ __forceinline__ uint32_t swizzle(uint32_t r) { return (r & 3) << 1 | (r >> 3 & 1) << 3 | (r >> 2 & 1); }
-    static __device__ __forceinline__ uint32_t narrow(uint32_t r) { return kTail == 8 ? r >> 1 & 7 : r & 15; }
+    static __device__ __forceinline__ uint32_t narrow(uint32_t r) { return kTail == 8 ? (r >> 1 & 1) << 2 : (r & 3) << 2; }
 };
 
 #pragma clang diagnostic ignored "-Winline-asm" // m0 is a reserved register; the compiler is told that it changes
@@ -405,41 +411,68 @@ __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(
 typedef __attribute__((address_space(3))) unsigned char lds_byte;
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-template <typename T, int KS, int HT, int DT> __global__ __launch_bounds__(256, 1) void attend_rows_kernel(const AttentionArgs a, const Plan plan, const Divider by_page) {
-    typedef RowsLayout<T, KS, HT, DT> L;
+template <typename T, int KS, int HT> __global__ __launch_bounds__((RowsLayout<T, KS, HT>::kThreads)) void attend_rows_kernel(const AttentionArgs a, const Plan plan, const Divider by_page) {
+    typedef RowsLayout<T, KS, HT> L;
+    constexpr int DT = L::DT;
+    constexpr uint32_t kThreads = L::kThreads, kBring = L::kBring;
     extern __shared__ __align__(16) unsigned char lds[];
-    __shared__ uint32_t sh[260];
+    __shared__ uint32_t sh[24];
     Chunk c;
-    if (!find_chunk(a, plan, &c, sh)) return;
+    if (!find_chunk<L::kThreads>(a, plan, &c, sh)) return;
     constexpr int kElems = 16 / sizeof(T); // elements in a 16-byte word
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, quad = lane >> 4;
     const uint32_t groups = (a.group + HT * 16 - 1) / (HT * 16), g = blockIdx.y / groups, h0 = (blockIdx.y % groups) * (HT * 16);
     const uint32_t heads = min(static_cast<uint32_t>(HT * 16), a.group - h0);
     unsigned char* probs = lds + L::kBuffers * L::kTileBytes;
     float* parts = reinterpret_cast<float*>(probs + L::kProbBytes);
-    uint32_t* masks = reinterpret_cast<uint32_t*>(probs + L::kProbBytes + L::kStatBytes); // [buffer][wave]: which of the wave's 16 rows are there
+    uint32_t* masks = reinterpret_cast<uint32_t*>(probs + L::kProbBytes + L::kStatBytes); // [buffer][wave]: which of the rows that the wave brought in are there
     const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_byte*)lds));
 
     const uint32_t words = a.dk / kElems; // of a row in memory; what LDS holds beyond them has to be finite
 
-    // the wave's queries: heads of tiles ht0 .., rows of tiles rt0 ..; through LDS, zeros where there is no head or column
-    const uint32_t ht0 = HT == 4 ? (wave & 1) * 2 : 0, rt0 = HT == 4 ? (wave >> 1) * 2 : wave, part = HT == 4 ? wave >> 1 : wave;
+    // the wave's queries: heads of tile ht, rows of tiles rt0 ..; through LDS, zeros where there is no head or column
+    const uint32_t ht = wave % HT, rt0 = wave / HT * L::kTilesPerWave, part = wave / HT;
     static_assert(HT * 16 * KS * 32 * sizeof(T) <= L::kBuffers * L::kTileBytes, "LDS");
-    Frag<T> q[L::kHeadsPerWave][KS];
+    Frag<T> q[KS];
     {
         T* stage = reinterpret_cast<T*>(lds);
         const T* from = static_cast<const T*>(a.queries) + c.query * a.query_stride + (g * a.group + h0) * a.query_head_stride;
-        for (uint32_t h = wave; h < HT * 16; h += 4)
-            for (uint32_t col = lane; col < KS * 32; col += 64) stage[h * (KS * 32) + col] = h < heads && col < a.dk ? from[h * a.query_head_stride + col] : from_f32<T>(0.0f);
+        constexpr uint32_t kRow = KS * 32, kBatch = 9;
+        if (a.wide_queries) {
+            constexpr uint32_t kAll = HT * 16 * kRow / 8;
+            for (uint32_t first = 0; first < kAll; first += kThreads * kBatch) {
+                Frag<T> f[kBatch];
+#pragma unroll
+                for (uint32_t i = 0; i < kBatch; ++i) {
+                    const uint32_t at = first + i * kThreads + threadIdx.x, h = at / (kRow / 8), col = at % (kRow / 8) * 8;
+                    f[i] = Frag<T>{};
+                    if (h < heads && col < a.dk) f[i] = *reinterpret_cast<const Frag<T>*>(from + h * a.query_head_stride + col);
+                }
+#pragma unroll
+                for (uint32_t i = 0; i < kBatch; ++i)
+                    if (const uint32_t at = first + i * kThreads + threadIdx.x; at < kAll) *reinterpret_cast<Frag<T>*>(stage + at * 8) = f[i];
+            }
+        } else {
+            constexpr uint32_t kAll = HT * 16 * kRow;
+            for (uint32_t first = 0; first < kAll; first += kThreads * kBatch) {
+                T f[kBatch];
+#pragma unroll
+                for (uint32_t i = 0; i < kBatch; ++i) {
+                    const uint32_t at = first + i * kThreads + threadIdx.x, h = at / kRow, col = at % kRow;
+                    f[i] = h < heads && col < a.dk ? from[h * a.query_head_stride + col] : from_f32<T>(0.0f);
+                }
+#pragma unroll
+                for (uint32_t i = 0; i < kBatch; ++i)
+                    if (const uint32_t at = first + i * kThreads + threadIdx.x; at < kAll) stage[at] = f[i];
+            }
+        }
         __syncthreads();
 #pragma unroll
-        for (int x = 0; x < L::kHeadsPerWave; ++x)
-#pragma unroll
-            for (int k = 0; k < KS; ++k) q[x][k] = *reinterpret_cast<const Frag<T>*>(stage + ((ht0 + x) * 16 + n) * (KS * 32) + k * 32 + quad * 8);
+        for (int k = 0; k < KS; ++k) q[k] = *reinterpret_cast<const Frag<T>*>(stage + (ht * 16 + n) * (KS * 32) + k * 32 + quad * 8);
         __syncthreads();
     }
     if (words < static_cast<uint32_t>(L::kWords)) {
-        for (uint32_t i = threadIdx.x; i < L::kBuffers * L::kTileBytes / 16; i += 256) reinterpret_cast<uint4*>(lds)[i] = make_uint4(0, 0, 0, 0);
+        for (uint32_t i = threadIdx.x; i < L::kBuffers * L::kTileBytes / 16; i += kThreads) reinterpret_cast<uint4*>(lds)[i] = make_uint4(0, 0, 0, 0);
         __syncthreads();
     }
     f32x4 o[HT][DT];
@@ -447,45 +480,45 @@ template <typename T, int KS, int HT, int DT> __global__ __launch_bounds__(256, 
     for (int x = 0; x < HT; ++x)
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[x][d] = f32x4{0, 0, 0, 0};
-    float top[HT], sum[L::kHeadsPerWave] = {};
+    float top[HT], sum = 0.0f;
 #pragma unroll
     for (int x = 0; x < HT; ++x) top[x] = -INFINITY;
     const float scale = a.scale * kLog2e;
     const T* keys = static_cast<const T*>(a.keys) + g * a.key_head_stride;
 
-    // rows that this wave brings in: 16 wave + n of a tile; one lane of four looks a row up
+    // rows that this wave brings in: kBring wave + n of a tile.  A row's page is looked up a tile before it is brought in, ahead of the loads that
+    // are to stay in flight: loads come back in order, and what waits for the page would wait for them.
     const T* row = keys;
-    uint32_t there = 0;
+    uint32_t there = 0, page_row = 0;
+    int32_t page = -1;
+    auto look = [&](uint32_t base) { page = c.table[by_page(min(base + wave * kBring + n % kBring, c.end - 1), &page_row)]; };
     auto find = [&](uint32_t base) {
-        const uint32_t r = base + wave * 16 + n;
-        uint32_t at;
-        const int32_t p = c.table[by_page(min(r, c.end - 1), &at)];
-        const bool page = static_cast<uint32_t>(p) < a.n_pages;
-        row = keys + (page ? static_cast<size_t>(p) : 0) * a.key_page_stride + at * a.key_row_stride;
-        there = static_cast<uint32_t>(__ballot(page && r < c.end)) & 0xFFFFu;
+        const bool is = static_cast<uint32_t>(page) < a.n_pages;
+        row = keys + (is ? static_cast<size_t>(page) : 0) * a.key_page_stride + page_row * a.key_row_stride;
+        there = static_cast<uint32_t>(__ballot(is && base + wave * kBring + n % kBring < c.end)) & ((1u << kBring) - 1);
     };
     auto bring = [&](uint32_t buffer) {
         const uint32_t to = lds0 + buffer * L::kTileBytes;
         const uint64_t addr = reinterpret_cast<uint64_t>(row);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
+        for (uint32_t r = 0; r < kBring; ++r) {
             const uint64_t base = static_cast<uint64_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(addr >> 32), r)) << 32 |
                                   static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(addr), r));
 #pragma unroll
-            for (int plane = 0; plane < L::kPlanes; ++plane) { // LDS is written lane by lane: the swizzle is in which word a lane fetches
-                const uint32_t word = plane * 64 + (lane ^ L::swizzle(r));
-                if (words >= (plane + 1) * 64u || word < words) direct_load(reinterpret_cast<const void*>(base), word * 16, to + plane * (kRowTile * 1024) + (wave * 16 + r) * 1024);
+            for (uint32_t plane = 0; plane < static_cast<uint32_t>(L::kPlanes); ++plane) {
+                const uint32_t word = plane * 64 + lane;
+                if (words >= (plane + 1) * 64 || word < words) direct_load(reinterpret_cast<const void*>(base), word * 16, to + plane * L::kPlaneBytes + (wave * kBring + r) * L::kPlaneRow);
             }
         }
         if constexpr (L::kTail > 0) {
-            constexpr int kRows = 64 / L::kTail; // rows in one go
+            constexpr uint32_t kRows = 64 / L::kTail; // rows in one go
 #pragma unroll
-            for (int r = 0; r < 16; r += kRows) {
+            for (uint32_t r = 0; r < kBring; r += kRows) {
                 const uint32_t mine = r + lane / L::kTail;
                 const uint64_t base = static_cast<uint64_t>(__shfl(static_cast<uint32_t>(addr >> 32), mine)) << 32 | __shfl(static_cast<uint32_t>(addr), mine);
                 const uint32_t word = L::kPlanes * 64 + (lane % L::kTail ^ L::narrow(mine));
                 const void* from = reinterpret_cast<const unsigned char*>(base) + word * 16;
-                const uint32_t dst = to + kRowTile * 1024 * L::kPlanes + (wave * 16 + r) * (L::kTail * 16);
+                const uint32_t dst = to + L::kPlaneBytes * L::kPlanes + (wave * kBring + r) * (L::kTail * 16);
                 if (word < words) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"(from) : "memory", "m0");
             }
         }
@@ -493,37 +526,37 @@ template <typename T, int KS, int HT, int DT> __global__ __launch_bounds__(256, 
     // once the rows are there: rows that are not to be seen become zeros (a weight of zero times what a page holds behind the last row need not be zero)
     auto settle = [&](uint32_t buffer, uint32_t mask) {
         direct_wait();
-        if (mask != 0xFFFFu) {
+        if (mask != (1u << kBring) - 1) {
             unsigned char* tile = lds + buffer * L::kTileBytes;
-            for (uint32_t r = 0; r < 16; ++r)
+            for (uint32_t r = 0; r < kBring; ++r)
                 if (!(mask >> r & 1))
-                    for (uint32_t j = lane; j < static_cast<uint32_t>(L::kWords); j += 64) *reinterpret_cast<uint4*>(tile + L::at(wave * 16 + r, j)) = make_uint4(0, 0, 0, 0);
+                    for (uint32_t j = lane; j < static_cast<uint32_t>(L::kWords); j += 64) *reinterpret_cast<uint4*>(tile + L::at(wave * kBring + r, j)) = make_uint4(0, 0, 0, 0);
         }
-        if (lane == 0) masks[buffer * 4 + wave] = mask;
+        if (lane == 0) masks[buffer * L::kWaves + wave] = mask;
     };
 
     uint32_t now = 0, mask = 0;
     if (c.begin < c.end) {
+        look(c.begin);
         find(c.begin);
+        look(c.begin + kRowTile);
         bring(0);
         mask = there;
-        find(c.begin + kRowTile);
         settle(0, mask);
         lds_barrier();
     }
     for (uint32_t base = c.begin; base < c.end; base += kRowTile) {
         const bool more = base + kRowTile < c.end;
         if (L::kBuffers == 2 && more) {
+            find(base + kRowTile);
+            look(base + 2 * kRowTile);
             bring(now ^ 1);
             mask = there;
-            find(base + 2 * kRowTile);
         }
         const unsigned char* tile = lds + now * L::kTileBytes;
-        f32x4 s[L::kTilesPerWave][L::kHeadsPerWave];
+        f32x4 s[L::kTilesPerWave];
 #pragma unroll
-        for (int t = 0; t < L::kTilesPerWave; ++t)
-#pragma unroll
-            for (int x = 0; x < L::kHeadsPerWave; ++x) s[t][x] = f32x4{0, 0, 0, 0};
+        for (int t = 0; t < L::kTilesPerWave; ++t) s[t] = f32x4{0, 0, 0, 0};
         uint32_t key_at[L::kTilesPerWave], tail_at[L::kTilesPerWave]; // this lane's first word of its rows
         constexpr int kStep = 2 * sizeof(T);                          // words in 32 columns
 #pragma unroll
@@ -536,7 +569,7 @@ template <typename T, int KS, int HT, int DT> __global__ __launch_bounds__(256, 
 #pragma unroll
             for (int t = 0; t < L::kTilesPerWave; ++t) {
                 const bool tail = k * kStep >= L::kPlanes * 64;
-                auto word = [&](uint32_t j) { return tile + (tail ? tail_at[t] ^ (j - L::kPlanes * 64) << 4 : L::wide(key_at[t], j)); };
+                auto word = [&](uint32_t j) { return tile + (tail ? tail_at[t] ^ (j - L::kPlanes * 64) << 4 : key_at[t] + (j >> 6) * L::kPlaneBytes + (j & 63) * 16); };
                 Frag<T> f;
                 if constexpr (sizeof(T) == 2) {
                     f = *reinterpret_cast<const Frag<T>*>(word(k * kStep));
@@ -544,26 +577,22 @@ template <typename T, int KS, int HT, int DT> __global__ __launch_bounds__(256, 
                     *reinterpret_cast<f32x4*>(&f) = *reinterpret_cast<const f32x4*>(word(k * kStep));
                     *(reinterpret_cast<f32x4*>(&f) + 1) = *reinterpret_cast<const f32x4*>(word(k * kStep + 1));
                 }
-#pragma unroll
-                for (int x = 0; x < L::kHeadsPerWave; ++x) s[t][x] = product16(f, q[x][k], s[t][x]);
+                s[t] = product16(f, q[k], s[t]);
             }
-        // lane: head n of tile ht0 + x, rows (rt0 + t) * 16 + quad * 4 + r
+        // lane: head n of tile ht, rows (rt0 + t) * 16 + quad * 4 + r
+        float most = -INFINITY;
 #pragma unroll
-        for (int x = 0; x < L::kHeadsPerWave; ++x) {
-            float most = -INFINITY;
+        for (int t = 0; t < L::kTilesPerWave; ++t) {
+            const uint32_t first = (rt0 + t) * 16 + quad * 4, seen = masks[now * L::kWaves + first / kBring] >> (first % kBring);
 #pragma unroll
-            for (int t = 0; t < L::kTilesPerWave; ++t) {
-                const uint32_t seen = masks[now * 4 + rt0 + t] >> (quad * 4);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    s[t][x][r] = seen >> r & 1 ? s[t][x][r] * scale : -INFINITY;
-                    most = fmaxf(most, s[t][x][r]);
-                }
+            for (int r = 0; r < 4; ++r) {
+                s[t][r] = seen >> r & 1 ? s[t][r] * scale : -INFINITY;
+                most = fmaxf(most, s[t][r]);
             }
-            most = fmaxf(most, __shfl_xor(most, 16));
-            most = fmaxf(most, __shfl_xor(most, 32));
-            if (quad == 0) parts[part * (HT * 16) + (ht0 + x) * 16 + n] = most;
         }
+        most = fmaxf(most, __shfl_xor(most, 16));
+        most = fmaxf(most, __shfl_xor(most, 32));
+        if (quad == 0) parts[part * (HT * 16) + ht * 16 + n] = most;
         lds_barrier();
 #pragma unroll
         for (int x = 0; x < HT; ++x) { // every wave keeps every head's maximum, from the same numbers
@@ -573,27 +602,25 @@ template <typename T, int KS, int HT, int DT> __global__ __launch_bounds__(256, 
             if (__any(most > top[x] + kSlack)) {
                 const float raised = fmaxf(top[x], most), shrink = top[x] == -INFINITY ? 0.0f : exp2_fast(top[x] - raised);
                 top[x] = raised;
-#pragma unroll
-                for (int y = 0; y < L::kHeadsPerWave; ++y)
-                    if (ht0 + y == static_cast<uint32_t>(x)) sum[y] *= shrink;
+                if (ht == static_cast<uint32_t>(x)) sum *= shrink;
 #pragma unroll
                 for (int d = 0; d < DT; ++d) o[x][d] *= shrink;
             }
         }
+        {
+            float ref = top[0];
 #pragma unroll
-        for (int x = 0; x < L::kHeadsPerWave; ++x) {
-            float ref = top[x];
-            if constexpr (HT == 4) ref = ht0 ? top[2 + x] : top[x];
+            for (int x = 1; x < HT; ++x) ref = ht == static_cast<uint32_t>(x) ? top[x] : ref;
             const float from = (ref == -INFINITY ? 0.0f : ref) - kLift<T>;
-            const uint32_t h = (ht0 + x) * 16 + n;
+            const uint32_t h = ht * 16 + n;
 #pragma unroll
             for (int t = 0; t < L::kTilesPerWave; ++t) {
                 typedef T Four __attribute__((ext_vector_type(4)));
                 Four w;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const float p = exp2_fast(s[t][x][r] - from);
-                    sum[x] += p;
+                    const float p = exp2_fast(s[t][r] - from);
+                    sum += p;
                     w[r] = from_f32<T>(p);
                 }
                 const uint32_t at = (rt0 + t) * 16 + quad * 4; // first of the four rows
@@ -602,7 +629,7 @@ template <typename T, int KS, int HT, int DT> __global__ __launch_bounds__(256, 
             }
         }
         lds_barrier();
-        uint32_t value_at[2]; // row of the first 32, the wave's first columns; columns 16 d further are 2 d words on, bits that the lane's word has not set
+        uint32_t value_at[2]; // row of the first 32, the wave's first columns
 #pragma unroll
         for (int half = 0; half < 2; ++half) value_at[half] = L::at(quad * 8 + half * 4 + (n >> 2), wave * (DT * 2) + (n >> 1 & 1)) + (n & 1) * 8;
 #pragma unroll
@@ -626,7 +653,7 @@ template <typename T, int KS, int HT, int DT> __global__ __launch_bounds__(256, 
                     // a transposing read: lane 4 i + j of 16 points at columns 4 j .. of row i; each lane gets its column's four rows
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
-                        const uint32_t at = (value_at[half] ^ (d & 7) << 5) + b * (32 * 1024);
+                        const uint32_t at = value_at[half] + d * 32 + b * (32 * L::kPlaneRow);
                         const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds_byte*)(tile + at));
                         *(reinterpret_cast<s16x4*>(&f) + half) = v;
                     }
@@ -645,9 +672,10 @@ template <typename T, int KS, int HT, int DT> __global__ __launch_bounds__(256, 
                 now ^= 1;
             } else {
                 lds_barrier();
+                find(base + kRowTile);
+                look(base + 2 * kRowTile);
                 bring(0);
                 mask = there;
-                find(base + 2 * kRowTile);
                 settle(0, mask);
                 lds_barrier();
             }
@@ -655,12 +683,9 @@ template <typename T, int KS, int HT, int DT> __global__ __launch_bounds__(256, 
     }
     // the probabilities' sums over the waves that share a head
     __syncthreads();
-#pragma unroll
-    for (int x = 0; x < L::kHeadsPerWave; ++x) {
-        sum[x] += __shfl_xor(sum[x], 16);
-        sum[x] += __shfl_xor(sum[x], 32);
-        if (quad == 0) parts[part * (HT * 16) + (ht0 + x) * 16 + n] = sum[x];
-    }
+    sum += __shfl_xor(sum, 16);
+    sum += __shfl_xor(sum, 32);
+    if (quad == 0) parts[part * (HT * 16) + ht * 16 + n] = sum;
     __syncthreads();
 #pragma unroll
     for (int x = 0; x < HT; ++x) {
@@ -673,17 +698,21 @@ template <typename T, int KS, int HT, int DT> __global__ __launch_bounds__(256, 
         const uint32_t head = g * a.group + h0 + h;
         const bool whole = c.count == 1;
         const size_t at = static_cast<size_t>(whole ? c.query : c.slot) * a.n_heads + head;
-        const float factor = !whole ? 1.0f : total == 0.0f ? 0.0f : 1.0f / total;
+        const float factor = total == 0.0f ? 0.0f : 1.0f / total;
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
+        for (int d = 0; d < DT; ++d) {
+            const uint32_t col = wave * (DT * 16) + d * 16 + quad * 4; // rows of whole 16-byte words: dv is a multiple of 4
+            if (col >= a.dv) continue;
+            if (whole) {
+                typedef T Four __attribute__((ext_vector_type(4)));
+                Four f;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const uint32_t col = wave * (DT * 16) + d * 16 + quad * 4 + r;
-                if (col < a.dv) {
-                    if (whole) static_cast<T*>(a.out)[at * a.dv + col] = from_f32<T>(o[x][d][r] * factor);
-                    else plan.partial[at * a.dv + col] = o[x][d][r];
-                }
+                for (int r = 0; r < 4; ++r) f[r] = from_f32<T>(o[x][d][r] * factor);
+                *reinterpret_cast<Four*>(static_cast<T*>(a.out) + at * a.dv + col) = f;
+            } else {
+                *reinterpret_cast<f32x4*>(plan.partial + at * a.dv + col) = o[x][d];
             }
+        }
         if (wave == 0 && quad == 0) {
             if (!whole) plan.stats[at] = make_float2(ref, total);
             else if (a.lse) a.lse[at] = total == 0.0f ? -INFINITY : (ref + log2f(total)) * kLn2;
@@ -691,17 +720,19 @@ template <typename T, int KS, int HT, int DT> __global__ __launch_bounds__(256, 
     }
 }
 
-// The chunks of a query joined: out = sum_k 2^(top_k - top) o_k / sum_k 2^(top_k - top) sum_k.  One workgroup per head and query; queries of one chunk are done already,
-// queries without rows (no slot is theirs) get their zeros here.
-template <typename T> __global__ __launch_bounds__(128) void join_kernel(const AttentionArgs a, const Plan plan) {
-    __shared__ float weight[128];
-    __shared__ float wide[2][2];
+// The chunks of a query joined: out = sum_k 2^(top_k - top) o_k / sum_k 2^(top_k - top) sum_k.  One workgroup per head and query; queries of one chunk are done
+// already, queries without rows (no slot is theirs) get their zeros here.  A thread takes W columns of every 256 W / dv-th chunk, so that few long queries
+// are not a chain of loads; the threads' parts meet in LDS.
+template <typename T, int W> __global__ __launch_bounds__(256) void join_kernel(const AttentionArgs a, const Plan plan) {
+    typedef float Cols __attribute__((ext_vector_type(W)));
+    __shared__ float weight[256], wide[8];
+    __shared__ Cols part[256];
     const uint32_t h = blockIdx.x, i = blockIdx.y, t = threadIdx.x;
     const size_t at = static_cast<size_t>(i) * a.n_heads + h;
     T* out = static_cast<T*>(a.out) + at * a.dv;
     const int32_t* table;
     if (rows_of(a, i, &table) == 0) {
-        for (uint32_t col = t; col < a.dv; col += 128) out[col] = from_f32<T>(0.0f);
+        for (uint32_t col = t; col < a.dv; col += 256) out[col] = from_f32<T>(0.0f);
         if (a.lse && t == 0) a.lse[at] = -INFINITY;
         return;
     }
@@ -709,47 +740,49 @@ template <typename T> __global__ __launch_bounds__(128) void join_kernel(const A
     if (mine.y == 1) return;
     const uint32_t n = static_cast<uint32_t>(mine.y);
     const float2* stats = plan.stats + static_cast<size_t>(mine.x) * a.n_heads + h;
-    float top = -INFINITY;
-    for (uint32_t k = t; k < n; k += 128) top = fmaxf(top, stats[static_cast<size_t>(k) * a.n_heads].x);
+    float top = -INFINITY, sum = 0.0f;
+    for (uint32_t k = t; k < n; k += 256) top = fmaxf(top, stats[static_cast<size_t>(k) * a.n_heads].x);
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
-    if ((t & 63) == 0) wide[0][t >> 6] = top;
+    if ((t & 63) == 0) wide[t >> 6] = top;
     __syncthreads();
-    top = fmaxf(wide[0][0], wide[0][1]);
-    float sum = 0.0f, acc[8] = {};
+    top = fmaxf(fmaxf(wide[0], wide[1]), fmaxf(wide[2], wide[3]));
+    const uint32_t cols = a.dv / W; // W divides dv
     const float* partial = plan.partial + (static_cast<size_t>(mine.x) * a.n_heads + h) * a.dv;
     const size_t step = static_cast<size_t>(a.n_heads) * a.dv;
-    for (uint32_t first = 0; first < n; first += 128) {
-        __syncthreads();
-        if (first + t < n) {
-            const float2 st = stats[static_cast<size_t>(first + t) * a.n_heads];
-            const float w = st.x == -INFINITY ? 0.0f : exp2_fast(st.x - top);
-            weight[t] = w;
-            sum += w * st.y;
+    for (uint32_t base = 0; base < cols; base += 256) { // one turn but for long odd rows
+        const uint32_t here = min(256u, cols - base), parts = 256 / here, p = t / here, col = (base + t % here) * W;
+        Cols acc = {};
+        for (uint32_t first = 0; first < n; first += 256) {
+            __syncthreads();
+            if (first + t < n) {
+                const float2 st = stats[static_cast<size_t>(first + t) * a.n_heads];
+                const float w = st.x == -INFINITY ? 0.0f : exp2_fast(st.x - top);
+                weight[t] = w;
+                if (base == 0) sum += w * st.y;
+            }
+            __syncthreads();
+            const uint32_t some = min(256u, n - first);
+            if (p < parts) {
+                const float* from = partial + first * step + col;
+#pragma unroll 8
+                for (uint32_t k = p; k < some; k += parts) acc += weight[k] * *reinterpret_cast<const Cols*>(from + k * step);
+            }
         }
-        __syncthreads();
-        const uint32_t some = min(128u, n - first);
+        if (base == 0) {
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-            const uint32_t col = t + 128 * c;
-            if (col >= a.dv) break;
-            const float* from = partial + first * step + col;
-            float x = acc[c];
-#pragma unroll 4
-            for (uint32_t k = 0; k < some; ++k) x = fmaf(weight[k], from[k * step], x);
-            acc[c] = x;
+            for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off);
+            if ((t & 63) == 0) wide[4 + (t >> 6)] = sum;
         }
-    }
+        part[t] = acc;
+        __syncthreads();
+        sum = wide[4] + wide[5] + wide[6] + wide[7];
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        if (t < here) {
+            for (uint32_t k = 1; k < parts; ++k) acc += part[t + k * here];
 #pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off);
-    if ((t & 63) == 0) wide[1][t >> 6] = sum;
-    __syncthreads();
-    sum = wide[1][0] + wide[1][1];
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-    for (int c = 0; c < 8; ++c) {
-        const uint32_t col = t + 128 * c;
-        if (col < a.dv) out[col] = from_f32<T>(acc[c] * inv);
+            for (int j = 0; j < W; ++j) out[col + j] = from_f32<T>(acc[j] * inv);
+        }
     }
     if (a.lse && t == 0) a.lse[at] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
 }
@@ -801,6 +834,8 @@ int check_attention(const svsx_attention_desc* d, AttentionArgs* a) {
     a->max_pages = static_cast<uint32_t>(d->max_pages);
     a->scale = d->scale;
     a->shared = d->d_values == nullptr;
+    const size_t es = paged_dtype_size(d->dtype);
+    a->wide_queries = d->key_dim % 8 == 0 && ((reinterpret_cast<size_t>(d->d_queries) | d->query_stride * es | d->query_head_stride * es) & 15) == 0;
     return SVSX_SUCCESS;
 }
 
@@ -857,22 +892,22 @@ Route route_of(const AttentionArgs& a, size_t es) {
     return r;
 }
 
-template <typename T, int KS, int HT, int DT> hipError_t launch_rows(const AttentionArgs& a, const Plan& plan, const Route& r, hipStream_t stream) {
-    typedef RowsLayout<T, KS, HT, DT> L;
+template <typename T, int KS, int HT> hipError_t launch_rows(const AttentionArgs& a, const Plan& plan, const Route& r, hipStream_t stream) {
+    typedef RowsLayout<T, KS, HT> L;
     // more than 64 KB of LDS has to be asked for; asking is cheap and the same every time
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(attend_rows_kernel<T, KS, HT, DT>), hipFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(attend_rows_kernel<T, KS, HT>), hipFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((attend_rows_kernel<T, KS, HT, DT>), dim3(r.slots, r.y), dim3(256), L::kBytes, stream, a, plan, divider(a.page_size));
+    hipLaunchKernelGGL((attend_rows_kernel<T, KS, HT>), dim3(r.slots, r.y), dim3(L::kThreads), L::kBytes, stream, a, plan, divider(a.page_size));
     return hipGetLastError();
 }
 
 template <typename T> hipError_t launch_rows(const AttentionArgs& a, const Plan& plan, const Route& r, hipStream_t stream) {
     if (r.ks == 10) {
-        if (r.ht == 1) return launch_rows<T, 10, 1, 4>(a, plan, r, stream);
-        if constexpr (sizeof(T) == 2) return r.ht == 2 ? launch_rows<T, 10, 2, 4>(a, plan, r, stream) : launch_rows<T, 10, 4, 4>(a, plan, r, stream);
+        if (r.ht == 1) return launch_rows<T, 10, 1>(a, plan, r, stream);
+        if constexpr (sizeof(T) == 2) return r.ht == 2 ? launch_rows<T, 10, 2>(a, plan, r, stream) : launch_rows<T, 10, 4>(a, plan, r, stream);
     } else {
-        if (r.ht == 1) return launch_rows<T, 18, 1, 8>(a, plan, r, stream);
-        if constexpr (sizeof(T) == 2) return r.ht == 2 ? launch_rows<T, 18, 2, 8>(a, plan, r, stream) : launch_rows<T, 18, 4, 8>(a, plan, r, stream);
+        if (r.ht == 1) return launch_rows<T, 18, 1>(a, plan, r, stream);
+        if constexpr (sizeof(T) == 2) return r.ht == 2 ? launch_rows<T, 18, 2>(a, plan, r, stream) : launch_rows<T, 18, 4>(a, plan, r, stream);
     }
     return hipErrorInvalidValue;
 }
@@ -906,7 +941,7 @@ template <typename T> hipError_t launch_split(const AttentionArgs& a, const Rout
         if (!kernel) return hipErrorInvalidValue;
         hipLaunchKernelGGL(kernel, dim3(r.slots, r.y), dim3(256), 0, stream, a, plan, divider(a.page_size));
     }
-    if (r.target) hipLaunchKernelGGL(join_kernel<T>, dim3(a.n_heads, a.n_queries), dim3(128), 0, stream, a, plan);
+    if (r.target) hipLaunchKernelGGL((a.dv % 4 == 0 ? join_kernel<T, 4> : join_kernel<T, 1>), dim3(a.n_heads, a.n_queries), dim3(256), 0, stream, a, plan);
     return hipGetLastError();
 }
 
