@@ -81,82 +81,120 @@ struct Plan {
     float* partial;  // [slot][head][dv] sums of p v
     float2* stats;   // [slot][head] {maximum (powers of two), sum of p}
     int2* chunks;    // [query] {first slot, chunks}
-    uint32_t target; // slots to aim at; 0: one chunk a query and no joining
-    uint32_t unit;   // rows that a workgroup takes at a time
+    uint32_t workers; // workgroups that share all rows; 0: one workgroup a query and no joining
+    uint32_t unit;    // rows that a workgroup takes at a time
 };
 
-// Which rows a workgroup has.  Lengths are known on the device only, so every workgroup derives the same plan from them: all queries' rows in units of plan.unit,
-// divided over `target` slots, give the chunk; slots are dealt out query by query (at most target + n_queries of them).  False: nothing to do.
+// Which rows a workgroup has.  Lengths are known on the device only, so every workgroup derives the same plan from them: all queries' rows, in units of plan.unit, one
+// query behind the other, are cut into `workers` equal runs; a workgroup takes its run query by query.  Worker w's part of query i goes to slot w + i: along the line of
+// units each step raises one of the two, so slots differ, and a query's are consecutive (at most workers + n_queries slots).
 struct Chunk {
-    uint32_t query, begin, end, slot, count;
+    uint32_t query, begin, end, slot, count; // count: parts of this query; 1: nothing to join
     const int32_t* table;
 };
-template <uint32_t kThreads> __device__ __forceinline__ bool find_chunk(const AttentionArgs& a, const Plan& plan, Chunk* c, uint32_t (&sh)[24]) {
-    constexpr uint32_t kWaves = kThreads / 64;
-    if (plan.target == 0) {
-        c->query = blockIdx.x;
-        c->table = nullptr;
-        c->begin = 0;
-        c->end = __builtin_amdgcn_readfirstlane(rows_of(a, c->query, &c->table));
-        c->slot = 0;
-        c->count = 1;
-        return true;
-    }
-    const uint32_t t = threadIdx.x, wave = t >> 6, lane = t & 63;
-    auto units = [&](uint32_t i) {
+template <uint32_t kThreads> struct Walk {
+    static constexpr uint32_t kWaves = kThreads / 64;
+    uint32_t total, workers, stop, query, before; // all units; workers that have some; the end of this worker's run; units before the query's first
+
+    static __device__ __forceinline__ uint32_t units(const AttentionArgs& a, const Plan& plan, uint32_t i) {
         const int32_t* unused;
         return i < a.n_queries ? (rows_of(a, i, &unused) + plan.unit - 1) / plan.unit : 0u;
-    };
-    uint32_t mine = 0;
-    for (uint32_t i = t; i < a.n_queries; i += kThreads) mine += units(i);
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) mine += __shfl_xor(mine, off);
-    if (lane == 0) sh[wave] = mine;
-    __syncthreads();
-    uint32_t total = 0;
-    for (uint32_t w = 0; w < kWaves; ++w) total += sh[w];
-    const uint32_t size = (total + plan.target - 1) / plan.target; // units in a chunk
-    if (threadIdx.x == 0) sh[16] = 0xFFFFFFFFu;
-    uint32_t base = 0;
-    for (uint32_t first = 0; first < a.n_queries; first += kThreads) { // which query has this slot
-        const uint32_t i = first + t, n = size ? (units(i) + size - 1) / size : 0;
-        uint32_t incl = n;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const uint32_t u = __shfl_up(incl, off);
-            if (lane >= static_cast<uint32_t>(off)) incl += u;
-        }
-        __syncthreads();
-        if (lane == 63) sh[8 + wave] = incl;
-        __syncthreads();
-        uint32_t before = base;
-        for (uint32_t w = 0; w < kWaves; ++w) {
-            before += w < wave ? sh[8 + w] : 0;
-            base += sh[8 + w];
-        }
-        const uint32_t at = before + incl - n;
-        if (n > 0 && blockIdx.x >= at && blockIdx.x < at + n) {
-            sh[16] = i;
-            sh[17] = at;
-            sh[18] = n;
-        }
-        if (base > blockIdx.x) break; // base is the same for all
     }
-    __syncthreads();
-    if (sh[16] == 0xFFFFFFFFu) return false;
-    c->query = __builtin_amdgcn_readfirstlane(sh[16]); // the same for all: in scalar registers, so that loops over it are too
-    c->slot = blockIdx.x;
-    c->count = __builtin_amdgcn_readfirstlane(sh[18]);
-    c->table = nullptr;
-    const uint32_t rows = rows_of(a, c->query, &c->table), k = blockIdx.x - __builtin_amdgcn_readfirstlane(sh[17]);
-    c->begin = __builtin_amdgcn_readfirstlane(k * size * plan.unit);
-    c->end = __builtin_amdgcn_readfirstlane(min(rows, (k + 1) * size * plan.unit));
-    if (k == 0 && threadIdx.x == 0 && blockIdx.y == 0) plan.chunks[c->query] = make_int2(static_cast<int>(blockIdx.x), static_cast<int>(c->count));
-    return true;
-}
+    // the worker whose run [floor(w total / workers), floor((w + 1) total / workers)) has unit u
+    __device__ __forceinline__ uint32_t owner(uint32_t u) const { return static_cast<uint32_t>(((u + 1ull) * workers - 1) / total); }
+
+    __device__ __forceinline__ void set(const AttentionArgs& a, const Plan& plan, uint32_t unit, Chunk* c) {
+        c->query = query;
+        c->table = nullptr;
+        const uint32_t rows = __builtin_amdgcn_readfirstlane(rows_of(a, query, &c->table)), mine = (rows + plan.unit - 1) / plan.unit;
+        const uint32_t first = owner(before);
+        c->begin = __builtin_amdgcn_readfirstlane((unit - before) * plan.unit);
+        c->end = __builtin_amdgcn_readfirstlane(min(rows, (min(before + mine, stop) - before) * plan.unit));
+        c->slot = blockIdx.x + query;
+        c->count = __builtin_amdgcn_readfirstlane(owner(before + mine - 1) - first + 1);
+        if (unit == before && threadIdx.x == 0 && blockIdx.y == 0) plan.chunks[query] = make_int2(static_cast<int>(first + query), static_cast<int>(c->count));
+    }
+    // the first part of this worker's run; false: it has none
+    __device__ __forceinline__ bool first(const AttentionArgs& a, const Plan& plan, Chunk* c, uint32_t (&sh)[24]) {
+        if (plan.workers == 0) {
+            c->query = blockIdx.x;
+            c->table = nullptr;
+            c->begin = 0;
+            c->end = __builtin_amdgcn_readfirstlane(rows_of(a, c->query, &c->table));
+            c->slot = 0;
+            c->count = 1;
+            return true;
+        }
+        const uint32_t t = threadIdx.x, wave = t >> 6, lane = t & 63;
+        auto scan = [&](uint32_t n, uint32_t base, uint32_t* all) { // units before this thread's query, after `base` of them; two barriers
+            uint32_t incl = n;
+#pragma unroll
+            for (int off = 1; off < 64; off <<= 1) {
+                const uint32_t u = __shfl_up(incl, off);
+                if (lane >= static_cast<uint32_t>(off)) incl += u;
+            }
+            __syncthreads();
+            if (lane == 63) sh[wave] = incl;
+            __syncthreads();
+            uint32_t at = base + incl - n;
+            *all = base;
+#pragma unroll
+            for (uint32_t w = 0; w < kWaves; ++w) {
+                const uint32_t some = __builtin_amdgcn_readfirstlane(sh[w]);
+                at += w < wave ? some : 0;
+                *all += some;
+            }
+            return at;
+        };
+        // all that follows waits for one load, for up to kThreads queries
+        const uint32_t mine = units(a, plan, t);
+        uint32_t n = mine, at = scan(mine, 0, &total), upto = total;
+        for (uint32_t from = kThreads; from < a.n_queries; from += kThreads) scan(units(a, plan, from + t), total, &total);
+        workers = min(plan.workers, total); // no run is empty: a query's parts are those of consecutive workers
+        if (blockIdx.x >= workers) return false;
+        const uint32_t start = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(static_cast<uint64_t>(blockIdx.x) * total / workers));
+        stop = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>((blockIdx.x + 1ull) * total / workers));
+        for (uint32_t from = 0;;) { // which query has the first unit
+            if (n > 0 && start >= at && start < at + n) {
+                sh[16] = from + t;
+                sh[17] = at;
+            }
+            from += kThreads;
+            if (upto > start || from >= a.n_queries) break;
+            n = units(a, plan, from + t);
+            at = scan(n, upto, &upto);
+        }
+        __syncthreads();
+        query = __builtin_amdgcn_readfirstlane(sh[16]); // the same for all: in scalar registers, so that loops over it are too
+        before = __builtin_amdgcn_readfirstlane(sh[17]);
+        set(a, plan, start, c);
+        return true;
+    }
+    // the next one
+    __device__ __forceinline__ bool next(const AttentionArgs& a, const Plan& plan, Chunk* c) {
+        if (plan.workers == 0) return false;
+        uint32_t mine = __builtin_amdgcn_readfirstlane(units(a, plan, query));
+        if (before + mine >= stop) return false;
+        do { // units are left, so there is a query that has them
+            before += mine;
+            ++query;
+            mine = __builtin_amdgcn_readfirstlane(units(a, plan, query));
+        } while (mine == 0 && query < a.n_queries);
+        set(a, plan, before, c);
+        return true;
+    }
+};
 
 // 2^x; the hardware's instruction, denormal results are zero
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// The lane, as something that the compiler cannot know to be the same for every part of a worker's run: what follows from it would otherwise be kept in registers over
+// the whole run (addresses and conditions of code that runs once a part), and there are none to spare.
+__device__ __forceinline__ uint32_t lane_here() {
+    uint32_t lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
+    return lane;
+}
 
 // Where a lane's rows are: pages of the two key rows and the eight value rows.  Page8: page_size is a multiple of 8, so eight consecutive rows share a page.
 template <bool Page8> struct TileRows {
@@ -165,198 +203,202 @@ template <bool Page8> struct TileRows {
 };
 
 template <typename T, int KS, int VB, bool Wide, bool Page8>
-__global__ __launch_bounds__(256, 2) void attend_group_kernel(const AttentionArgs a, const Plan plan, const Divider by_page) {
+__global__ __launch_bounds__(256, sizeof(T) == 2 && VB == 1 ? 3 : 2) void attend_group_kernel(const AttentionArgs a, const Plan plan, const Divider by_page) {
     __shared__ uint32_t sh[24];
     __shared__ float join[2][VB * 32 + 2][64];
     Chunk c;
-    if (!find_chunk<256>(a, plan, &c, sh)) return;
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, quad = lane >> 4;
+    Walk<256> walk;
+    if (!walk.first(a, plan, &c, sh)) return;
+    const uint32_t wave = threadIdx.x >> 6;
     const uint32_t tiles = (a.group + 15) / 16, g = blockIdx.y / tiles, h0 = (blockIdx.y % tiles) * 16; // key head; first head within its group
-    const uint32_t heads = min(16u, a.group - h0), head = g * a.group + h0 + n;
-    const bool live = n < heads;
+    const uint32_t heads = min(16u, a.group - h0);
 
-    Frag<T> q[KS];
-    {
-        const T* row = static_cast<const T*>(a.queries) + c.query * a.query_stride + (live ? head : g * a.group) * a.query_head_stride;
+    do {
+        const uint32_t lane = lane_here(), n = lane & 15, quad = lane >> 4, head = g * a.group + h0 + n;
+        const bool live = n < heads;
+        Frag<T> q[KS];
+        {
+            const T* row = static_cast<const T*>(a.queries) + c.query * a.query_stride + (live ? head : g * a.group) * a.query_head_stride;
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
-            q[k] = load_frag<T, false>(row, k * 32 + quad * 8, a.dk);
-            if (!live) q[k] = Frag<T>{};
+            for (int k = 0; k < KS; ++k) {
+                q[k] = a.wide_queries ? load_frag<T, true>(row, k * 32 + quad * 8, a.dk) : load_frag<T, false>(row, k * 32 + quad * 8, a.dk);
+                if (!live) q[k] = Frag<T>{};
+            }
         }
-    }
-    const T* keys = static_cast<const T*>(a.keys) + g * a.key_head_stride;
-    const T* values = static_cast<const T*>(a.values) + g * a.value_head_stride;
-    const float scale = a.scale * kLog2e;
+        const T* keys = static_cast<const T*>(a.keys) + g * a.key_head_stride;
+        const T* values = static_cast<const T*>(a.values) + g * a.value_head_stride;
+        const float scale = a.scale * kLog2e;
 
-    f32x4 o[VB * 8];
+        f32x4 o[VB * 8];
 #pragma unroll
-    for (int i = 0; i < VB * 8; ++i) o[i] = f32x4{0, 0, 0, 0};
-    float top = -INFINITY, sum = 0.0f; // the maximum that probabilities are relative to, in powers of two; this lane's share of their sum
+        for (int i = 0; i < VB * 8; ++i) o[i] = f32x4{0, 0, 0, 0};
+        float top = -INFINITY, sum = 0.0f; // the maximum that probabilities are relative to, in powers of two; this lane's share of their sum
 
-    const uint32_t last = c.end - 1; // rows behind the end are looked up at the last one, and masked
-    auto find = [&](uint32_t base) {
-        TileRows<Page8> r;
-        if constexpr (Page8) {
-            r.key[0] = c.table[by_page(min(base + (n >> 2) * 8, last), &r.key_at[0])];
-            r.value[0] = c.table[by_page(min(base + quad * 8, last), &r.value_at[0])];
-            // the page's row of the block's first row: `last` may be in its middle
-            r.key_at[0] &= ~7u;
-            r.value_at[0] &= ~7u;
-        } else {
+        const uint32_t last = c.end - 1; // rows behind the end are looked up at the last one, and masked
+        auto find = [&](uint32_t base) {
+            TileRows<Page8> r;
+            if constexpr (Page8) {
+                r.key[0] = c.table[by_page(min(base + (n >> 2) * 8, last), &r.key_at[0])];
+                r.value[0] = c.table[by_page(min(base + quad * 8, last), &r.value_at[0])];
+                // the page's row of the block's first row: `last` may be in its middle
+                r.key_at[0] &= ~7u;
+                r.value_at[0] &= ~7u;
+            } else {
 #pragma unroll
-            for (int s = 0; s < 2; ++s) r.key[s] = c.table[by_page(min(base + (n >> 2) * 8 + s * 4 + (n & 3), last), &r.key_at[s])];
+                for (int s = 0; s < 2; ++s) r.key[s] = c.table[by_page(min(base + (n >> 2) * 8 + s * 4 + (n & 3), last), &r.key_at[s])];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) r.value[j] = c.table[by_page(min(base + quad * 8 + j, last), &r.value_at[j])];
-        }
-        return r;
-    };
-    auto is_page = [&](int32_t p) { return static_cast<uint32_t>(p) < a.n_pages; }; // negative ones are large
-    auto load_keys = [&](const TileRows<Page8>& r, Frag<T> (&k)[2][KS]) {
+                for (int j = 0; j < 8; ++j) r.value[j] = c.table[by_page(min(base + quad * 8 + j, last), &r.value_at[j])];
+            }
+            return r;
+        };
+        auto is_page = [&](int32_t p) { return static_cast<uint32_t>(p) < a.n_pages; }; // negative ones are large
+        auto load_keys = [&](const TileRows<Page8>& r, Frag<T> (&k)[2][KS]) {
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            const int32_t p = Page8 ? r.key[0] : r.key[Page8 ? 0 : s];
-            const uint32_t at = Page8 ? r.key_at[0] + s * 4 + (n & 3) : r.key_at[Page8 ? 0 : s];
-            const T* row = keys + (is_page(p) ? static_cast<size_t>(p) : 0) * a.key_page_stride + at * a.key_row_stride;
+            for (int s = 0; s < 2; ++s) {
+                const int32_t p = Page8 ? r.key[0] : r.key[Page8 ? 0 : s];
+                const uint32_t at = Page8 ? r.key_at[0] + s * 4 + (n & 3) : r.key_at[Page8 ? 0 : s];
+                const T* row = keys + (is_page(p) ? static_cast<size_t>(p) : 0) * a.key_page_stride + at * a.key_row_stride;
 #pragma unroll
-            for (int i = 0; i < KS; ++i) k[s][i] = load_frag<T, Wide>(row, i * 32 + quad * 8, a.dk);
-        }
-    };
+                for (int i = 0; i < KS; ++i) k[s][i] = load_frag<T, Wide>(row, i * 32 + quad * 8, a.dk);
+            }
+        };
 
-    uint32_t base = c.begin + wave * kTile;
-    Frag<T> k[2][KS];
-    TileRows<Page8> here, next;
-    if (base < c.end) {
-        here = find(base);
-        load_keys(here, k);
-        next = find(base + kChunkUnit);
-    }
-    for (; base < c.end; base += kChunkUnit) {
-        Frag<T> v[VB][8];
-        uint32_t mask = 0; // which of the lane's eight rows are there
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int32_t p = Page8 ? here.value[0] : here.value[Page8 ? 0 : j];
-            const uint32_t at = Page8 ? here.value_at[0] + j : here.value_at[Page8 ? 0 : j];
-            if (base + quad * 8 + j < c.end && is_page(p)) mask |= 1u << j;
-            const T* row = values + (is_page(p) ? static_cast<size_t>(p) : 0) * a.value_page_stride + at * a.value_row_stride;
-#pragma unroll
-            for (int b = 0; b < VB; ++b) v[b][j] = load_frag<T, Wide>(row, b * 128 + n * 8, a.dv);
-        }
-        f32x4 s[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
-#pragma unroll
-        for (int i = 0; i < KS; ++i) {
-            s[0] = product16(k[0][i], q[i], s[0]);
-            s[1] = product16(k[1][i], q[i], s[1]);
-        }
-        if (base + kChunkUnit < c.end) {
-            here = next;
+        uint32_t base = c.begin + wave * kTile;
+        Frag<T> k[2][KS];
+        TileRows<Page8> here, next;
+        if (base < c.end) {
+            here = find(base);
             load_keys(here, k);
-            next = find(base + 2 * kChunkUnit);
+            next = find(base + kChunkUnit);
         }
-        float p[8], most = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) p[j] = s[j >> 2][j & 3] * scale;
-        if (!__all(mask == 0xFFu)) {
+        for (; base < c.end; base += kChunkUnit) {
+            Frag<T> v[VB][8];
+            uint32_t mask = 0; // which of the lane's eight rows are there
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const bool there = mask >> j & 1;
-                p[j] = there ? p[j] : -INFINITY;
+                const int32_t p = Page8 ? here.value[0] : here.value[Page8 ? 0 : j];
+                const uint32_t at = Page8 ? here.value_at[0] + j : here.value_at[Page8 ? 0 : j];
+                if (base + quad * 8 + j < c.end && is_page(p)) mask |= 1u << j;
+                const T* row = values + (is_page(p) ? static_cast<size_t>(p) : 0) * a.value_page_stride + at * a.value_row_stride;
 #pragma unroll
-                for (int b = 0; b < VB; ++b) // what a page holds behind the last row is not defined: zero times it need not be zero
-                    if (!there) v[b][j] = Frag<T>{};
+                for (int b = 0; b < VB; ++b) v[b][j] = load_frag<T, Wide>(row, b * 128 + n * 8, a.dv);
+            }
+            f32x4 s[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+                s[0] = product16(k[0][i], q[i], s[0]);
+                s[1] = product16(k[1][i], q[i], s[1]);
+            }
+            if (base + kChunkUnit < c.end) {
+                here = next;
+                load_keys(here, k);
+                next = find(base + 2 * kChunkUnit);
+            }
+            float p[8], most = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) p[j] = s[j >> 2][j & 3] * scale;
+            if (!__all(mask == 0xFFu)) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const bool there = mask >> j & 1;
+                    p[j] = there ? p[j] : -INFINITY;
+#pragma unroll
+                    for (int b = 0; b < VB; ++b) // what a page holds behind the last row is not defined: zero times it need not be zero
+                        if (!there) v[b][j] = Frag<T>{};
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) most = fmaxf(most, p[j]);
+            most = fmaxf(most, __shfl_xor(most, 16));
+            most = fmaxf(most, __shfl_xor(most, 32));
+            if (__any(most > top + kSlack)) { // also the first tile: top is -inf
+                const float raised = fmaxf(top, most), shrink = top == -INFINITY ? 0.0f : exp2_fast(top - raised);
+                top = raised;
+                sum *= shrink;
+#pragma unroll
+                for (int i = 0; i < VB * 8; ++i) o[i] *= shrink;
+            }
+            const float from = (top == -INFINITY ? 0.0f : top) - kLift<T>;
+            Frag<T> w;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                p[j] = exp2_fast(p[j] - from);
+                sum += p[j];
+                w[j] = from_f32<T>(p[j]);
+            }
+#pragma unroll
+            for (int b = 0; b < VB; ++b) {
+#pragma unroll
+                for (int d = 0; d < 8; ++d) {
+                    Frag<T> column;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) column[j] = v[b][j][d];
+                    o[b * 8 + d] = product16(column, w, o[b * 8 + d]);
+                }
             }
         }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) most = fmaxf(most, p[j]);
-        most = fmaxf(most, __shfl_xor(most, 16));
-        most = fmaxf(most, __shfl_xor(most, 32));
-        if (__any(most > top + kSlack)) { // also the first tile: top is -inf
-            const float raised = fmaxf(top, most), shrink = top == -INFINITY ? 0.0f : exp2_fast(top - raised);
-            top = raised;
-            sum *= shrink;
-#pragma unroll
-            for (int i = 0; i < VB * 8; ++i) o[i] *= shrink;
-        }
-        const float from = (top == -INFINITY ? 0.0f : top) - kLift<T>;
-        Frag<T> w;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            p[j] = exp2_fast(p[j] - from);
-            sum += p[j];
-            w[j] = from_f32<T>(p[j]);
-        }
-#pragma unroll
-        for (int b = 0; b < VB; ++b) {
-#pragma unroll
-            for (int d = 0; d < 8; ++d) {
-                Frag<T> column;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) column[j] = v[b][j][d];
-                o[b * 8 + d] = product16(column, w, o[b * 8 + d]);
-            }
-        }
-    }
-    sum += __shfl_xor(sum, 16);
-    sum += __shfl_xor(sum, 32);
-    top -= kLift<T>; // sums are of 2^(score - top)
+        sum += __shfl_xor(sum, 16);
+        sum += __shfl_xor(sum, 32);
+        top -= kLift<T>; // sums are of 2^(score - top)
 
-    // the four waves' results, two at a time: waves 2 and 3 into 0 and 1, then 1 into 0
+        // the four waves' results, two at a time: waves 2 and 3 into 0 and 1, then 1 into 0
 #pragma unroll
-    for (int half = 2; half >= 1; half >>= 1) {
-        __syncthreads();
-        if (wave >= static_cast<uint32_t>(half) && wave < 2u * half) {
+        for (int half = 2; half >= 1; half >>= 1) {
+            __syncthreads();
+            if (wave >= static_cast<uint32_t>(half) && wave < 2u * half) {
 #pragma unroll
-            for (int i = 0; i < VB * 32; ++i) join[wave - half][i][lane] = o[i >> 2][i & 3];
-            join[wave - half][VB * 32][lane] = top;
-            join[wave - half][VB * 32 + 1][lane] = sum;
+                for (int i = 0; i < VB * 32; ++i) join[wave - half][i][lane] = o[i >> 2][i & 3];
+                join[wave - half][VB * 32][lane] = top;
+                join[wave - half][VB * 32 + 1][lane] = sum;
+            }
+            __syncthreads();
+            if (wave < static_cast<uint32_t>(half)) {
+                const float other = join[wave][VB * 32][lane], all = fmaxf(top, other);
+                const float wa = top == -INFINITY ? 0.0f : exp2_fast(top - all), wb = other == -INFINITY ? 0.0f : exp2_fast(other - all);
+                sum = sum * wa + join[wave][VB * 32 + 1][lane] * wb;
+                top = all;
+#pragma unroll
+                for (int i = 0; i < VB * 32; ++i) o[i >> 2][i & 3] = o[i >> 2][i & 3] * wa + join[wave][i][lane] * wb;
+            }
         }
-        __syncthreads();
-        if (wave < static_cast<uint32_t>(half)) {
-            const float other = join[wave][VB * 32][lane], all = fmaxf(top, other);
-            const float wa = top == -INFINITY ? 0.0f : exp2_fast(top - all), wb = other == -INFINITY ? 0.0f : exp2_fast(other - all);
-            sum = sum * wa + join[wave][VB * 32 + 1][lane] * wb;
-            top = all;
+        if (wave != 0 || !live) continue;
+        // o[b * 8 + d][r]: column b * 128 + (quad * 4 + r) * 8 + d of head n
+        if (c.count > 1) {
+            const size_t at = static_cast<size_t>(c.slot) * a.n_heads + head;
+            if (quad == 0) plan.stats[at] = make_float2(top, sum);
+            float* out = plan.partial + at * a.dv;
 #pragma unroll
-            for (int i = 0; i < VB * 32; ++i) o[i >> 2][i & 3] = o[i >> 2][i & 3] * wa + join[wave][i][lane] * wb;
+            for (int b = 0; b < VB; ++b)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int d = 0; d < 8; ++d) {
+                        const uint32_t col = b * 128 + (quad * 4 + r) * 8 + d;
+                        if (col < a.dv) out[col] = o[b * 8 + d][r];
+                    }
+            continue;
         }
-    }
-    if (wave != 0 || !live) return;
-    // o[b * 8 + d][r]: column b * 128 + (quad * 4 + r) * 8 + d of head n
-    if (c.count > 1) {
-        const size_t at = static_cast<size_t>(c.slot) * a.n_heads + head;
-        if (quad == 0) plan.stats[at] = make_float2(top, sum);
-        float* out = plan.partial + at * a.dv;
+        const size_t at = static_cast<size_t>(c.query) * a.n_heads + head;
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        T* out = static_cast<T*>(a.out) + at * a.dv;
 #pragma unroll
         for (int b = 0; b < VB; ++b)
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
+            for (int r = 0; r < 4; ++r) {
+                const uint32_t col = b * 128 + (quad * 4 + r) * 8;
+                Frag<T> f;
 #pragma unroll
-                for (int d = 0; d < 8; ++d) {
-                    const uint32_t col = b * 128 + (quad * 4 + r) * 8 + d;
-                    if (col < a.dv) out[col] = o[b * 8 + d][r];
+                for (int d = 0; d < 8; ++d) f[d] = from_f32<T>(o[b * 8 + d][r] * inv);
+                if (a.dv % 8 == 0) {
+                    if (col < a.dv) *reinterpret_cast<Frag<T>*>(out + col) = f;
+                } else {
+#pragma unroll
+                    for (uint32_t d = 0; d < 8; ++d)
+                        if (col + d < a.dv) out[col + d] = f[d];
                 }
-        return;
-    }
-    const size_t at = static_cast<size_t>(c.query) * a.n_heads + head;
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    T* out = static_cast<T*>(a.out) + at * a.dv;
-#pragma unroll
-    for (int b = 0; b < VB; ++b)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const uint32_t col = b * 128 + (quad * 4 + r) * 8;
-            Frag<T> f;
-#pragma unroll
-            for (int d = 0; d < 8; ++d) f[d] = from_f32<T>(o[b * 8 + d][r] * inv);
-            if (a.dv % 8 == 0) {
-                if (col < a.dv) *reinterpret_cast<Frag<T>*>(out + col) = f;
-            } else {
-#pragma unroll
-                for (uint32_t d = 0; d < 8; ++d)
-                    if (col + d < a.dv) out[col + d] = f[d];
             }
-        }
-    if (a.lse && quad == 0) a.lse[at] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
+        if (a.lse && quad == 0) a.lse[at] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
+    } while (walk.next(a, plan, &c));
 }
 
 // ---- rows that are key and value at once, for many heads ------------------------------------------------------------------------------------------
@@ -371,26 +413,29 @@ __global__ __launch_bounds__(256, 2) void attend_group_kernel(const AttentionArg
 // LDS holds a row as 16-byte words in planes of 64 words, rows 32 bytes further apart than they are long, so that neither eight rows of a key fragment nor the 16
 // half-words of a transposed one meet in a bank; and a narrow plane for the rest, which is brought in several rows at a time and has its words exchanged in fours instead.
 // (Exchanging single words of the long rows as well, with no padding, was measured: the loads then cross each 64-byte line out of order and cost twice the time.)
-// LDS reads bound it at 64 heads (416 KB per 64 rows, 3250 cycles, against 2176 cycles of products), HBM at 16.
-
-constexpr int kRowTile = 64;
+// At 16 heads HBM bounds it; at 64 the latency of the steps between a tile's barriers (LDS is busy for 2400 cycles of a tile's 8800, the matrix units for 2176).  Two workgroups
+// of 32-row buffers and four waves on a compute unit were measured in place of one of eight waves: their registers spill, 104 -> 127 us (32 sequences, 128 heads).
 
 template <typename T, int KS, int HT> struct RowsLayout { // KS: 32-column steps of a key row; HT: 16-head tiles
+    static constexpr uint32_t kRows = 64;                                      // rows of a tile
     static constexpr int kWaves = HT == 1 ? 4 : 8, kThreads = kWaves * 64;
     static constexpr int DT = (KS > 10 ? 32 : 16) / kWaves;                    // 16-column value tiles of a wave: 512 or 256 columns in all
-    static constexpr uint32_t kBring = kRowTile / kWaves;                      // rows that a wave brings in
+    static constexpr uint32_t kBring = kRows / kWaves;                         // rows that a wave brings in
     static constexpr int kWords = KS * 32 * sizeof(T) / 16;                    // 16-byte words in a row
     static constexpr int kPlanes = kWords < 64 ? 1 : kWords / 64, kTail = kWords < 64 ? 0 : kWords % 64;
-    static constexpr uint32_t kPlaneRow = 1024 + 32, kPlaneBytes = kRowTile * kPlaneRow;
-    static constexpr int kTileBytes = kPlaneBytes * kPlanes + kRowTile * 16 * kTail;
+    static constexpr uint32_t kPlaneRow = 1024 + 32, kPlaneBytes = kRows * kPlaneRow;
+    static constexpr int kTileBytes = kPlaneBytes * kPlanes + kRows * 16 * kTail;
     static constexpr int kBuffers = sizeof(T) == 2 ? 2 : 1;                    // float32 rows: one buffer is 144 KB
-    static constexpr int kProbBytes = HT * 16 * kRowTile * sizeof(T);
+    static constexpr uint32_t kProbRow = kRows * sizeof(T), kProbWords = kProbRow / 16;
+    static constexpr int kProbBytes = HT * 16 * kProbRow;
     static constexpr int kTilesPerWave = HT == 4 ? 2 : 1;                      // of 16 rows, for one tile of 16 heads
-    static constexpr int kParts = 4 / kTilesPerWave;                           // waves that share a head's rows
+    static constexpr int kParts = kRows / 16 / kTilesPerWave;                  // waves that share a head's rows
     static constexpr int kStatBytes = kParts * HT * 16 * 4;
     static constexpr int kBytes = kBuffers * kTileBytes + kProbBytes + kStatBytes + 64;
+    static_assert(kWaves == HT * kParts, "a wave is a tile of heads and a part of the rows");
+    static __device__ __forceinline__ uint32_t prob(uint32_t h, uint32_t word) { return h * kProbRow + (word ^ (h / (16 / kProbWords) & (kProbWords - 1))) * 16; }
     static_assert(kTail == 0 || kTail == 8 || kTail == 16, "a narrow plane of 8 or 16 words");
-    static_assert(kBytes <= 160 * 1024 - 1088, "LDS");
+    static_assert(kBytes + 128 <= 160 * 1024, "LDS");
     // byte of word j of row r
     static __device__ __forceinline__ uint32_t at(uint32_t r, uint32_t j) {
         if (kTail > 0 && j >= kPlanes * 64) return kPlaneBytes * kPlanes + r * (kTail * 16) + ((j - kPlanes * 64) ^ narrow(r)) * 16;
@@ -418,13 +463,14 @@ template <typename T, int KS, int HT> __global__ __launch_bounds__((RowsLayout<T
     extern __shared__ __align__(16) unsigned char lds[];
     __shared__ uint32_t sh[24];
     Chunk c;
-    if (!find_chunk<L::kThreads>(a, plan, &c, sh)) return;
+    Walk<L::kThreads> walk;
+    if (!walk.first(a, plan, &c, sh)) return;
     constexpr int kElems = 16 / sizeof(T); // elements in a 16-byte word
-    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, quad = lane >> 4;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t groups = (a.group + HT * 16 - 1) / (HT * 16), g = blockIdx.y / groups, h0 = (blockIdx.y % groups) * (HT * 16);
     const uint32_t heads = min(static_cast<uint32_t>(HT * 16), a.group - h0);
     unsigned char* probs = lds + L::kBuffers * L::kTileBytes;
-    float* parts = reinterpret_cast<float*>(probs + L::kProbBytes);
+    float* parts = reinterpret_cast<float*>(probs + L::kProbBytes); // [part][head]: maxima; sums
     uint32_t* masks = reinterpret_cast<uint32_t*>(probs + L::kProbBytes + L::kStatBytes); // [buffer][wave]: which of the rows that the wave brought in are there
     const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_byte*)lds));
 
@@ -433,186 +479,179 @@ template <typename T, int KS, int HT> __global__ __launch_bounds__((RowsLayout<T
     // the wave's queries: heads of tile ht, rows of tiles rt0 ..; through LDS, zeros where there is no head or column
     const uint32_t ht = wave % HT, rt0 = wave / HT * L::kTilesPerWave, part = wave / HT;
     static_assert(HT * 16 * KS * 32 * sizeof(T) <= L::kBuffers * L::kTileBytes, "LDS");
-    Frag<T> q[KS];
-    {
-        T* stage = reinterpret_cast<T*>(lds);
-        const T* from = static_cast<const T*>(a.queries) + c.query * a.query_stride + (g * a.group + h0) * a.query_head_stride;
-        constexpr uint32_t kRow = KS * 32, kBatch = 9;
-        if (a.wide_queries) {
-            constexpr uint32_t kAll = HT * 16 * kRow / 8;
-            for (uint32_t first = 0; first < kAll; first += kThreads * kBatch) {
-                Frag<T> f[kBatch];
+    do {
+        const uint32_t lane = lane_here(), thread = wave * 64 + lane, n = lane & 15, quad = lane >> 4;
+        Frag<T> q[KS];
+        {
+            const T* from = static_cast<const T*>(a.queries) + c.query * a.query_stride + (g * a.group + h0) * a.query_head_stride;
+            T* stage = reinterpret_cast<T*>(lds);
+            constexpr uint32_t kRow = KS * 32, kBatch = 9;
+            if (a.wide_queries) {
+                constexpr uint32_t kAll = HT * 16 * kRow / 8;
+                for (uint32_t first = 0; first < kAll; first += kThreads * kBatch) {
+                    Frag<T> f[kBatch];
 #pragma unroll
-                for (uint32_t i = 0; i < kBatch; ++i) {
-                    const uint32_t at = first + i * kThreads + threadIdx.x, h = at / (kRow / 8), col = at % (kRow / 8) * 8;
-                    f[i] = Frag<T>{};
-                    if (h < heads && col < a.dk) f[i] = *reinterpret_cast<const Frag<T>*>(from + h * a.query_head_stride + col);
+                    for (uint32_t i = 0; i < kBatch; ++i) {
+                        const uint32_t at = first + i * kThreads + thread, h = at / (kRow / 8), col = at % (kRow / 8) * 8;
+                        f[i] = Frag<T>{};
+                        if (h < heads && col < a.dk) f[i] = *reinterpret_cast<const Frag<T>*>(from + h * a.query_head_stride + col);
+                    }
+#pragma unroll
+                    for (uint32_t i = 0; i < kBatch; ++i)
+                        if (const uint32_t at = first + i * kThreads + thread; at < kAll) *reinterpret_cast<Frag<T>*>(stage + at * 8) = f[i];
                 }
-#pragma unroll
-                for (uint32_t i = 0; i < kBatch; ++i)
-                    if (const uint32_t at = first + i * kThreads + threadIdx.x; at < kAll) *reinterpret_cast<Frag<T>*>(stage + at * 8) = f[i];
-            }
-        } else {
-            constexpr uint32_t kAll = HT * 16 * kRow;
-            for (uint32_t first = 0; first < kAll; first += kThreads * kBatch) {
-                T f[kBatch];
-#pragma unroll
-                for (uint32_t i = 0; i < kBatch; ++i) {
-                    const uint32_t at = first + i * kThreads + threadIdx.x, h = at / kRow, col = at % kRow;
-                    f[i] = h < heads && col < a.dk ? from[h * a.query_head_stride + col] : from_f32<T>(0.0f);
+            } else {
+                for (uint32_t i = thread; i < HT * 16 * kRow; i += kThreads) {
+                    const uint32_t h = i / kRow, col = i % kRow;
+                    stage[i] = h < heads && col < a.dk ? from[h * a.query_head_stride + col] : from_f32<T>(0.0f);
                 }
-#pragma unroll
-                for (uint32_t i = 0; i < kBatch; ++i)
-                    if (const uint32_t at = first + i * kThreads + threadIdx.x; at < kAll) stage[at] = f[i];
             }
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < KS; ++k) q[k] = *reinterpret_cast<const Frag<T>*>(stage + (ht * 16 + n) * kRow + k * 32 + quad * 8);
+            __syncthreads();
         }
-        __syncthreads();
+        if (words < static_cast<uint32_t>(L::kWords)) {
+            for (uint32_t i = thread; i < L::kBuffers * L::kTileBytes / 16; i += kThreads) reinterpret_cast<uint4*>(lds)[i] = make_uint4(0, 0, 0, 0);
+            __syncthreads();
+        }
+        f32x4 o[HT][DT];
 #pragma unroll
-        for (int k = 0; k < KS; ++k) q[k] = *reinterpret_cast<const Frag<T>*>(stage + (ht * 16 + n) * (KS * 32) + k * 32 + quad * 8);
-        __syncthreads();
-    }
-    if (words < static_cast<uint32_t>(L::kWords)) {
-        for (uint32_t i = threadIdx.x; i < L::kBuffers * L::kTileBytes / 16; i += kThreads) reinterpret_cast<uint4*>(lds)[i] = make_uint4(0, 0, 0, 0);
-        __syncthreads();
-    }
-    f32x4 o[HT][DT];
+        for (int x = 0; x < HT; ++x)
 #pragma unroll
-    for (int x = 0; x < HT; ++x)
+            for (int d = 0; d < DT; ++d) o[x][d] = f32x4{0, 0, 0, 0};
+        float top[HT], sum = 0.0f;
 #pragma unroll
-        for (int d = 0; d < DT; ++d) o[x][d] = f32x4{0, 0, 0, 0};
-    float top[HT], sum = 0.0f;
-#pragma unroll
-    for (int x = 0; x < HT; ++x) top[x] = -INFINITY;
-    const float scale = a.scale * kLog2e;
-    const T* keys = static_cast<const T*>(a.keys) + g * a.key_head_stride;
+        for (float& x : top) x = -INFINITY;
+        const float scale = a.scale * kLog2e;
+        const T* keys = static_cast<const T*>(a.keys) + g * a.key_head_stride;
 
-    // rows that this wave brings in: kBring wave + n of a tile.  A row's page is looked up a tile before it is brought in, ahead of the loads that
-    // are to stay in flight: loads come back in order, and what waits for the page would wait for them.
-    const T* row = keys;
-    uint32_t there = 0, page_row = 0;
-    int32_t page = -1;
-    auto look = [&](uint32_t base) { page = c.table[by_page(min(base + wave * kBring + n % kBring, c.end - 1), &page_row)]; };
-    auto find = [&](uint32_t base) {
-        const bool is = static_cast<uint32_t>(page) < a.n_pages;
-        row = keys + (is ? static_cast<size_t>(page) : 0) * a.key_page_stride + page_row * a.key_row_stride;
-        there = static_cast<uint32_t>(__ballot(is && base + wave * kBring + n % kBring < c.end)) & ((1u << kBring) - 1);
-    };
-    auto bring = [&](uint32_t buffer) {
-        const uint32_t to = lds0 + buffer * L::kTileBytes;
-        const uint64_t addr = reinterpret_cast<uint64_t>(row);
+        // rows that this wave brings in: kBring wave + n of a tile.  A row's page is looked up a tile before it is brought in, ahead of the loads that
+        // are to stay in flight: loads come back in order, and what waits for the page would wait for them.
+        const T* row = keys;
+        uint32_t there = 0, page_row = 0;
+        int32_t page = -1;
+        auto look = [&](uint32_t base) { page = c.table[by_page(min(base + wave * kBring + n % kBring, c.end - 1), &page_row)]; };
+        auto find = [&](uint32_t base) {
+            const bool is = static_cast<uint32_t>(page) < a.n_pages;
+            row = keys + (is ? static_cast<size_t>(page) : 0) * a.key_page_stride + page_row * a.key_row_stride;
+            there = static_cast<uint32_t>(__ballot(is && base + wave * kBring + n % kBring < c.end)) & ((1u << kBring) - 1);
+        };
+        auto bring = [&](uint32_t buffer) {
+            const uint32_t to = __builtin_amdgcn_readfirstlane(lds0 + buffer * L::kTileBytes);
+            const uint64_t addr = reinterpret_cast<uint64_t>(row);
 #pragma unroll
-        for (uint32_t r = 0; r < kBring; ++r) {
-            const uint64_t base = static_cast<uint64_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(addr >> 32), r)) << 32 |
-                                  static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(addr), r));
+            for (uint32_t r = 0; r < kBring; ++r) {
+                const uint64_t base = static_cast<uint64_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(addr >> 32), r)) << 32 |
+                                      static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(addr), r));
 #pragma unroll
-            for (uint32_t plane = 0; plane < static_cast<uint32_t>(L::kPlanes); ++plane) {
-                const uint32_t word = plane * 64 + lane;
-                if (words >= (plane + 1) * 64 || word < words) direct_load(reinterpret_cast<const void*>(base), word * 16, to + plane * L::kPlaneBytes + (wave * kBring + r) * L::kPlaneRow);
+                for (uint32_t plane = 0; plane < static_cast<uint32_t>(L::kPlanes); ++plane) {
+                    const uint32_t word = plane * 64 + lane;
+                    if (words >= (plane + 1) * 64 || word < words) direct_load(reinterpret_cast<const void*>(base), word * 16, to + plane * L::kPlaneBytes + (wave * kBring + r) * L::kPlaneRow);
+                }
             }
-        }
-        if constexpr (L::kTail > 0) {
-            constexpr uint32_t kRows = 64 / L::kTail; // rows in one go
+            if constexpr (L::kTail > 0) {
+                constexpr uint32_t kRows = 64 / L::kTail; // rows in one go
 #pragma unroll
-            for (uint32_t r = 0; r < kBring; r += kRows) {
-                const uint32_t mine = r + lane / L::kTail;
-                const uint64_t base = static_cast<uint64_t>(__shfl(static_cast<uint32_t>(addr >> 32), mine)) << 32 | __shfl(static_cast<uint32_t>(addr), mine);
-                const uint32_t word = L::kPlanes * 64 + (lane % L::kTail ^ L::narrow(mine));
-                const void* from = reinterpret_cast<const unsigned char*>(base) + word * 16;
-                const uint32_t dst = to + L::kPlaneBytes * L::kPlanes + (wave * kBring + r) * (L::kTail * 16);
-                if (word < words) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"(from) : "memory", "m0");
+                for (uint32_t r = 0; r < kBring; r += kRows) {
+                    const uint32_t mine = r + lane / L::kTail;
+                    const uint64_t base = static_cast<uint64_t>(__shfl(static_cast<uint32_t>(addr >> 32), mine)) << 32 | __shfl(static_cast<uint32_t>(addr), mine);
+                    const uint32_t word = L::kPlanes * 64 + (lane % L::kTail ^ L::narrow(mine));
+                    const void* from = reinterpret_cast<const unsigned char*>(base) + word * 16;
+                    const uint32_t dst = to + L::kPlaneBytes * L::kPlanes + (wave * kBring + r) * (L::kTail * 16);
+                    if (word < words) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"(from) : "memory", "m0");
+                }
             }
-        }
-    };
-    // once the rows are there: rows that are not to be seen become zeros (a weight of zero times what a page holds behind the last row need not be zero)
-    auto settle = [&](uint32_t buffer, uint32_t mask) {
-        direct_wait();
-        if (mask != (1u << kBring) - 1) {
-            unsigned char* tile = lds + buffer * L::kTileBytes;
-            for (uint32_t r = 0; r < kBring; ++r)
-                if (!(mask >> r & 1))
-                    for (uint32_t j = lane; j < static_cast<uint32_t>(L::kWords); j += 64) *reinterpret_cast<uint4*>(tile + L::at(wave * kBring + r, j)) = make_uint4(0, 0, 0, 0);
-        }
-        if (lane == 0) masks[buffer * L::kWaves + wave] = mask;
-    };
+        };
+        // once the rows are there: rows that are not to be seen become zeros (a weight of zero times what a page holds behind the last row need not be zero)
+        auto settle = [&](uint32_t buffer, uint32_t mask) {
+            direct_wait();
+            if (mask != (1u << kBring) - 1) {
+                unsigned char* tile = lds + buffer * L::kTileBytes;
+                for (uint32_t r = 0; r < kBring; ++r)
+                    if (!(mask >> r & 1))
+                        for (uint32_t j = lane; j < static_cast<uint32_t>(L::kWords); j += 64) *reinterpret_cast<uint4*>(tile + L::at(wave * kBring + r, j)) = make_uint4(0, 0, 0, 0);
+            }
+            if (lane == 0) masks[buffer * L::kWaves + wave] = mask;
+        };
 
-    uint32_t now = 0, mask = 0;
-    if (c.begin < c.end) {
-        look(c.begin);
-        find(c.begin);
-        look(c.begin + kRowTile);
-        bring(0);
-        mask = there;
-        settle(0, mask);
-        lds_barrier();
-    }
-    for (uint32_t base = c.begin; base < c.end; base += kRowTile) {
-        const bool more = base + kRowTile < c.end;
-        if (L::kBuffers == 2 && more) {
-            find(base + kRowTile);
-            look(base + 2 * kRowTile);
-            bring(now ^ 1);
+        uint32_t now = 0, mask = 0;
+        if (c.begin < c.end) {
+            look(c.begin);
+            find(c.begin);
+            look(c.begin + L::kRows);
+            bring(0);
             mask = there;
+            settle(0, mask);
+            lds_barrier();
         }
-        const unsigned char* tile = lds + now * L::kTileBytes;
-        f32x4 s[L::kTilesPerWave];
+        for (uint32_t base = c.begin; base < c.end; base += L::kRows) {
+            const bool more = base + L::kRows < c.end;
+            if (L::kBuffers == 2 && more) {
+                find(base + L::kRows);
+                look(base + 2 * L::kRows);
+                bring(now ^ 1);
+                mask = there;
+            }
+            const unsigned char* tile = lds + now * L::kTileBytes;
+            f32x4 s[L::kTilesPerWave];
 #pragma unroll
-        for (int t = 0; t < L::kTilesPerWave; ++t) s[t] = f32x4{0, 0, 0, 0};
-        uint32_t key_at[L::kTilesPerWave], tail_at[L::kTilesPerWave]; // this lane's first word of its rows
-        constexpr int kStep = 2 * sizeof(T);                          // words in 32 columns
-#pragma unroll
-        for (int t = 0; t < L::kTilesPerWave; ++t) {
-            key_at[t] = L::at((rt0 + t) * 16 + n, quad * (kStep / 4));
-            tail_at[t] = L::kTail ? L::at((rt0 + t) * 16 + n, L::kPlanes * 64 + quad * (kStep / 4)) : 0;
-        }
-#pragma unroll
-        for (int k = 0; k < KS; ++k)
+            for (int t = 0; t < L::kTilesPerWave; ++t) s[t] = f32x4{0, 0, 0, 0};
+            uint32_t key_at[L::kTilesPerWave], tail_at[L::kTilesPerWave]; // this lane's first word of its rows
+            constexpr int kStep = 2 * sizeof(T);                          // words in 32 columns
 #pragma unroll
             for (int t = 0; t < L::kTilesPerWave; ++t) {
-                const bool tail = k * kStep >= L::kPlanes * 64;
-                auto word = [&](uint32_t j) { return tile + (tail ? tail_at[t] ^ (j - L::kPlanes * 64) << 4 : key_at[t] + (j >> 6) * L::kPlaneBytes + (j & 63) * 16); };
-                Frag<T> f;
-                if constexpr (sizeof(T) == 2) {
-                    f = *reinterpret_cast<const Frag<T>*>(word(k * kStep));
-                } else {
-                    *reinterpret_cast<f32x4*>(&f) = *reinterpret_cast<const f32x4*>(word(k * kStep));
-                    *(reinterpret_cast<f32x4*>(&f) + 1) = *reinterpret_cast<const f32x4*>(word(k * kStep + 1));
+                key_at[t] = L::at((rt0 + t) * 16 + n, quad * (kStep / 4));
+                tail_at[t] = L::kTail ? L::at((rt0 + t) * 16 + n, L::kPlanes * 64 + quad * (kStep / 4)) : 0;
+            }
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+#pragma unroll
+                for (int t = 0; t < L::kTilesPerWave; ++t) {
+                    const bool tail = k * kStep >= L::kPlanes * 64;
+                    auto word = [&](uint32_t j) { return tile + (tail ? tail_at[t] ^ (j - L::kPlanes * 64) << 4 : key_at[t] + (j >> 6) * L::kPlaneBytes + (j & 63) * 16); };
+                    Frag<T> f;
+                    if constexpr (sizeof(T) == 2) {
+                        f = *reinterpret_cast<const Frag<T>*>(word(k * kStep));
+                    } else {
+                        *reinterpret_cast<f32x4*>(&f) = *reinterpret_cast<const f32x4*>(word(k * kStep));
+                        *(reinterpret_cast<f32x4*>(&f) + 1) = *reinterpret_cast<const f32x4*>(word(k * kStep + 1));
+                    }
+                    s[t] = product16(f, q[k], s[t]);
                 }
-                s[t] = product16(f, q[k], s[t]);
+            // lane: head n of tile ht, rows (rt0 + t) * 16 + quad * 4 + r
+            float most = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < L::kTilesPerWave; ++t) {
+                const uint32_t first = (rt0 + t) * 16 + quad * 4, seen = masks[now * L::kWaves + first / kBring] >> (first % kBring);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    s[t][r] = seen >> r & 1 ? s[t][r] * scale : -INFINITY;
+                    most = fmaxf(most, s[t][r]);
+                }
             }
-        // lane: head n of tile ht, rows (rt0 + t) * 16 + quad * 4 + r
-        float most = -INFINITY;
+            most = fmaxf(most, __shfl_xor(most, 16));
+            most = fmaxf(most, __shfl_xor(most, 32));
+            const uint32_t h = ht * 16 + n;
+            if (quad == 0) parts[part * (HT * 16) + h] = most;
+            lds_barrier();
 #pragma unroll
-        for (int t = 0; t < L::kTilesPerWave; ++t) {
-            const uint32_t first = (rt0 + t) * 16 + quad * 4, seen = masks[now * L::kWaves + first / kBring] >> (first % kBring);
+            for (int x = 0; x < HT; ++x) { // every wave keeps every head's maximum, from the same numbers
+                most = parts[x * 16 + n];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                s[t][r] = seen >> r & 1 ? s[t][r] * scale : -INFINITY;
-                most = fmaxf(most, s[t][r]);
+                for (int i = 1; i < L::kParts; ++i) most = fmaxf(most, parts[i * (HT * 16) + x * 16 + n]);
+                if (__any(most > top[x] + kSlack)) {
+                    const float raised = fmaxf(top[x], most), shrink = top[x] == -INFINITY ? 0.0f : exp2_fast(top[x] - raised);
+                    top[x] = raised;
+                    if (ht == static_cast<uint32_t>(x)) sum *= shrink;
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) o[x][d] *= shrink;
+                }
             }
-        }
-        most = fmaxf(most, __shfl_xor(most, 16));
-        most = fmaxf(most, __shfl_xor(most, 32));
-        if (quad == 0) parts[part * (HT * 16) + ht * 16 + n] = most;
-        lds_barrier();
-#pragma unroll
-        for (int x = 0; x < HT; ++x) { // every wave keeps every head's maximum, from the same numbers
-            float most = parts[x * 16 + n];
-#pragma unroll
-            for (int i = 1; i < L::kParts; ++i) most = fmaxf(most, parts[i * (HT * 16) + x * 16 + n]);
-            if (__any(most > top[x] + kSlack)) {
-                const float raised = fmaxf(top[x], most), shrink = top[x] == -INFINITY ? 0.0f : exp2_fast(top[x] - raised);
-                top[x] = raised;
-                if (ht == static_cast<uint32_t>(x)) sum *= shrink;
-#pragma unroll
-                for (int d = 0; d < DT; ++d) o[x][d] *= shrink;
-            }
-        }
-        {
             float ref = top[0];
 #pragma unroll
             for (int x = 1; x < HT; ++x) ref = ht == static_cast<uint32_t>(x) ? top[x] : ref;
             const float from = (ref == -INFINITY ? 0.0f : ref) - kLift<T>;
-            const uint32_t h = ht * 16 + n;
 #pragma unroll
             for (int t = 0; t < L::kTilesPerWave; ++t) {
                 typedef T Four __attribute__((ext_vector_type(4)));
@@ -623,101 +662,101 @@ template <typename T, int KS, int HT> __global__ __launch_bounds__((RowsLayout<T
                     sum += p;
                     w[r] = from_f32<T>(p);
                 }
-                const uint32_t at = (rt0 + t) * 16 + quad * 4; // first of the four rows
-                if constexpr (sizeof(T) == 2) *reinterpret_cast<Four*>(probs + h * 128 + ((at >> 3) ^ (h >> 1 & 7)) * 16 + (at & 4) * 2) = w;
-                else *reinterpret_cast<Four*>(probs + h * 256 + ((at >> 2) ^ (h & 15)) * 16) = w;
+                const uint32_t at = ((rt0 + t) * 16 + quad * 4) * sizeof(T); // byte of the first of the four rows
+                *reinterpret_cast<Four*>(probs + L::prob(h, at >> 4) + (at & 15)) = w;
             }
-        }
-        lds_barrier();
-        uint32_t value_at[2]; // row of the first 32, the wave's first columns
+            lds_barrier();
+            uint32_t value_at[2]; // row of the first 32, the wave's first columns
 #pragma unroll
-        for (int half = 0; half < 2; ++half) value_at[half] = L::at(quad * 8 + half * 4 + (n >> 2), wave * (DT * 2) + (n >> 1 & 1)) + (n & 1) * 8;
+            for (int half = 0; half < 2; ++half) value_at[half] = L::at(quad * 8 + half * 4 + (n >> 2), wave * (DT * 2) + (n >> 1 & 1)) + (n & 1) * 8;
 #pragma unroll
-        for (int b = 0; b < kRowTile / 32; ++b) {
-            Frag<T> w[HT];
+            for (int b = 0; b < L::kRows / 32; ++b) {
+                Frag<T> w[HT];
 #pragma unroll
-            for (int x = 0; x < HT; ++x) {
-                const uint32_t h = x * 16 + n;
-                if constexpr (sizeof(T) == 2) {
-                    w[x] = *reinterpret_cast<const Frag<T>*>(probs + h * 128 + ((b * 4 + quad) ^ (h >> 1 & 7)) * 16);
-                } else {
-                    *reinterpret_cast<f32x4*>(&w[x]) = *reinterpret_cast<const f32x4*>(probs + h * 256 + ((b * 8 + quad * 2) ^ (h & 15)) * 16);
-                    *(reinterpret_cast<f32x4*>(&w[x]) + 1) = *reinterpret_cast<const f32x4*>(probs + h * 256 + ((b * 8 + quad * 2 + 1) ^ (h & 15)) * 16);
+                for (int x = 0; x < HT; ++x) {
+                    const uint32_t h = x * 16 + n;
+                    if constexpr (sizeof(T) == 2) {
+                        w[x] = *reinterpret_cast<const Frag<T>*>(probs + L::prob(h, b * 4 + quad));
+                    } else {
+                        *reinterpret_cast<f32x4*>(&w[x]) = *reinterpret_cast<const f32x4*>(probs + L::prob(h, b * 8 + quad * 2));
+                        *(reinterpret_cast<f32x4*>(&w[x]) + 1) = *reinterpret_cast<const f32x4*>(probs + L::prob(h, b * 8 + quad * 2 + 1));
+                    }
+                }
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+                    const uint32_t col = wave * (DT * 16) + d * 16; // first of 16 columns
+                    Frag<T> f;
+                    if constexpr (sizeof(T) == 2) {
+                        // a transposing read: lane 4 i + j of 16 points at columns 4 j .. of row i; each lane gets its column's four rows
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            const uint32_t at = value_at[half] + d * 32 + b * (32 * L::kPlaneRow);
+                            const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds_byte*)(tile + at));
+                            *(reinterpret_cast<s16x4*>(&f) + half) = v;
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) f[i] = *reinterpret_cast<const float*>(tile + L::at(b * 32 + quad * 8 + i, (col + n) >> 2) + (n & 3) * 4);
+                    }
+#pragma unroll
+                    for (int x = 0; x < HT; ++x) o[x][d] = product16(f, w[x], o[x][d]);
                 }
             }
+            if (more) {
+                if constexpr (L::kBuffers == 2) {
+                    settle(now ^ 1, mask);
+                    lds_barrier();
+                    now ^= 1;
+                } else {
+                    lds_barrier();
+                    find(base + L::kRows);
+                    look(base + 2 * L::kRows);
+                    bring(0);
+                    mask = there;
+                    settle(0, mask);
+                    lds_barrier();
+                }
+            }
+        }
+        // the probabilities' sums over the waves that share a head
+        __syncthreads();
+        sum += __shfl_xor(sum, 16);
+        sum += __shfl_xor(sum, 32);
+        if (quad == 0) parts[part * (HT * 16) + ht * 16 + n] = sum;
+        __syncthreads();
+#pragma unroll
+        for (int x = 0; x < HT; ++x) {
+            const uint32_t h = x * 16 + n;
+            if (h >= heads) continue;
+            float total = 0.0f;
+#pragma unroll
+            for (int i = 0; i < L::kParts; ++i) total += parts[i * (HT * 16) + h];
+            const float ref = top[x] - kLift<T>; // sums are of 2^(score - ref)
+            const uint32_t head = g * a.group + h0 + h;
+            const bool whole = c.count == 1;
+            const size_t at = static_cast<size_t>(whole ? c.query : c.slot) * a.n_heads + head;
+            const float factor = total == 0.0f ? 0.0f : 1.0f / total;
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
-                const uint32_t col = wave * (DT * 16) + d * 16; // first of 16 columns
-                Frag<T> f;
-                if constexpr (sizeof(T) == 2) {
-                    // a transposing read: lane 4 i + j of 16 points at columns 4 j .. of row i; each lane gets its column's four rows
+                const uint32_t col = wave * (DT * 16) + d * 16 + quad * 4; // rows of whole 16-byte words: dv is a multiple of 4
+                if (col >= a.dv) continue;
+                if (whole) {
+                    typedef T Four __attribute__((ext_vector_type(4)));
+                    Four f;
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const uint32_t at = value_at[half] + d * 32 + b * (32 * L::kPlaneRow);
-                        const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds_byte*)(tile + at));
-                        *(reinterpret_cast<s16x4*>(&f) + half) = v;
-                    }
+                    for (int r = 0; r < 4; ++r) f[r] = from_f32<T>(o[x][d][r] * factor);
+                    *reinterpret_cast<Four*>(static_cast<T*>(a.out) + at * a.dv + col) = f;
                 } else {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) f[i] = *reinterpret_cast<const float*>(tile + L::at(b * 32 + quad * 8 + i, (col + n) >> 2) + (n & 3) * 4);
+                    *reinterpret_cast<f32x4*>(plan.partial + at * a.dv + col) = o[x][d];
                 }
-#pragma unroll
-                for (int x = 0; x < HT; ++x) o[x][d] = product16(f, w[x], o[x][d]);
+            }
+            if (wave == 0 && quad == 0) {
+                if (!whole) plan.stats[at] = make_float2(ref, total);
+                else if (a.lse) a.lse[at] = total == 0.0f ? -INFINITY : (ref + log2f(total)) * kLn2;
             }
         }
-        if (more) {
-            if constexpr (L::kBuffers == 2) {
-                settle(now ^ 1, mask);
-                lds_barrier();
-                now ^= 1;
-            } else {
-                lds_barrier();
-                find(base + kRowTile);
-                look(base + 2 * kRowTile);
-                bring(0);
-                mask = there;
-                settle(0, mask);
-                lds_barrier();
-            }
-        }
-    }
-    // the probabilities' sums over the waves that share a head
-    __syncthreads();
-    sum += __shfl_xor(sum, 16);
-    sum += __shfl_xor(sum, 32);
-    if (quad == 0) parts[part * (HT * 16) + ht * 16 + n] = sum;
-    __syncthreads();
-#pragma unroll
-    for (int x = 0; x < HT; ++x) {
-        const uint32_t h = x * 16 + n;
-        if (h >= heads) continue;
-        float total = 0.0f;
-#pragma unroll
-        for (int i = 0; i < L::kParts; ++i) total += parts[i * (HT * 16) + h];
-        const float ref = top[x] - kLift<T>; // sums are of 2^(score - ref)
-        const uint32_t head = g * a.group + h0 + h;
-        const bool whole = c.count == 1;
-        const size_t at = static_cast<size_t>(whole ? c.query : c.slot) * a.n_heads + head;
-        const float factor = total == 0.0f ? 0.0f : 1.0f / total;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) {
-            const uint32_t col = wave * (DT * 16) + d * 16 + quad * 4; // rows of whole 16-byte words: dv is a multiple of 4
-            if (col >= a.dv) continue;
-            if (whole) {
-                typedef T Four __attribute__((ext_vector_type(4)));
-                Four f;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) f[r] = from_f32<T>(o[x][d][r] * factor);
-                *reinterpret_cast<Four*>(static_cast<T*>(a.out) + at * a.dv + col) = f;
-            } else {
-                *reinterpret_cast<f32x4*>(plan.partial + at * a.dv + col) = o[x][d];
-            }
-        }
-        if (wave == 0 && quad == 0) {
-            if (!whole) plan.stats[at] = make_float2(ref, total);
-            else if (a.lse) a.lse[at] = total == 0.0f ? -INFINITY : (ref + log2f(total)) * kLn2;
-        }
-    }
+        __syncthreads(); // the next part's queries go where this one's rows were
+    } while (walk.next(a, plan, &c));
 }
 
 // The chunks of a query joined: out = sum_k 2^(top_k - top) o_k / sum_k 2^(top_k - top) sum_k.  One workgroup per head and query; queries of one chunk are done
@@ -844,12 +883,12 @@ struct Route {
     bool rows, group; // many heads over shared rows, or heads that share a key head, on the matrix units; else one workgroup per head
     bool wide, page8;
     int ks, vb, ht;
-    uint32_t slots, target, unit, y;
+    uint32_t workers, unit, y;
     size_t stats_at, chunks_at, bytes;
 };
 
-// Slots to aim at are this many workgroups: four a compute unit even out ragged batches; where LDS holds one workgroup a compute unit, two.
-constexpr uint32_t kGroupTarget = 1024, kRowsTarget = 512;
+// Workgroups that are resident at once, on 256 compute units: all rows are cut into as many equal runs.
+constexpr uint32_t kUnits = 256;
 
 Route route_of(const AttentionArgs& a, size_t es) {
     Route r = {};
@@ -867,7 +906,7 @@ Route route_of(const AttentionArgs& a, size_t es) {
     if (r.rows) {
         r.ks = a.dk <= 320 && a.dv <= 256 ? 10 : 18;
         r.ht = a.group <= 16 || es == 4 ? 1 : a.group <= 32 ? 2 : 4; // float32 queries of 16 heads fill the registers
-        r.unit = kRowTile;
+        r.unit = 64;
         r.y = a.n_key_heads * ((a.group + r.ht * 16 - 1) / (r.ht * 16));
     } else {
         r.page8 = a.page_size % 8 == 0;
@@ -876,16 +915,13 @@ Route route_of(const AttentionArgs& a, size_t es) {
         r.unit = kChunkUnit;
         r.y = a.n_key_heads * ((a.group + 15) / 16);
     }
-    // one chunk a query where queries alone fill the machine, where no query can have more rows than one unit, or where the sum of all units might not fit 32 bits
-    const uint32_t goal = r.rows ? kRowsTarget : kGroupTarget;
+    // One workgroup a query where queries alone fill the machine several times over, where no query can have more rows than one unit, or where the sum of all units
+    // might not fit 32 bits.
+    const uint32_t resident = kUnits * (r.rows ? 1 : r.vb == 2 || es == 4 ? 2 : 3);
     const uint64_t groups = static_cast<uint64_t>(a.n_queries) * r.y, units = (static_cast<uint64_t>(a.max_pages) * a.page_size + r.unit - 1) / r.unit;
-    if (groups >= 4 * goal || units <= 1 || units * a.n_queries >= (1ull << 32)) {
-        r.slots = a.n_queries;
-        return r;
-    }
-    r.target = std::max(1u, goal / r.y);
-    r.slots = static_cast<uint32_t>(std::min<uint64_t>(static_cast<uint64_t>(r.target) + a.n_queries, a.n_queries * units));
-    const size_t parts = static_cast<size_t>(r.slots) * a.n_heads;
+    if (groups >= 8 * resident || units <= 1 || units * a.n_queries >= (1ull << 32)) return r;
+    r.workers = static_cast<uint32_t>(std::min<uint64_t>(std::max(1u, resident / r.y), a.n_queries * units));
+    const size_t parts = (static_cast<size_t>(r.workers) + a.n_queries) * a.n_heads;
     r.stats_at = (parts * a.dv * 4 + 15) / 16 * 16;
     r.chunks_at = r.stats_at + parts * 8;
     r.bytes = r.chunks_at + static_cast<size_t>(a.n_queries) * 8;
@@ -897,7 +933,7 @@ template <typename T, int KS, int HT> hipError_t launch_rows(const AttentionArgs
     // more than 64 KB of LDS has to be asked for; asking is cheap and the same every time
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(attend_rows_kernel<T, KS, HT>), hipFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((attend_rows_kernel<T, KS, HT>), dim3(r.slots, r.y), dim3(L::kThreads), L::kBytes, stream, a, plan, divider(a.page_size));
+    hipLaunchKernelGGL((attend_rows_kernel<T, KS, HT>), dim3(r.workers ? r.workers : a.n_queries, r.y), dim3(L::kThreads), L::kBytes, stream, a, plan, divider(a.page_size));
     return hipGetLastError();
 }
 
@@ -914,9 +950,9 @@ template <typename T> hipError_t launch_rows(const AttentionArgs& a, const Plan&
 
 template <typename T> hipError_t launch_split(const AttentionArgs& a, const Route& r, void* workspace, hipStream_t stream) {
     Plan plan = {};
-    plan.target = r.target;
+    plan.workers = r.workers;
     plan.unit = r.unit;
-    if (r.target) {
+    if (r.workers) {
         char* base = static_cast<char*>(workspace);
         plan.partial = reinterpret_cast<float*>(base);
         plan.stats = reinterpret_cast<float2*>(base + r.stats_at);
@@ -939,9 +975,9 @@ template <typename T> hipError_t launch_split(const AttentionArgs& a, const Rout
         if (e != hipSuccess) return e;
     } else {
         if (!kernel) return hipErrorInvalidValue;
-        hipLaunchKernelGGL(kernel, dim3(r.slots, r.y), dim3(256), 0, stream, a, plan, divider(a.page_size));
+        hipLaunchKernelGGL(kernel, dim3(r.workers ? r.workers : a.n_queries, r.y), dim3(256), 0, stream, a, plan, divider(a.page_size));
     }
-    if (r.target) hipLaunchKernelGGL((a.dv % 4 == 0 ? join_kernel<T, 4> : join_kernel<T, 1>), dim3(a.n_heads, a.n_queries), dim3(256), 0, stream, a, plan);
+    if (r.workers) hipLaunchKernelGGL((a.dv % 4 == 0 ? join_kernel<T, 4> : join_kernel<T, 1>), dim3(a.n_heads, a.n_queries), dim3(256), 0, stream, a, plan);
     return hipGetLastError();
 }
 
