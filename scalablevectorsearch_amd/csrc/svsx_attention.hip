@@ -70,12 +70,6 @@ template <typename T> __global__ __launch_bounds__(256) void attend_head_kernel(
 // A workgroup is four waves that deal the tiles of one chunk of rows among themselves.  Chunks: see plan below.
 
 constexpr int kTile = 32, kChunkUnit = 4 * kTile; // rows of a wave's tile; rows that a workgroup takes at a time
-constexpr float kSlack = 4.0f;                    // in powers of two
-constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
-
-// Probabilities are rounded to the row type before they meet the values; float16 gets them 2^8 up, so that small ones stay normal numbers (at most 2^12 with the slack).
-template <typename T> constexpr float kLift = 0.0f;
-template <> constexpr float kLift<_Float16> = 8.0f;
 
 struct Plan {
     float* partial;  // [slot][head][dv] sums of p v
@@ -184,9 +178,6 @@ template <uint32_t kThreads> struct Walk {
         return true;
     }
 };
-
-// 2^x; the hardware's instruction, denormal results are zero
-__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // The lane, as something that the compiler cannot know to be the same for every part of a worker's run: what follows from it would otherwise be kept in registers over
 // the whole run (addresses and conditions of code that runs once a part), and there are none to spare.
@@ -444,16 +435,6 @@ template <typename T, int KS, int HT> struct RowsLayout { // KS: 32-column steps
     static __device__ __forceinline__ uint32_t narrow(uint32_t r) { return kTail == 8 ? (r >> 1 & 1) << 2 : (r & 3) << 2; }
 };
 
-#pragma clang diagnostic ignored "-Winline-asm" // m0 is a reserved register; the compiler is told that it changes
-// 16 bytes per lane from base + offset to LDS at `to` + 16 * lane; not waited for (direct_wait).
-__device__ __forceinline__ void direct_load(const void* base, uint32_t offset, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory", "m0");
-}
-__device__ __forceinline__ void direct_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-// a barrier for what went through LDS: loads from HBM stay in flight over it
-__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
-
-typedef __attribute__((address_space(3))) unsigned char lds_byte;
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 template <typename T, int KS, int HT> __global__ __launch_bounds__((RowsLayout<T, KS, HT>::kThreads)) void attend_rows_kernel(const AttentionArgs a, const Plan plan, const Divider by_page) {

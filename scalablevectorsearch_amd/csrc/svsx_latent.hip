@@ -1,6 +1,10 @@
 // svsx_latent.hip -- latent attention in its expanded form, for prompts (include/svsx.h: svsx_latent_expanded_device).
+//
+// Two launches.  The first expands: keys K[head][row][dim] (the head's projection of the latent vector, then the rotary part, then zeros up to DK columns) and TRANSPOSED
+// values V[head][column][row], products of 128 x 128 tiles; and it writes the list of query tiles, because only the device knows the sequences' offsets.  The second
+// attends: prompts are long, so the products are large and the matrix units bound both.
 #include "svsx_host.h"
-#include "svsx_paged.h"
+#include "svsx_mfma.h"
 
 namespace svsx {
 namespace {
@@ -17,12 +21,13 @@ struct ExpandedArgs {
     uint32_t n_sequences, n_tokens, n_rows, n_heads, nope, rope, rank, dv;
     float scale;
     int causal, keep_rest;
+    int wide_queries, wide_out; // rows begin at 16-byte boundaries and are whole 16-byte words
 };
 
-// One workgroup per query and head, in the latent space: w_key applied to the query, w_value to the result.
+// One workgroup per query and head, in the latent space: w_key applied to the query, w_value to the result.  For heads of more than 256 columns.
 template <typename T> __global__ __launch_bounds__(256) void expanded_head_kernel(const ExpandedArgs a) {
     __shared__ RowsShared sm;
-    const uint32_t h = blockIdx.x, t = blockIdx.y;
+    const uint32_t h = blockIdx.x % a.n_heads, t = blockIdx.x / a.n_heads;
     T* out = static_cast<T*>(a.out) + (static_cast<size_t>(t) * a.n_heads + h) * a.dv;
     int lo = 0, hi = static_cast<int>(a.n_sequences); // the last sequence whose queries begin at or before t
     while (hi - lo > 1) {
@@ -60,6 +65,408 @@ template <typename T> __global__ __launch_bounds__(256) void expanded_head_kerne
     }
 }
 
+struct Space { // the first launch's results
+    void* keys;      // [head][key_rows][DK]
+    void* values;    // [head][DV][value_rows]
+    int2* tiles;     // {sequence, first query}
+    uint32_t* count; // of tiles
+    size_t key_rows, value_rows; // at least n_rows + 64: a tile of rows may begin at the last one
+    uint32_t dk, dv, most_tiles, tile_queries;
+};
+
+// A plane in LDS is rows of 128 bytes (8 words of 16), in groups of eight rows that lie 16 bytes further apart than they are long; in the third and fourth
+// row of four the two 64-byte halves are exchanged.  Eight lanes that read the same word of rows 0 .. 3 and 8 .. 11 (or 4 .. 7 and 12 .. 15: row32) meet in no bank, and a load
+// straight from HBM fills a group in whole 64-byte pieces.
+constexpr uint32_t kGroupBytes = 1024 + 16;
+__device__ __forceinline__ uint32_t plane_at(uint32_t r, uint32_t word) { return (r >> 3) * kGroupBytes + (r & 7) * 128 + ((word ^ (r & 2) << 1) << 4); }
+template <typename T> constexpr int kPlaneCols = 128 / sizeof(T);
+template <typename T> constexpr int kSteps = kPlaneCols<T> / 16; // of product32 in a plane's columns
+
+// the fragment of step `step` of row r of a plane for this half of the lanes
+template <typename T> __device__ __forceinline__ Frag<T> plane_frag(const unsigned char* plane, uint32_t r, uint32_t step, uint32_t half) {
+    if constexpr (sizeof(T) == 2) {
+        return *reinterpret_cast<const Frag<T>*>(plane + plane_at(r, step * 2 + half));
+    } else {
+        Frag<T> f;
+        *reinterpret_cast<f32x4*>(&f) = *reinterpret_cast<const f32x4*>(plane + plane_at(r, step * 4 + half * 2));
+        *(reinterpret_cast<f32x4*>(&f) + 1) = *reinterpret_cast<const f32x4*>(plane + plane_at(r, step * 4 + half * 2 + 1));
+        return f;
+    }
+}
+
+// 16 bytes of a row from column col on, zeros beyond dim
+template <typename T> struct WordOf { typedef Frag<T> type; };
+template <> struct WordOf<float> { typedef f32x4 type; };
+template <typename T> using Word = typename WordOf<T>::type;
+template <typename T, bool Wide> __device__ __forceinline__ Word<T> load_word(const T* row, uint32_t col, uint32_t dim) {
+    constexpr uint32_t kElems = 16 / sizeof(T);
+    Word<T> w = {};
+    if constexpr (Wide) {
+        if (col < dim) w = *reinterpret_cast<const Word<T>*>(row + col);
+    } else {
+#pragma unroll
+        for (uint32_t j = 0; j < kElems; ++j)
+            if (col + j < dim) w[j] = row[col + j];
+    }
+    return w;
+}
+
+// C[i][j] = sum_k A[i][k] B[j][k] for one 128 x 128 tile; four waves of 64 x 64.  row_a(i) / row_b(j): the row, NULL = zeros.  put(i, j, v): eight consecutive i of one j.
+// The next 128 bytes of every row are on their way to registers while these are multiplied.
+template <typename T, bool Wide, typename A, typename B, typename P> __device__ __forceinline__ void product_tile(unsigned char* lds, uint32_t depth, A row_a, B row_b, P put) {
+    const uint32_t t = threadIdx.x, lane = t & 63, wave = t >> 6, half = lane >> 5, r = row32(lane);
+    unsigned char* const plane_a = lds;
+    unsigned char* const plane_b = lds + 16 * kGroupBytes;
+    const T* rows[2][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        rows[0][i] = row_a((t >> 3) + 32 * i);
+        rows[1][i] = row_b((t >> 3) + 32 * i);
+    }
+    Word<T> next[2][4];
+    auto fetch = [&](uint32_t col) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) next[s][i] = rows[s][i] ? load_word<T, Wide>(rows[s][i], col + (t & 7) * (16 / sizeof(T)), depth) : Word<T>{};
+    };
+    f32x16 c[2][2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[i >> 1][i & 1] = f32x16{};
+    fetch(0);
+    for (uint32_t col = 0; col < depth; col += kPlaneCols<T>) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            *reinterpret_cast<Word<T>*>(plane_a + plane_at((t >> 3) + 32 * i, t & 7)) = next[0][i];
+            *reinterpret_cast<Word<T>*>(plane_b + plane_at((t >> 3) + 32 * i, t & 7)) = next[1][i];
+        }
+        __syncthreads();
+        if (col + kPlaneCols<T> < depth) fetch(col + kPlaneCols<T>);
+#pragma unroll
+        for (int s = 0; s < kSteps<T>; ++s) {
+            Frag<T> fa[2], fb[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                fa[i] = plane_frag<T>(plane_a, (wave & 1) * 64 + i * 32 + r, s, half);
+                fb[i] = plane_frag<T>(plane_b, (wave >> 1) * 64 + i * 32 + r, s, half);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) c[i >> 1][i & 1] = product32(fa[i >> 1], fb[i & 1], c[i >> 1][i & 1]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                Frag<T> v;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = from_f32<T>(c[i][j][8 * k + e]);
+                put((wave & 1) * 64 + i * 32 + 16 * k + 8 * half, (wave >> 1) * 64 + j * 32 + r, v);
+            }
+}
+
+struct ExpandGrid { // workgroups of the first launch: keys, values, rotary parts, then one for the tiles
+    uint32_t key_i, keys, value_i, values, copies;
+};
+
+// the queries of sequence i, inside the array
+__device__ __forceinline__ void queries_of(const ExpandedArgs& a, uint32_t i, uint32_t* begin, uint32_t* end) {
+    const int32_t b = a.query_offsets[i], e = a.query_offsets[i + 1], n = static_cast<int32_t>(a.n_tokens);
+    *begin = static_cast<uint32_t>(b < 0 ? 0 : b < n ? b : n);
+    *end = static_cast<uint32_t>(e < static_cast<int32_t>(*begin) ? static_cast<int32_t>(*begin) : e < n ? e : n);
+}
+
+// the query tiles, sequence by sequence, and zeros for the queries of no sequence
+template <typename T> __device__ __forceinline__ void list_tiles(const ExpandedArgs& a, const Space& w, uint32_t* sh) {
+    const uint32_t t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    uint32_t base = 0;
+    for (uint32_t first = 0; first < a.n_sequences; first += 256) {
+        uint32_t b = 0, e = 0;
+        if (first + t < a.n_sequences) queries_of(a, first + t, &b, &e);
+        const uint32_t n = (e - b + w.tile_queries - 1) / w.tile_queries;
+        uint32_t incl = n;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const uint32_t u = __shfl_up(incl, off);
+            if (lane >= static_cast<uint32_t>(off)) incl += u;
+        }
+        __syncthreads();
+        if (lane == 63) sh[wave] = incl;
+        __syncthreads();
+        uint32_t at = base + incl - n;
+        for (uint32_t k = 0; k < 4; ++k) {
+            at += k < wave ? sh[k] : 0;
+            base += sh[k];
+        }
+        for (uint32_t k = 0; k < n; ++k)
+            if (at + k < w.most_tiles) w.tiles[at + k] = make_int2(static_cast<int>(first + t), static_cast<int>(b + k * w.tile_queries));
+    }
+    if (t == 0) *w.count = base < w.most_tiles ? base : w.most_tiles;
+}
+
+template <typename T, bool Wide> __global__ __launch_bounds__(256) void expand_kernel(const ExpandedArgs a, const Space w, const ExpandGrid grid) {
+    __shared__ __align__(16) unsigned char lds[2 * 16 * kGroupBytes];
+    uint32_t block = blockIdx.x;
+    const T* rows = static_cast<const T*>(a.rows);
+    T* keys = static_cast<T*>(w.keys);
+    T* values = static_cast<T*>(w.values);
+    if (block < grid.keys) { // i: (head, column), j: row
+        const uint32_t i0 = block % grid.key_i * 128, j0 = block / grid.key_i * 128, n = a.n_heads * a.nope;
+        const T* wk = static_cast<const T*>(a.w_key);
+        product_tile<T, Wide>(
+            lds, a.rank, [&](uint32_t i) { return i0 + i < n ? wk + static_cast<size_t>(i0 + i) * a.rank : nullptr; },
+            [&](uint32_t j) { return j0 + j < a.n_rows ? rows + static_cast<size_t>(j0 + j) * a.row_stride : nullptr; },
+            [&](uint32_t i, uint32_t j, const Frag<T>& v) {
+                if (j0 + j >= a.n_rows) return;
+                if (a.nope % 8 == 0) {
+                    const uint32_t h = (i0 + i) / a.nope, col = (i0 + i) % a.nope;
+                    if (h < a.n_heads) *reinterpret_cast<Frag<T>*>(keys + (h * w.key_rows + j0 + j) * w.dk + col) = v;
+                } else {
+                    for (uint32_t e = 0; e < 8; ++e) {
+                        const uint32_t h = (i0 + i + e) / a.nope, col = (i0 + i + e) % a.nope;
+                        if (h < a.n_heads) keys[(h * w.key_rows + j0 + j) * w.dk + col] = v[e];
+                    }
+                }
+            });
+        return;
+    }
+    block -= grid.keys;
+    if (block < grid.values) { // i: row, j: (head, column); zeros in columns beyond the head's and rows beyond the last
+        const uint32_t i0 = block % grid.value_i * 128, j0 = block / grid.value_i * 128, n = a.n_heads * w.dv;
+        const T* wv = static_cast<const T*>(a.w_value);
+        product_tile<T, Wide>(
+            lds, a.rank, [&](uint32_t i) { return i0 + i < a.n_rows ? rows + static_cast<size_t>(i0 + i) * a.row_stride : nullptr; },
+            [&](uint32_t j) {
+                const uint32_t h = (j0 + j) / w.dv, col = (j0 + j) % w.dv;
+                return j0 + j < n && col < a.dv ? wv + (static_cast<size_t>(h) * a.dv + col) * a.rank : nullptr;
+            },
+            [&](uint32_t i, uint32_t j, const Frag<T>& v) {
+                if (i0 + i < w.value_rows && j0 + j < n) *reinterpret_cast<Frag<T>*>(values + static_cast<size_t>(j0 + j) * w.value_rows + i0 + i) = v;
+            });
+        return;
+    }
+    block -= grid.values;
+    if (block < grid.copies) { // the rotary part behind every head's columns, zeros behind that
+        constexpr uint32_t kElems = 16 / sizeof(T);
+        const bool words = Wide && a.nope % kElems == 0 && a.rope % kElems == 0;
+        const uint32_t step = words ? kElems : 1, per_row = (w.dk - a.nope) / step;
+        const uint64_t all = static_cast<uint64_t>(a.n_heads) * a.n_rows * per_row;
+        for (uint64_t at = static_cast<uint64_t>(block) * 256 + threadIdx.x; at < all; at += static_cast<uint64_t>(grid.copies) * 256) {
+            const uint32_t col = static_cast<uint32_t>(at % per_row) * step;
+            const uint64_t hr = at / per_row;
+            const uint32_t r = static_cast<uint32_t>(hr % a.n_rows), h = static_cast<uint32_t>(hr / a.n_rows);
+            const T* from = rows + static_cast<size_t>(r) * a.row_stride + a.rank + col;
+            T* to = keys + (h * w.key_rows + r) * w.dk + a.nope + col;
+            if (words) *reinterpret_cast<Word<T>*>(to) = col < a.rope ? *reinterpret_cast<const Word<T>*>(from) : Word<T>{};
+            else *to = col < a.rope ? *from : from_f32<T>(0.0f);
+        }
+        if (!a.keep_rest) { // queries before the first sequence and behind the last
+            uint32_t b = a.n_tokens, e = a.n_tokens, unused;
+            if (a.n_sequences > 0) {
+                queries_of(a, 0, &b, &unused);
+                queries_of(a, a.n_sequences - 1, &unused, &e);
+                e = e < b ? b : e;
+            }
+            const size_t per_query = static_cast<size_t>(a.n_heads) * a.dv, rest = (b + (a.n_tokens - e)) * per_query;
+            T* out = static_cast<T*>(a.out);
+            for (size_t at = static_cast<size_t>(block) * 256 + threadIdx.x; at < rest; at += static_cast<size_t>(grid.copies) * 256)
+                out[at < b * per_query ? at : at + (e - b) * per_query] = from_f32<T>(0.0f);
+        }
+        return;
+    }
+    list_tiles<T>(a, w, reinterpret_cast<uint32_t*>(lds));
+}
+
+// One workgroup: NW waves of 32 queries of one head, over the rows they see in tiles of 64 (float32: 32), two buffers in LDS, one barrier a tile.
+//   S^T = K Q^T    rows x queries, queries as fragments in registers; with row32, a lane's results are eight consecutive rows at a time for its query:
+//   O^T = V^T P^T  the probabilities are the next product's fragments where they are.
+// A query is a lane's column throughout, so its maximum, sum and rescaling need one exchange between two lanes.  Per 64 rows a wave has 1280 cycles of products
+// (DK 192, DV 128) against 320 of LDS reads, which eight waves share.
+template <typename T, int DK, int DV, int NW> struct PromptLayout {
+    static constexpr uint32_t kRows = kPlaneCols<T>; // of a tile: a plane of V^T
+    static constexpr int kKeyPlanes = DK / kPlaneCols<T>, kTiles = kRows / 32;
+    static constexpr uint32_t kKeyPlane = kRows / 8 * kGroupBytes, kKeyBytes = kKeyPlanes * kKeyPlane, kBytes = kKeyBytes + DV / 8 * kGroupBytes;
+    static constexpr uint32_t kLoads = kKeyPlanes * (kRows / 8) + DV / 8; // of 1 KB
+    static_assert(2 * kBytes <= 160 * 1024, "LDS");
+};
+template <typename T, int DK, int DV, int NW> __global__ __launch_bounds__(NW * 64) void prompt_kernel(const ExpandedArgs a, const Space w) {
+    typedef PromptLayout<T, DK, DV, NW> L;
+    extern __shared__ __align__(16) unsigned char lds[];
+    const uint32_t count = *w.count, turn = blockIdx.x / a.n_heads, h = blockIdx.x % a.n_heads; // a head's tiles on one of the eight L2s where heads are a multiple of 8
+    if (turn >= count) return;
+    const int2 tile = w.tiles[count - 1 - turn]; // a sequence's last queries see the most rows: they go first
+    const uint32_t seq = __builtin_amdgcn_readfirstlane(tile.x), q0 = __builtin_amdgcn_readfirstlane(tile.y);
+    uint32_t qb, qe;
+    queries_of(a, seq, &qb, &qe);
+    qe = __builtin_amdgcn_readfirstlane(qe);
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, r = row32(lane);
+    // rows [begin, end) of the sequence, inside the array; a query at t sees those up to t + shift
+    const int32_t rb = a.row_offsets[seq], re = a.row_offsets[seq + 1], shift = re - a.query_offsets[seq + 1];
+    const int32_t begin = __builtin_amdgcn_readfirstlane(rb < 0 ? 0 : rb), end = __builtin_amdgcn_readfirstlane(re < static_cast<int32_t>(a.n_rows) ? re : static_cast<int32_t>(a.n_rows));
+    auto sees = [&](uint32_t t) { // the last row that query t sees; less than begin: none
+        const int32_t own = static_cast<int32_t>(t) + shift;
+        return a.causal && own < end - 1 ? own : end - 1;
+    };
+    const uint32_t q_last = min(qe, q0 + NW * 32) - 1, mine = min(q0 + wave * 32 + (lane & 31), q_last);
+    const int32_t see = sees(mine);
+    const int32_t wave_first = __builtin_amdgcn_readfirstlane(sees(min(q0 + wave * 32, q_last))), wave_last = __builtin_amdgcn_readfirstlane(sees(min(q0 + wave * 32 + 31, q_last)));
+    const int32_t base0 = begin & ~7, group_last = __builtin_amdgcn_readfirstlane(sees(q_last)); // V^T is read in 16-byte words
+
+    Frag<T> q[DK / 16];
+    {
+        const T* row = static_cast<const T*>(a.queries) + mine * a.query_stride + h * a.query_head_stride;
+        const uint32_t dk = a.nope + a.rope;
+#pragma unroll
+        for (int s = 0; s < DK / 16; ++s) q[s] = a.wide_queries ? load_frag<T, true>(row, s * 16 + half * 8, dk) : load_frag<T, false>(row, s * 16 + half * 8, dk);
+    }
+    f32x16 o[DV / 32];
+#pragma unroll
+    for (int d = 0; d < DV / 32; ++d) o[d] = f32x16{};
+    float top = -INFINITY, sum = 0.0f;
+    const float scale = a.scale * kLog2e;
+
+    const T* keys = static_cast<const T*>(w.keys) + h * w.key_rows * DK;
+    const T* values = static_cast<const T*>(w.values) + static_cast<size_t>(h) * DV * w.value_rows;
+    const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_byte*)lds));
+    // a lane's place in a group of eight rows: row lane / 8, and the word that belongs at lane % 8 there
+    const uint32_t in_row = ((lane & 7) ^ (lane >> 3 & 2) << 1) * 16;
+    const uint32_t key_offset = (lane >> 3) * (DK * sizeof(T)) + in_row, value_offset = (lane >> 3) * static_cast<uint32_t>(w.value_rows * sizeof(T)) + in_row;
+    auto bring = [&](uint32_t buffer, int32_t base) {
+        const uint32_t to = lds0 + buffer * L::kBytes;
+#pragma unroll
+        for (uint32_t i = 0; i < (L::kLoads + NW - 1) / NW; ++i) {
+            const uint32_t k = i * NW + wave;
+            if (k < L::kKeyPlanes * (L::kRows / 8)) {
+                const uint32_t plane = k / (L::kRows / 8), group = k % (L::kRows / 8);
+                direct_load(keys + (static_cast<size_t>(base) + group * 8) * DK + plane * kPlaneCols<T>, key_offset, __builtin_amdgcn_readfirstlane(to + plane * L::kKeyPlane + group * kGroupBytes));
+            } else if (k < L::kLoads) {
+                const uint32_t group = k - L::kKeyPlanes * (L::kRows / 8);
+                direct_load(values + static_cast<size_t>(group) * 8 * w.value_rows + base, value_offset, __builtin_amdgcn_readfirstlane(to + L::kKeyBytes + group * kGroupBytes));
+            }
+        }
+    };
+
+    uint32_t now = 0;
+    if (base0 <= group_last) bring(0, base0);
+    direct_wait();
+    lds_barrier();
+    for (int32_t base = base0; base <= group_last; base += L::kRows) {
+        if (base + static_cast<int32_t>(L::kRows) <= group_last) bring(now ^ 1, base + L::kRows);
+        if (base <= wave_last) {
+            const unsigned char* kt = lds + now * L::kBytes;
+            const unsigned char* vt = kt + L::kKeyBytes;
+            f32x16 s[L::kTiles];
+#pragma unroll
+            for (int x = 0; x < L::kTiles; ++x) {
+                s[x] = f32x16{};
+#pragma unroll
+                for (int k = 0; k < DK / 16; ++k) s[x] = product32(plane_frag<T>(kt + k / kSteps<T> * L::kKeyPlane, x * 32 + r, k % kSteps<T>, half), q[k], s[x]);
+            }
+            // register 8 i + e of s[x]: row base + 32 x + 16 i + 8 half + e
+            const bool edge = base < begin || base + static_cast<int32_t>(L::kRows) - 1 > wave_first;
+            float most = -INFINITY;
+#pragma unroll
+            for (int x = 0; x < L::kTiles; ++x)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[x][i] *= scale;
+            if (edge) {
+#pragma unroll
+                for (int x = 0; x < L::kTiles; ++x)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int32_t row = base + 32 * x + 16 * (i >> 3) + 8 * static_cast<int32_t>(half) + (i & 7);
+                        if (row < begin || row > see) s[x][i] = -INFINITY;
+                    }
+            }
+#pragma unroll
+            for (int x = 0; x < L::kTiles; ++x)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) most = fmaxf(most, s[x][i]);
+            most = fmaxf(most, __shfl_xor(most, 32));
+            if (__any(most > top + kSlack)) {
+                const float raised = fmaxf(top, most), shrink = top == -INFINITY ? 0.0f : exp2_fast(top - raised);
+                top = raised;
+                sum *= shrink;
+#pragma unroll
+                for (int d = 0; d < DV / 32; ++d) o[d] *= shrink;
+            }
+            const float from = (top == -INFINITY ? 0.0f : top) - kLift<T>;
+            Frag<T> p[2 * L::kTiles];
+#pragma unroll
+            for (int x = 0; x < L::kTiles; ++x)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float e = exp2_fast(s[x][i] - from);
+                    sum += e;
+                    p[2 * x + (i >> 3)][i & 7] = from_f32<T>(e);
+                }
+            bool odd = false; // values of rows that some query does not see, infinite or not a number: a weight of zero does not take them away
+            if (edge) {
+                uint32_t worst = 0;
+#pragma unroll
+                for (int d = 0; d < DV / 32; ++d)
+#pragma unroll
+                    for (int k = 0; k < 2 * L::kTiles; ++k) {
+                        const Frag<T> f = plane_frag<T>(vt, d * 32 + r, k, half);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) worst |= !__builtin_isfinite(to_f32(f[e]));
+                    }
+                odd = __any(worst != 0);
+            }
+            if (!odd) {
+#pragma unroll
+                for (int k = 0; k < 2 * L::kTiles; ++k)
+#pragma unroll
+                    for (int d = 0; d < DV / 32; ++d) o[d] = product32(plane_frag<T>(vt, d * 32 + r, k, half), p[k], o[d]);
+            } else { // row by row, each added where it is seen
+#pragma unroll
+                for (int k = 0; k < 2 * L::kTiles; ++k)
+                    for (int e = 0; e < 16; ++e) {
+                        const int32_t row = base + 16 * k + e;
+                        const bool here = (e >> 3) == static_cast<int>(half), seen = row >= begin && row <= see;
+#pragma unroll
+                        for (int d = 0; d < DV / 32; ++d) {
+                            Frag<T> f = plane_frag<T>(vt, d * 32 + r, k, half), one = p[k];
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) {
+                                if (!here || j != (e & 7)) f[j] = one[j] = from_f32<T>(0.0f);
+                            }
+                            const f32x16 add = product32(f, one, f32x16{});
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) o[d][j] = seen ? o[d][j] + add[j] : o[d][j];
+                        }
+                    }
+            }
+        }
+        direct_wait();
+        lds_barrier();
+        now ^= 1;
+    }
+    sum += __shfl_xor(sum, 32);
+    if (q0 + wave * 32 + (lane & 31) > q_last) return;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    T* out = static_cast<T*>(a.out) + (static_cast<size_t>(mine) * a.n_heads + h) * a.dv;
+#pragma unroll
+    for (int d = 0; d < DV / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t col = d * 32 + 16 * i + 8 * half;
+            Frag<T> f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = from_f32<T>(o[d][8 * i + e] * inv);
+            if (a.wide_out) {
+                if (col < a.dv) *reinterpret_cast<Frag<T>*>(out + col) = f;
+            } else {
+#pragma unroll
+                for (uint32_t e = 0; e < 8; ++e)
+                    if (col + e < a.dv) out[col + e] = f[e];
+            }
+        }
+}
+
 int check_expanded(const svsx_expanded_desc* d, ExpandedArgs* a) {
     if (!d) return fail(SVSX_INVALID_ARGUMENT, "null argument");
     if (d->struct_size != sizeof(svsx_expanded_desc))
@@ -71,14 +478,94 @@ int check_expanded(const svsx_expanded_desc* d, ExpandedArgs* a) {
         return fail(SVSX_INVALID_ARGUMENT, "rank (%zu) + rope_dim (%zu), nope_dim (%zu) + rope_dim and value_dim (%zu) must be in [1, %d]", d->rank, d->rope_dim, d->nope_dim,
                     d->value_dim, kMaxDim);
     const size_t limit = size_t(1) << 31;
-    if (d->n_tokens > 65535 * size_t(16) || d->n_rows >= limit || d->n_sequences >= limit) return fail(SVSX_INVALID_ARGUMENT, "too many queries, rows or sequences in one call");
+    if (d->n_tokens >= limit || d->n_rows >= (size_t(1) << 27) - 128 || d->n_sequences >= limit || d->n_tokens * d->n_heads >= limit || d->n_sequences * d->n_heads >= limit ||
+        d->n_heads * (d->nope_dim + kMaxDim) >= limit) return fail(SVSX_INVALID_ARGUMENT, "too many queries, rows or sequences in one call");
     if (d->n_tokens > 0 && (!d->d_queries || !d->d_out || !d->d_w_value || (d->nope_dim > 0 && !d->d_w_key))) return fail(SVSX_INVALID_ARGUMENT, "null argument");
     if (d->n_tokens > 0 && d->n_sequences > 0 && (!d->d_query_offsets || !d->d_row_offsets || (d->n_rows > 0 && !d->d_rows))) return fail(SVSX_INVALID_ARGUMENT, "null argument");
     *a = ExpandedArgs{d->d_queries, d->d_rows, d->d_w_key, d->d_w_value, d->d_query_offsets, d->d_row_offsets, d->d_out, d->query_stride, d->query_head_stride, d->row_stride,
                       static_cast<uint32_t>(d->n_sequences), static_cast<uint32_t>(d->n_tokens), static_cast<uint32_t>(d->n_rows), static_cast<uint32_t>(d->n_heads),
                       static_cast<uint32_t>(d->nope_dim), static_cast<uint32_t>(d->rope_dim), static_cast<uint32_t>(d->rank), static_cast<uint32_t>(d->value_dim), d->scale,
-                      d->causal, d->keep_rest};
+                      d->causal, d->keep_rest, 0, 0};
+    const size_t es = paged_dtype_size(d->dtype), dk = d->nope_dim + d->rope_dim;
+    a->wide_queries = dk % 8 == 0 && ((reinterpret_cast<size_t>(d->d_queries) | d->query_stride * es | d->query_head_stride * es) & 15) == 0;
+    a->wide_out = d->value_dim % 8 == 0 && (reinterpret_cast<size_t>(d->d_out) & 15) == 0;
     return SVSX_SUCCESS;
+}
+
+// How a call is answered; decided from sizes, types, strides and addresses alone.
+struct PromptRoute {
+    bool tiles; // on the matrix units; else one workgroup per query and head (heads of more than 256 columns)
+    bool wide;
+    int dk, dv, waves;
+    Space space;
+    size_t values_at, tiles_at, count_at, bytes;
+};
+
+PromptRoute route_of(const ExpandedArgs& a, size_t es) {
+    PromptRoute r = {};
+    const uint32_t dk = a.nope + a.rope;
+    r.tiles = dk <= 256 && a.dv <= 256;
+    if (!r.tiles) return r;
+    r.dk = dk <= 128 && a.dv <= 128 ? 128 : dk <= 192 && a.dv <= 128 ? 192 : 256;
+    r.dv = r.dk == 256 ? 256 : a.dv <= 64 ? 64 : 128;
+    const size_t elems = 16 / es;
+    r.wide = a.rank % elems == 0 && ((reinterpret_cast<size_t>(a.rows) | reinterpret_cast<size_t>(a.w_key) | reinterpret_cast<size_t>(a.w_value) | a.row_stride * es) & 15) == 0;
+    // Eight waves share a tile's rows where that leaves every compute unit a workgroup; float32 and 256-column heads have no registers for two waves a SIMD.
+    r.waves = es == 2 && r.dk <= 192 && static_cast<uint64_t>(a.n_tokens) * a.n_heads >= 256 * 256 ? 8 : 4;
+    Space& w = r.space;
+    w.dk = r.dk;
+    w.dv = r.dv;
+    w.tile_queries = r.waves * 32;
+    w.most_tiles = (a.n_tokens + w.tile_queries - 1) / w.tile_queries + a.n_sequences;
+    w.key_rows = static_cast<size_t>(a.n_rows) + 64;
+    w.value_rows = (static_cast<size_t>(a.n_rows) + 63) / 64 * 64 + 64;
+    r.values_at = a.n_heads * w.key_rows * r.dk * es;
+    r.tiles_at = r.values_at + a.n_heads * w.value_rows * r.dv * es;
+    r.count_at = r.tiles_at + static_cast<size_t>(w.most_tiles) * 8;
+    r.bytes = r.count_at + 4;
+    return r;
+}
+
+template <typename T, int DK, int DV, int NW> hipError_t launch_prompt(const ExpandedArgs& a, const Space& w, hipStream_t stream) {
+    typedef PromptLayout<T, DK, DV, NW> L;
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(prompt_kernel<T, DK, DV, NW>), hipFuncAttributeMaxDynamicSharedMemorySize, 2 * L::kBytes);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((prompt_kernel<T, DK, DV, NW>), dim3(w.most_tiles * a.n_heads), dim3(NW * 64), 2 * L::kBytes, stream, a, w);
+    return hipGetLastError();
+}
+
+template <typename T> hipError_t launch_expanded(const ExpandedArgs& a, PromptRoute& r, void* workspace, hipStream_t stream) {
+    if (!r.tiles) {
+        hipLaunchKernelGGL(expanded_head_kernel<T>, dim3(a.n_heads * a.n_tokens), dim3(256), 0, stream, a);
+        return hipGetLastError();
+    }
+    char* base = static_cast<char*>(workspace);
+    Space& w = r.space;
+    w.keys = base;
+    w.values = base + r.values_at;
+    w.tiles = reinterpret_cast<int2*>(base + r.tiles_at);
+    w.count = reinterpret_cast<uint32_t*>(base + r.count_at);
+    ExpandGrid g = {};
+    g.key_i = (a.n_heads * a.nope + 127) / 128;
+    g.keys = g.key_i * ((a.n_rows + 127) / 128);
+    g.value_i = static_cast<uint32_t>((w.value_rows + 127) / 128);
+    g.values = g.value_i * ((a.n_heads * r.dv + 127) / 128);
+    g.copies = 1024;
+    if (static_cast<uint64_t>(g.key_i) * ((a.n_rows + 127) / 128) + static_cast<uint64_t>(g.value_i) * ((a.n_heads * r.dv + 127) / 128) >= (1ull << 31) - 2048) return hipErrorInvalidValue;
+    if (static_cast<uint64_t>(w.most_tiles) * a.n_heads >= (1ull << 31)) return hipErrorInvalidValue;
+    auto expand = r.wide ? expand_kernel<T, true> : expand_kernel<T, false>;
+    hipLaunchKernelGGL(expand, dim3(g.keys + g.values + g.copies + 1), dim3(256), 0, stream, a, w, g);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || w.most_tiles == 0) return e;
+    if constexpr (sizeof(T) == 2) {
+        if (r.waves == 8) {
+            if (r.dk == 128) return r.dv == 64 ? launch_prompt<T, 128, 64, 8>(a, w, stream) : launch_prompt<T, 128, 128, 8>(a, w, stream);
+            return r.dv == 64 ? launch_prompt<T, 192, 64, 8>(a, w, stream) : launch_prompt<T, 192, 128, 8>(a, w, stream);
+        }
+    }
+    if (r.dk == 128) return r.dv == 64 ? launch_prompt<T, 128, 64, 4>(a, w, stream) : launch_prompt<T, 128, 128, 4>(a, w, stream);
+    if (r.dk == 192) return r.dv == 64 ? launch_prompt<T, 192, 64, 4>(a, w, stream) : launch_prompt<T, 192, 128, 4>(a, w, stream);
+    return launch_prompt<T, 256, 256, 4>(a, w, stream);
 }
 
 } // namespace
@@ -90,22 +577,23 @@ int svsx_latent_expanded_workspace(const svsx_expanded_desc* desc, size_t* bytes
     ExpandedArgs a;
     if (const int rc = check_expanded(desc, &a)) return rc;
     if (!bytes) return fail(SVSX_INVALID_ARGUMENT, "null argument");
-    *bytes = 0;
+    *bytes = a.n_tokens ? route_of(a, paged_dtype_size(desc->dtype)).bytes : 0;
     return SVSX_SUCCESS;
 }
 
 int svsx_latent_expanded_device(const svsx_expanded_desc* desc, void* d_workspace, size_t workspace_bytes, void* hip_stream) {
-    (void)d_workspace;
-    (void)workspace_bytes;
     ExpandedArgs a;
     if (const int rc = check_expanded(desc, &a)) return rc;
     if (a.n_tokens == 0) return SVSX_SUCCESS;
-    if (a.n_tokens > 65535) return fail(SVSX_INVALID_ARGUMENT, "too many queries in one call");
+    PromptRoute r = route_of(a, paged_dtype_size(desc->dtype));
+    if (r.bytes > 0 && (!d_workspace || workspace_bytes < r.bytes || reinterpret_cast<uintptr_t>(d_workspace) % 16 != 0))
+        return fail(SVSX_INVALID_ARGUMENT, "a workspace of %zu bytes, aligned to 16, is needed", r.bytes);
     DeviceScope on(desc->device);
     if (on.error != hipSuccess) return fail(SVSX_RUNTIME_ERROR, "hipSetDevice(%d) failed: %s", desc->device, hipGetErrorString(on.error));
-    auto kernel = desc->dtype == SVSX_F32 ? expanded_head_kernel<float> : desc->dtype == SVSX_F16 ? expanded_head_kernel<_Float16> : expanded_head_kernel<bf16_t>;
-    hipLaunchKernelGGL(kernel, dim3(a.n_heads, a.n_tokens), dim3(256), 0, static_cast<hipStream_t>(hip_stream), a);
-    const hipError_t e = hipGetLastError();
+    const hipStream_t s = static_cast<hipStream_t>(hip_stream);
+    const hipError_t e = desc->dtype == SVSX_F32   ? launch_expanded<float>(a, r, d_workspace, s)
+                         : desc->dtype == SVSX_F16 ? launch_expanded<_Float16>(a, r, d_workspace, s)
+                                                   : launch_expanded<bf16_t>(a, r, d_workspace, s);
     return e == hipSuccess ? SVSX_SUCCESS : fail(SVSX_RUNTIME_ERROR, "expanded attention launch failed: %s", hipGetErrorString(e));
 }
 

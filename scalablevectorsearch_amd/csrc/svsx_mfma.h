@@ -28,6 +28,40 @@ __device__ __forceinline__ f32x4 product16(f32x8 a, f32x8 b, f32x4 c) {
     return c;
 }
 
+// product32(a, b, c): c[32 x 32] += A[32 x 16] B[16 x 32]; lane l holds row / column l % 32, elements 8 (l / 32) .. + 7 of the 16; of c column l % 32, and in register
+// 4 i + j row 8 i + 4 (l / 32) + j.
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+__device__ __forceinline__ f32x16 product32(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 product32(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 product32(f32x8 a, f32x8 b, f32x16 c) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+    return c;
+}
+// Which of 32 rows a lane of product32 reads so that registers 8 i .. 8 i + 7 of the result are rows 16 i + 8 (l / 32) .. + 7, eight consecutive ones: a fragment of the
+// next product as they are, and one 16-byte word of a 16-bit type.
+__device__ __forceinline__ uint32_t row32(uint32_t lane) { return (lane & 0x13) | (lane & 8) >> 1 | (lane & 4) << 1; }
+
+// 2^x; the hardware's instruction, denormal results are zero
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+
+// The running maximum of a softmax is raised only when a score exceeds it by more than kSlack powers of two.
+constexpr float kSlack = 4.0f;
+// Probabilities are rounded to the row type before they meet the values; float16 gets them 2^8 up, so that small ones stay normal numbers (at most 2^12 with the slack).
+template <typename T> inline constexpr float kLift = 0.0f;
+template <> inline constexpr float kLift<_Float16> = 8.0f;
+
+#pragma clang diagnostic ignored "-Winline-asm" // m0 is a reserved register; the compiler is told that it changes
+// 16 bytes per lane from base + offset to LDS at `to` + 16 * lane; not waited for (direct_wait).
+__device__ __forceinline__ void direct_load(const void* base, uint32_t offset, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory", "m0");
+}
+__device__ __forceinline__ void direct_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// a barrier for what went through LDS: loads from HBM stay in flight over it
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+typedef __attribute__((address_space(3))) unsigned char lds_byte;
+
 // elements [col, col + 8) of a row of `dim`; zero beyond it.  Wide: rows begin at 16-byte boundaries and dim is a multiple of 8.
 template <typename T, bool Wide> __device__ __forceinline__ Frag<T> load_frag(const T* row, uint32_t col, uint32_t dim) {
     Frag<T> f = {};
