@@ -5,6 +5,7 @@
 // attends: prompts are long, so the products are large and the matrix units bound both.
 #include "svsx_host.h"
 #include "svsx_mfma.h"
+#include <type_traits>
 
 namespace svsx {
 namespace {
@@ -292,6 +293,51 @@ template <typename T, int DK, int DV, int NW> struct PromptLayout {
     static constexpr uint32_t kLoads = kKeyPlanes * (kRows / 8) + DV / 8; // of 1 KB
     static_assert(2 * kBytes <= 160 * 1024, "LDS");
 };
+template <typename T> __device__ __forceinline__ bool all_finite(const Frag<T>& f) { // no exponent of all ones
+    constexpr uint32_t kExponent = sizeof(T) == 4 ? 0x7F800000u : std::is_same<T, _Float16>::value ? 0x7C00u : 0x7F80u;
+    bool fine = true;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        uint32_t bits;
+        if constexpr (sizeof(T) == 4) bits = __builtin_bit_cast(uint32_t, static_cast<float>(f[e]));
+        else bits = __builtin_bit_cast(uint16_t, static_cast<T>(f[e]));
+        fine = fine && (bits & kExponent) != kExponent;
+    }
+    return fine;
+}
+
+// One query by one wave, over the expanded rows [begin, last] alone: its lanes across the columns.
+template <typename T, int DK, int DV> __device__ void slow_query(const ExpandedArgs& a, const Space& w, uint32_t t, uint32_t h, int32_t begin, int32_t last) {
+    const uint32_t lane = threadIdx.x & 63, dk = a.nope + a.rope;
+    const T* row = static_cast<const T*>(a.queries) + t * a.query_stride + h * a.query_head_stride;
+    const T* keys = static_cast<const T*>(w.keys) + h * w.key_rows * DK;
+    const T* values = static_cast<const T*>(w.values) + static_cast<size_t>(h) * DV * w.value_rows;
+    float q[DK / 64], o[DV / 64], top = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < DK / 64; ++i) q[i] = lane + 64 * i < dk ? to_f32(row[lane + 64 * i]) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < DV / 64; ++i) o[i] = 0.0f;
+    for (int32_t r = begin; r <= last; ++r) {
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < DK / 64; ++i) s = fmaf(q[i], to_f32(keys[static_cast<size_t>(r) * DK + lane + 64 * i]), s);
+#pragma unroll
+        for (int off = 32; off >= 1; off >>= 1) s += __shfl_xor(s, off);
+        s *= a.scale;
+        if (s == -INFINITY) continue;
+        const float raised = s > top || s != s ? s : top, was = expf(top - raised), p = expf(s - raised);
+        top = raised;
+        sum = fmaf(sum, was, p);
+#pragma unroll
+        for (int i = 0; i < DV / 64; ++i) o[i] = fmaf(p, to_f32(values[(lane + 64 * i) * w.value_rows + r]), o[i] * was);
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    T* out = static_cast<T*>(a.out) + (static_cast<size_t>(t) * a.n_heads + h) * a.dv;
+#pragma unroll
+    for (int i = 0; i < DV / 64; ++i)
+        if (lane + 64 * i < a.dv) out[lane + 64 * i] = from_f32<T>(o[i] * inv);
+}
+
 template <typename T, int DK, int DV, int NW> __global__ __launch_bounds__(NW * 64) void prompt_kernel(const ExpandedArgs a, const Space w) {
     typedef PromptLayout<T, DK, DV, NW> L;
     extern __shared__ __align__(16) unsigned char lds[];
@@ -350,6 +396,7 @@ template <typename T, int DK, int DV, int NW> __global__ __launch_bounds__(NW * 
     };
 
     uint32_t now = 0;
+    bool odd = false;
     if (base0 <= group_last) bring(0, base0);
     direct_wait();
     lds_barrier();
@@ -403,47 +450,24 @@ template <typename T, int DK, int DV, int NW> __global__ __launch_bounds__(NW * 
                     sum += e;
                     p[2 * x + (i >> 3)][i & 7] = from_f32<T>(e);
                 }
-            bool odd = false; // values of rows that some query does not see, infinite or not a number: a weight of zero does not take them away
-            if (edge) {
-                uint32_t worst = 0;
+            if (edge) { // values of rows that some query does not see: a weight of zero does not take away what is infinite or not a number
 #pragma unroll
                 for (int d = 0; d < DV / 32; ++d)
 #pragma unroll
-                    for (int k = 0; k < 2 * L::kTiles; ++k) {
-                        const Frag<T> f = plane_frag<T>(vt, d * 32 + r, k, half);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) worst |= !__builtin_isfinite(to_f32(f[e]));
-                    }
-                odd = __any(worst != 0);
+                    for (int k = 0; k < 2 * L::kTiles; ++k) odd |= __any(!all_finite<T>(plane_frag<T>(vt, d * 32 + r, k, half)));
             }
-            if (!odd) {
 #pragma unroll
-                for (int k = 0; k < 2 * L::kTiles; ++k)
+            for (int k = 0; k < 2 * L::kTiles; ++k)
 #pragma unroll
-                    for (int d = 0; d < DV / 32; ++d) o[d] = product32(plane_frag<T>(vt, d * 32 + r, k, half), p[k], o[d]);
-            } else { // row by row, each added where it is seen
-#pragma unroll
-                for (int k = 0; k < 2 * L::kTiles; ++k)
-                    for (int e = 0; e < 16; ++e) {
-                        const int32_t row = base + 16 * k + e;
-                        const bool here = (e >> 3) == static_cast<int>(half), seen = row >= begin && row <= see;
-#pragma unroll
-                        for (int d = 0; d < DV / 32; ++d) {
-                            Frag<T> f = plane_frag<T>(vt, d * 32 + r, k, half), one = p[k];
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) {
-                                if (!here || j != (e & 7)) f[j] = one[j] = from_f32<T>(0.0f);
-                            }
-                            const f32x16 add = product32(f, one, f32x16{});
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) o[d][j] = seen ? o[d][j] + add[j] : o[d][j];
-                        }
-                    }
-            }
+                for (int d = 0; d < DV / 32; ++d) o[d] = product32(plane_frag<T>(vt, d * 32 + r, k, half), p[k], o[d]);
         }
         direct_wait();
         lds_barrier();
         now ^= 1;
+    }
+    if (odd) { // anew, row by row, from the rows that each query sees
+        for (uint32_t t = q0 + wave * 32; t <= min(q_last, q0 + wave * 32 + 31); ++t) slow_query<T, DK, DV>(a, w, t, h, begin, sees(t));
+        return;
     }
     sum += __shfl_xor(sum, 32);
     if (q0 + wave * 32 + (lane & 31) > q_last) return;
