@@ -281,17 +281,19 @@ template <typename T, bool Wide> __global__ __launch_bounds__(256) void expand_k
     list_tiles<T>(a, w, reinterpret_cast<uint32_t*>(lds));
 }
 
-// One workgroup: NW waves of 32 queries of one head, over the rows they see in tiles of 64 (float32: 32), two buffers in LDS, one barrier a tile.
+// One workgroup: NW waves of 32 queries of one head, over the rows they see in tiles of 64 (float32: 32).
 //   S^T = K Q^T    rows x queries, queries as fragments in registers; with row32, a lane's results are eight consecutive rows at a time for its query:
 //   O^T = V^T P^T  the probabilities are the next product's fragments where they are.
 // A query is a lane's column throughout, so its maximum, sum and rescaling need one exchange between two lanes.  Per 64 rows a wave has 1280 cycles of products
-// (DK 192, DV 128) against 320 of LDS reads, which eight waves share.
+// (DK 192, DV 128) against 320 of LDS reads, which eight waves share, and about 1000 of softmax on the vector units: so of the two waves on a SIMD, one does its products (a tile's
+// scores and the last tile's values) while the other does its softmax, and they change over at a barrier.
 template <typename T, int DK, int DV, int NW> struct PromptLayout {
     static constexpr uint32_t kRows = kPlaneCols<T>; // of a tile: a plane of V^T
     static constexpr int kKeyPlanes = DK / kPlaneCols<T>, kTiles = kRows / 32;
-    static constexpr uint32_t kKeyPlane = kRows / 8 * kGroupBytes, kKeyBytes = kKeyPlanes * kKeyPlane, kBytes = kKeyBytes + DV / 8 * kGroupBytes;
-    static constexpr uint32_t kLoads = kKeyPlanes * (kRows / 8) + DV / 8; // of 1 KB
-    static_assert(2 * kBytes <= 160 * 1024, "LDS");
+    static constexpr uint32_t kGroups = kRows / 8, kKeyPlane = kGroups * kGroupBytes, kKeyBytes = kKeyPlanes * kKeyPlane, kValueBytes = DV / 8 * kGroupBytes;
+    static constexpr uint32_t kAhead = 3 * kKeyBytes + 2 * kValueBytes <= 160 * 1024 ? 2 : 1; // tiles that keys are brought in ahead of their use
+    static constexpr uint32_t kBytes = (kAhead + 1) * kKeyBytes + 2 * kValueBytes;
+    static_assert(kBytes <= 160 * 1024 && kGroups % 4 == 0 && DV % 32 == 0, "LDS; loads of four waves");
 };
 template <typename T> __device__ __forceinline__ bool all_finite(const Frag<T>& f) { // no exponent of all ones
     constexpr uint32_t kExponent = sizeof(T) == 4 ? 0x7F800000u : std::is_same<T, _Float16>::value ? 0x7C00u : 0x7F80u;
@@ -366,13 +368,23 @@ template <typename T, int DK, int DV, int NW> __global__ __launch_bounds__(NW * 
         const T* row = static_cast<const T*>(a.queries) + mine * a.query_stride + h * a.query_head_stride;
         const uint32_t dk = a.nope + a.rope;
 #pragma unroll
-        for (int s = 0; s < DK / 16; ++s) q[s] = a.wide_queries ? load_frag<T, true>(row, s * 16 + half * 8, dk) : load_frag<T, false>(row, s * 16 + half * 8, dk);
+        for (int s = 0; s < DK / 16; ++s) {
+            q[s] = a.wide_queries ? load_frag<T, true>(row, s * 16 + half * 8, dk) : load_frag<T, false>(row, s * 16 + half * 8, dk);
+            // the scale's sign goes into the queries (exactly), so that the largest product has the largest score; so does a scale of zero
+            if (!(a.scale > 0.0f)) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) q[s][e] = a.scale < 0.0f ? -q[s][e] : from_f32<T>(0.0f);
+            }
+        }
     }
+    // the compiler is to wait for the queries here: in the loop, where it cannot tell them from the rows on their way, it would wait for both
+#pragma unroll
+    for (int s = 0; s < DK / 16; ++s) asm volatile("" : "+v"(q[s]));
     f32x16 o[DV / 32];
 #pragma unroll
     for (int d = 0; d < DV / 32; ++d) o[d] = f32x16{};
     float top = -INFINITY, sum = 0.0f;
-    const float scale = a.scale * kLog2e;
+    const float scale = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * kLog2e;
 
     const T* keys = static_cast<const T*>(w.keys) + h * w.key_rows * DK;
     const T* values = static_cast<const T*>(w.values) + static_cast<size_t>(h) * DV * w.value_rows;
@@ -380,90 +392,120 @@ template <typename T, int DK, int DV, int NW> __global__ __launch_bounds__(NW * 
     // a lane's place in a group of eight rows: row lane / 8, and the word that belongs at lane % 8 there
     const uint32_t in_row = ((lane & 7) ^ (lane >> 3 & 2) << 1) * 16;
     const uint32_t key_offset = (lane >> 3) * (DK * sizeof(T)) + in_row, value_offset = (lane >> 3) * static_cast<uint32_t>(w.value_rows * sizeof(T)) + in_row;
-    auto bring = [&](uint32_t buffer, int32_t base) {
-        const uint32_t to = lds0 + buffer * L::kBytes;
+    // Four waves bring in a tile's keys, or its values, 1 KB a load.  Issuing a load takes a wave about a hundred cycles, so it is done beside the softmax.
+    const uint32_t of_four = wave & 3;
+    unsigned char* const value_buffers = lds + (L::kAhead + 1) * L::kKeyBytes;
+    auto bring_keys = [&](uint32_t buffer, int32_t base) {
+        const T* from = keys + (static_cast<size_t>(base) + of_four * 8) * DK;
+        const uint32_t to = lds0 + buffer * L::kKeyBytes + of_four * kGroupBytes;
 #pragma unroll
-        for (uint32_t i = 0; i < (L::kLoads + NW - 1) / NW; ++i) {
-            const uint32_t k = i * NW + wave;
-            if (k < L::kKeyPlanes * (L::kRows / 8)) {
-                const uint32_t plane = k / (L::kRows / 8), group = k % (L::kRows / 8);
-                direct_load(keys + (static_cast<size_t>(base) + group * 8) * DK + plane * kPlaneCols<T>, key_offset, __builtin_amdgcn_readfirstlane(to + plane * L::kKeyPlane + group * kGroupBytes));
-            } else if (k < L::kLoads) {
-                const uint32_t group = k - L::kKeyPlanes * (L::kRows / 8);
-                direct_load(values + static_cast<size_t>(group) * 8 * w.value_rows + base, value_offset, __builtin_amdgcn_readfirstlane(to + L::kKeyBytes + group * kGroupBytes));
-            }
-        }
+        for (uint32_t k = 0; k < L::kKeyPlanes * L::kGroups; k += 4)
+            direct_load(from + (k % L::kGroups) * 8 * DK + k / L::kGroups * kPlaneCols<T>, key_offset,
+                        __builtin_amdgcn_readfirstlane(to + k / L::kGroups * L::kKeyPlane + k % L::kGroups * kGroupBytes));
+    };
+    auto bring_values = [&](uint32_t buffer, int32_t base) {
+        const T* from = values + static_cast<size_t>(of_four) * 8 * w.value_rows + base;
+        const uint32_t to = lds0 + (L::kAhead + 1) * L::kKeyBytes + buffer * L::kValueBytes + of_four * kGroupBytes;
+#pragma unroll
+        for (uint32_t k = 0; k < DV / 8; k += 4) direct_load(from + k * 8 * w.value_rows, value_offset, __builtin_amdgcn_readfirstlane(to + k * kGroupBytes));
     };
 
-    uint32_t now = 0;
-    bool odd = false;
-    if (base0 <= group_last) bring(0, base0);
-    direct_wait();
-    lds_barrier();
-    for (int32_t base = base0; base <= group_last; base += L::kRows) {
-        if (base + static_cast<int32_t>(L::kRows) <= group_last) bring(now ^ 1, base + L::kRows);
-        if (base <= wave_last) {
-            const unsigned char* kt = lds + now * L::kBytes;
-            const unsigned char* vt = kt + L::kKeyBytes;
-            f32x16 s[L::kTiles];
+    // Where eight waves run, the second four are half a tile behind the first: tile i's products ("M": its scores, and tile i - 1's values) stand beside the other four's softmax
+    // ("S") of i - 1 or i.  During its S(i) the first four bring in the keys of tile i + kAhead, the second four (or the only ones) the values of i + 1: the buffers
+    // those go to were last read in M(i - 1) and M(i), which a barrier has ended for all.
+    const bool paired = NW > 4, second = wave >= 4;
+    const int32_t step = L::kRows;
+    uint32_t key_buffer = 0, value_buffer = 0; // of this tile
+    bool odd = false, pending = false, pending_edge = false; // a tile whose probabilities wait for its values
+    f32x16 s[L::kTiles];
+    Frag<T> p[2 * L::kTiles];
+    auto add_values = [&](uint32_t buffer) {
+        const unsigned char* vt = value_buffers + buffer * L::kValueBytes;
+        if (pending_edge) { // values of rows that some query does not see: a weight of zero does not take away what is infinite or not a number
 #pragma unroll
-            for (int x = 0; x < L::kTiles; ++x) {
-                s[x] = f32x16{};
+            for (int d = 0; d < DV / 32; ++d)
 #pragma unroll
-                for (int k = 0; k < DK / 16; ++k) s[x] = product32(plane_frag<T>(kt + k / kSteps<T> * L::kKeyPlane, x * 32 + r, k % kSteps<T>, half), q[k], s[x]);
+                for (int k = 0; k < 2 * L::kTiles; ++k) odd |= __any(!all_finite<T>(plane_frag<T>(vt, d * 32 + r, k, half)));
+        }
+#pragma unroll
+        for (int k = 0; k < 2 * L::kTiles; ++k)
+#pragma unroll
+            for (int d = 0; d < DV / 32; ++d) o[d] = product32(plane_frag<T>(vt, d * 32 + r, k, half), p[k], o[d]);
+        reads_ahead<T, 2 * L::kTiles * (DV / 32), 4>();
+    };
+    if (base0 <= group_last) {
+        if (!second) {
+            bring_keys(0, base0);
+            if (L::kAhead > 1 && base0 + step <= group_last) bring_keys(1, base0 + step);
+            bring_values(0, base0);
+        }
+        direct_wait();
+        lds_barrier();
+        if (second) lds_barrier();
+        for (int32_t base = base0; base <= group_last; base += step) {
+            const bool active = base <= wave_last, edge = base < begin || base + step - 1 > wave_first;
+            if (active) {
+                const unsigned char* kt = lds + key_buffer * L::kKeyBytes;
+#pragma unroll
+                for (int x = 0; x < L::kTiles; ++x) s[x] = f32x16{};
+#pragma unroll
+                for (int k = 0; k < DK / 16; ++k)
+#pragma unroll
+                    for (int x = 0; x < L::kTiles; ++x) s[x] = product32(plane_frag<T>(kt + k / kSteps<T> * L::kKeyPlane, x * 32 + r, k % kSteps<T>, half), q[k], s[x]);
+                reads_ahead<T, DK / 16 * L::kTiles, 4>();
             }
-            // register 8 i + e of s[x]: row base + 32 x + 16 i + 8 half + e
-            const bool edge = base < begin || base + static_cast<int32_t>(L::kRows) - 1 > wave_first;
-            float most = -INFINITY;
+            if (pending) add_values(value_buffer ^ 1);
+            if (second) direct_wait(); // the values of this tile, which M(i + 1) of the first four is about to read
+            lds_barrier();
+            if (!second) {
+                if (L::kAhead > 1) direct_wait(); // what S(i - 1) brought: the keys of tile i + 1
+                const int32_t far = base + static_cast<int32_t>(L::kAhead) * step;
+                if (far <= group_last) bring_keys(key_buffer ? key_buffer - 1 : L::kAhead, far);
+            }
+            if ((!paired || second) && base + step <= group_last) bring_values(value_buffer ^ 1, base + step);
+            if (active) {
+                // register 8 i + e of s[x]: row base + 32 x + 16 i + 8 half + e
+                if (edge) {
 #pragma unroll
-            for (int x = 0; x < L::kTiles; ++x)
+                    for (int x = 0; x < L::kTiles; ++x)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[x][i] *= scale;
-            if (edge) {
+                        for (int i = 0; i < 16; ++i) {
+                            const int32_t row = base + 32 * x + 16 * (i >> 3) + 8 * static_cast<int32_t>(half) + (i & 7);
+                            if (row < begin || row > see) s[x][i] = -INFINITY;
+                        }
+                }
+                float most = -INFINITY;
+#pragma unroll
+                for (int x = 0; x < L::kTiles; ++x)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) most = fmaxf(most, s[x][i]);
+                most = fmaxf(most, __shfl_xor(most, 32)) * scale;
+                if (__any(most > top + kSlack)) {
+                    const float raised = fmaxf(top, most), shrink = top == -INFINITY ? 0.0f : exp2_fast(top - raised);
+                    top = raised;
+                    sum *= shrink;
+#pragma unroll
+                    for (int d = 0; d < DV / 32; ++d) o[d] *= shrink;
+                }
+                const float from = (top == -INFINITY ? 0.0f : top) - kLift<T>;
 #pragma unroll
                 for (int x = 0; x < L::kTiles; ++x)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const int32_t row = base + 32 * x + 16 * (i >> 3) + 8 * static_cast<int32_t>(half) + (i & 7);
-                        if (row < begin || row > see) s[x][i] = -INFINITY;
+                        const float e = exp2_fast(fmaf(s[x][i], scale, -from));
+                        sum += e;
+                        p[2 * x + (i >> 3)][i & 7] = from_f32<T>(e);
                     }
             }
-#pragma unroll
-            for (int x = 0; x < L::kTiles; ++x)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) most = fmaxf(most, s[x][i]);
-            most = fmaxf(most, __shfl_xor(most, 32));
-            if (__any(most > top + kSlack)) {
-                const float raised = fmaxf(top, most), shrink = top == -INFINITY ? 0.0f : exp2_fast(top - raised);
-                top = raised;
-                sum *= shrink;
-#pragma unroll
-                for (int d = 0; d < DV / 32; ++d) o[d] *= shrink;
-            }
-            const float from = (top == -INFINITY ? 0.0f : top) - kLift<T>;
-            Frag<T> p[2 * L::kTiles];
-#pragma unroll
-            for (int x = 0; x < L::kTiles; ++x)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float e = exp2_fast(s[x][i] - from);
-                    sum += e;
-                    p[2 * x + (i >> 3)][i & 7] = from_f32<T>(e);
-                }
-            if (edge) { // values of rows that some query does not see: a weight of zero does not take away what is infinite or not a number
-#pragma unroll
-                for (int d = 0; d < DV / 32; ++d)
-#pragma unroll
-                    for (int k = 0; k < 2 * L::kTiles; ++k) odd |= __any(!all_finite<T>(plane_frag<T>(vt, d * 32 + r, k, half)));
-            }
-#pragma unroll
-            for (int k = 0; k < 2 * L::kTiles; ++k)
-#pragma unroll
-                for (int d = 0; d < DV / 32; ++d) o[d] = product32(plane_frag<T>(vt, d * 32 + r, k, half), p[k], o[d]);
+            pending = active;
+            pending_edge = edge;
+            if (!second && L::kAhead == 1) direct_wait();
+            lds_barrier();
+            key_buffer = key_buffer == L::kAhead ? 0 : key_buffer + 1;
+            value_buffer ^= 1;
         }
-        direct_wait();
-        lds_barrier();
-        now ^= 1;
+        if (pending) add_values(value_buffer ^ 1);
+        if (paired && !second) lds_barrier();
     }
     if (odd) { // anew, row by row, from the rows that each query sees
         for (uint32_t t = q0 + wave * 32; t <= min(q_last, q0 + wave * 32 + 31); ++t) slow_query<T, DK, DV>(a, w, t, h, begin, sees(t));
@@ -552,9 +594,9 @@ PromptRoute route_of(const ExpandedArgs& a, size_t es) {
 
 template <typename T, int DK, int DV, int NW> hipError_t launch_prompt(const ExpandedArgs& a, const Space& w, hipStream_t stream) {
     typedef PromptLayout<T, DK, DV, NW> L;
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(prompt_kernel<T, DK, DV, NW>), hipFuncAttributeMaxDynamicSharedMemorySize, 2 * L::kBytes);
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(prompt_kernel<T, DK, DV, NW>), hipFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((prompt_kernel<T, DK, DV, NW>), dim3(w.most_tiles * a.n_heads), dim3(NW * 64), 2 * L::kBytes, stream, a, w);
+    hipLaunchKernelGGL((prompt_kernel<T, DK, DV, NW>), dim3(w.most_tiles * a.n_heads), dim3(NW * 64), L::kBytes, stream, a, w);
     return hipGetLastError();
 }
 

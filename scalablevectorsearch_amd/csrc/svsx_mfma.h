@@ -62,6 +62,19 @@ __device__ __forceinline__ void direct_wait() { asm volatile("s_waitcnt vmcnt(0)
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 typedef __attribute__((address_space(3))) unsigned char lds_byte;
 
+// Orders the block that it stands in: LDS reads Ahead fragments ahead of the products that use them (N fragments and N products in all; reads and instructions
+// per fragment and product by type).  Left to itself the compiler reads each fragment right before its product and waits for it.
+template <typename T, int N, int Ahead> __device__ __forceinline__ void reads_ahead() {
+    constexpr int kReads = sizeof(T) == 2 ? 1 : 2, kProducts = sizeof(T) == 2 ? 1 : 8;
+    __builtin_amdgcn_sched_group_barrier(0x100, Ahead * kReads, 0);
+#pragma unroll
+    for (int i = 0; i < N - Ahead; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, kProducts, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, kReads, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, Ahead * kProducts, 0);
+}
+
 // elements [col, col + 8) of a row of `dim`; zero beyond it.  Wide: rows begin at 16-byte boundaries and dim is a multiple of 8.
 template <typename T, bool Wide> __device__ __forceinline__ Frag<T> load_frag(const T* row, uint32_t col, uint32_t dim) {
     Frag<T> f = {};
