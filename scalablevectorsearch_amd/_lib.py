@@ -212,15 +212,15 @@ def lib() -> C.CDLL:
             if not os.environ.get("SVSX_LIB"):
                 raise
         try:  # operators over paged rows: likewise absent from an older build
-            L.svsx_cache_workspace.argtypes = [C.POINTER(CacheDesc), C.c_size_t, C.POINTER(C.c_size_t)]
-            L.svsx_cache_extend_device.argtypes = [C.POINTER(CacheDesc), C.c_void_p, C.c_void_p, C.c_size_t, C.c_size_t, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]
-            L.svsx_cache_write_device.argtypes = [C.POINTER(CacheDesc), C.c_size_t, C.c_void_p, C.c_size_t, C.c_void_p, C.c_size_t, C.c_size_t, C.c_void_p, C.c_size_t,
+            L.svsx_cache_workspace.argtypes = [C.c_void_p, C.c_size_t, C.POINTER(C.c_size_t)]
+            L.svsx_cache_extend_device.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_size_t, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]
+            L.svsx_cache_write_device.argtypes = [C.c_void_p, C.c_size_t, C.c_void_p, C.c_size_t, C.c_void_p, C.c_size_t, C.c_size_t, C.c_void_p, C.c_size_t,
                                                   C.c_size_t, C.c_void_p]
-            L.svsx_cache_copy_device.argtypes = [C.POINTER(CacheDesc), C.c_void_p, C.c_void_p, C.c_size_t, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p]
-            L.svsx_cache_free_device.argtypes = [C.POINTER(CacheDesc), C.c_void_p, C.c_size_t, C.c_void_p]
-            L.svsx_cache_compact_device.argtypes = [C.POINTER(CacheDesc), C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]
-            L.svsx_paged_attention_workspace.argtypes = [C.POINTER(AttentionDesc), C.POINTER(C.c_size_t)]
-            L.svsx_paged_attention_device.argtypes = [C.POINTER(AttentionDesc), C.c_void_p, C.c_size_t, C.c_void_p]
+            L.svsx_cache_copy_device.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p]
+            L.svsx_cache_free_device.argtypes = [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]
+            L.svsx_cache_compact_device.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]
+            L.svsx_paged_attention_workspace.argtypes = [C.c_void_p, C.c_void_p]  # packed by attention.py; AttentionDesc is the layout
+            L.svsx_paged_attention_device.argtypes = [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]
             L.svsx_latent_expanded_workspace.argtypes = [C.POINTER(ExpandedDesc), C.POINTER(C.c_size_t)]
             L.svsx_latent_expanded_device.argtypes = [C.POINTER(ExpandedDesc), C.c_void_p, C.c_size_t, C.c_void_p]
         except AttributeError:

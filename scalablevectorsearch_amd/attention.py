@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import struct
 
 from . import _lib
 
@@ -22,15 +23,20 @@ def _invalid(message: str) -> _lib.SvsxError:
     return _lib.SvsxError(_lib.INVALID_ARGUMENT, message)
 
 
+def _elsewhere(name, x) -> _lib.SvsxError:
+    return _invalid(f"{name} must be on one GPU with the other arrays, is on {x.device}")
+
+
 def _on_device(name, x, device) -> None:
     if x.device != device or device.type != "cuda":
-        raise _invalid(f"{name} must be on one GPU with the other arrays, is on {x.device}")
+        raise _elsewhere(name, x)
 
 
-def _stream(device) -> int:
+def _stream(index: int) -> int:
+    """torch's current stream of a device, as the library takes it."""
     import torch
 
-    return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def _rows(name, x, dims):
@@ -38,6 +44,10 @@ def _rows(name, x, dims):
         raise _invalid(f"{name} must have {dims} dimensions, has {x.dim()}")
     if x.stride(-1) != 1 and x.shape[-1] > 1:
         raise _invalid(f"rows of {name} must be contiguous")
+
+
+# svsx_attention_desc, laid out by struct: a third of the time that filling a ctypes structure takes
+_ATTENTION = struct.Struct("@Nii10NP2NP3NP3N3PfPP")
 
 
 def paged_attention(queries, keys, values, table, lengths, sequences=None, value_dim: int | None = None, scale: float | None = None, return_lse: bool = False):
@@ -53,54 +63,73 @@ def paged_attention(queries, keys, values, table, lengths, sequences=None, value
     logarithm of each softmax's denominator [n, heads] float32, which joins results over parts of the rows.  A query with no rows gives zeros and -inf."""
     import torch
 
-    _rows("queries", queries, 3)
-    _rows("keys", keys, 4)
+    if queries.dim() != 3 or keys.dim() != 4:
+        raise _invalid(f"queries must have 3 dimensions and keys 4, have {queries.dim()} and {keys.dim()}")
     n, heads, dim = queries.shape
-    pages, key_heads, page_size, key_dim = keys.shape
-    dtype, device = queries.dtype, queries.device
-    if dtype not in _dtypes():
+    pages, key_heads, page_size, key_dim = key_shape = keys.shape
+    qs, ks = queries.stride(), keys.stride()
+    dtype, device = queries.dtype, queries.get_device()
+    code = _dtypes().get(dtype)
+    if code is None:
         raise _invalid(f"unsupported row type {dtype} (float32, float16, bfloat16)")
     if keys.dtype != dtype or key_dim != dim:
         raise _invalid(f"keys must be {dtype} rows of {dim}, are {keys.dtype} rows of {key_dim}")
+    if (qs[2] != 1 or ks[3] != 1) and dim > 1:
+        raise _invalid("rows of queries and keys must be contiguous")
     if values is not None:
-        _rows("values", values, 4)
-        if values.dtype != dtype or values.shape[:3] != keys.shape[:3]:
-            raise _invalid(f"values must be {dtype} {list(keys.shape[:3])} rows, are {values.dtype} {list(values.shape[:3])}")
+        if values.dim() != 4 or values.dtype != dtype or values.shape[:3] != key_shape[:3]:
+            raise _invalid(f"values must be {dtype} {list(key_shape[:3])} rows, are {values.dtype} {list(values.shape)}")
+        columns, vs = values.shape[3], values.stride()
+        if vs[3] != 1 and columns > 1:
+            raise _invalid("rows of values must be contiguous")
         if value_dim is None:
-            value_dim = values.shape[3]
-        if value_dim != values.shape[3]:
-            raise _invalid(f"value_dim {value_dim} of values with {values.shape[3]} columns")
-        _on_device("values", values, device)
-    elif value_dim is None:
-        value_dim = dim
-    if table.dim() != 2 or table.dtype != torch.int32 or (table.stride(1) != 1 and table.shape[1] > 1):
+            value_dim = columns
+        elif value_dim != columns:
+            raise _invalid(f"value_dim {value_dim} of values with {columns} columns")
+        if values.get_device() != device:
+            raise _elsewhere("values", values)
+        value_ptr = values.data_ptr()
+    else:
+        vs, value_ptr = (0, 0, 0), 0
+        if value_dim is None:
+            value_dim = dim
+    if table.dim() != 2 or table.dtype != torch.int32:
         raise _invalid("table must be int32 [sequences, pages], rows contiguous")
-    if lengths.dtype != torch.int32 or lengths.shape != table.shape[:1] or not lengths.is_contiguous():
+    table_sequences, max_pages = table.shape
+    ts = table.stride()
+    if ts[1] != 1 and max_pages > 1:
+        raise _invalid("table must be int32 [sequences, pages], rows contiguous")
+    if lengths.dtype != torch.int32 or lengths.shape != (table_sequences,) or not lengths.is_contiguous():
         raise _invalid("lengths must be int32, one for each row of table")
+    sequence_ptr = 0
     if sequences is not None:
         if sequences.dtype != torch.int32 or sequences.shape != (n,) or not sequences.is_contiguous():
             raise _invalid("sequences must be int32, one for each query")
-        _on_device("sequences", sequences, device)
-    elif table.shape[0] != n:
-        raise _invalid(f"{n} queries and {table.shape[0]} sequences: say which with `sequences`")
-    for name, x in (("queries", queries), ("keys", keys), ("table", table), ("lengths", lengths)):
-        _on_device(name, x, device)
-    out = torch.empty((n, heads, value_dim), dtype=dtype, device=device)
-    lse = torch.empty((n, heads), dtype=torch.float32, device=device) if return_lse else None
-    qs, ks = queries.stride(), keys.stride()
-    vs = values.stride() if values is not None else (0, 0, 0)
-    desc = _lib.AttentionDesc(
-        C.sizeof(_lib.AttentionDesc), device.index, _dtypes()[dtype], n, heads, key_heads, dim, value_dim, pages, page_size, table.shape[0], table.shape[1],
-        table.stride(0), queries.data_ptr(), qs[0], qs[1], keys.data_ptr(), ks[0], ks[1], ks[2],
-        values.data_ptr() if values is not None else None, vs[0], vs[1], vs[2],
-        table.data_ptr(), lengths.data_ptr(), sequences.data_ptr() if sequences is not None else None, dim**-0.5 if scale is None else scale,
-        out.data_ptr(), lse.data_ptr() if return_lse else None)
-    ref = C.byref(desc)
-    size = C.c_size_t()
+        if sequences.get_device() != device:
+            raise _elsewhere("sequences", sequences)
+        sequence_ptr = sequences.data_ptr()
+    elif table_sequences != n:
+        raise _invalid(f"{n} queries and {table_sequences} sequences: say which with `sequences`")
+    if device < 0 or keys.get_device() != device or table.get_device() != device or lengths.get_device() != device:
+        for name, x in (("queries", queries), ("keys", keys), ("table", table), ("lengths", lengths)):
+            _on_device(name, x, queries.device)
+    if value_dim < 0:
+        raise _invalid("value_dim must be positive")
+    out = queries.new_empty((n, heads, value_dim))
+    lse = queries.new_empty((n, heads), dtype=torch.float32) if return_lse else None
+    desc = _ATTENTION.pack(
+        _ATTENTION.size, device, code, n, heads, key_heads, dim, value_dim, pages, page_size, table_sequences, max_pages, ts[0], queries.data_ptr(), qs[0], qs[1],
+        keys.data_ptr(), ks[0], ks[1], ks[2], value_ptr, vs[0], vs[1], vs[2], table.data_ptr(), lengths.data_ptr(), sequence_ptr, dim**-0.5 if scale is None else scale,
+        out.data_ptr(), lse.data_ptr() if return_lse else 0)
     L = _lib.lib()
-    _lib.check(L.svsx_paged_attention_workspace(ref, C.byref(size)))
-    ws = torch.empty(size.value, dtype=torch.uint8, device=device) if size.value else None
-    _lib.check(L.svsx_paged_attention_device(ref, ws.data_ptr() if ws is not None else None, size.value, _stream(device)))
+    size = C.c_size_t()
+    rc = L.svsx_paged_attention_workspace(desc, C.byref(size))
+    if rc == 0:
+        bytes_ = size.value
+        ws = queries.new_empty(bytes_, dtype=torch.uint8) if bytes_ else None
+        rc = L.svsx_paged_attention_device(desc, ws.data_ptr() if bytes_ else 0, bytes_, _stream(device))
+    if rc:
+        _lib.check(rc)
     return (out, lse) if return_lse else out
 
 
@@ -162,5 +191,5 @@ def latent_attention_expanded(queries, rows, w_key, w_value, query_offsets, row_
     L = _lib.lib()
     _lib.check(L.svsx_latent_expanded_workspace(ref, C.byref(size)))
     ws = torch.empty(size.value, dtype=torch.uint8, device=device) if size.value else None
-    _lib.check(L.svsx_latent_expanded_device(ref, ws.data_ptr() if ws is not None else None, size.value, _stream(device)))
+    _lib.check(L.svsx_latent_expanded_device(ref, ws.data_ptr() if ws is not None else None, size.value, _stream(device.index)))
     return out

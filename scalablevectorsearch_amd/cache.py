@@ -8,18 +8,9 @@ from __future__ import annotations
 import ctypes as C
 
 from . import _lib
-from .attention import _dtypes, _invalid, _on_device, _stream, paged_attention
+from .attention import _dtypes, _elsewhere, _invalid, _on_device, _stream, paged_attention
 
-
-def _list(x, device, name):
-    import torch
-
-    if not isinstance(x, torch.Tensor):
-        x = torch.as_tensor(x, dtype=torch.int32).to(device)
-    if x.dtype != torch.int32 or x.dim() != 1 or not x.is_contiguous():
-        raise _invalid(f"{name} must be a contiguous vector of int32")
-    _on_device(name, x, device)
-    return x
+_MOST = 4096  # entries of one call (include/svsx.h)
 
 
 class PagedCache:
@@ -68,69 +59,84 @@ class PagedCache:
                     raise _invalid(f"{name} must be contiguous")
         self.keys, self.values, self.table, self.lengths, self.refs = keys, values, table, lengths, refs
         self.failures = torch.zeros(1, dtype=torch.int32, device=keys.device)
-        self.device = keys.device
+        self.device, self._index = keys.device, keys.get_device()
         self.n_sequences, self.page_size = table.shape[0], page_size
-        self._desc = _lib.CacheDesc(C.sizeof(_lib.CacheDesc), keys.device.index, _dtypes()[keys.dtype], layers, pages, heads, page_size, key_dim,
+        self._int32, self._int64 = torch.int32, torch.int64
+        self._rows = ((heads, key_dim), (heads, values.shape[4]) if values is not None else None)
+        self._desc = _lib.CacheDesc(C.sizeof(_lib.CacheDesc), self._index, _dtypes()[keys.dtype], layers, pages, heads, page_size, key_dim,
                                     values.shape[4] if values is not None else 0, table.shape[0], table.shape[1], keys.data_ptr(),
                                     values.data_ptr() if values is not None else None, table.data_ptr(), lengths.data_ptr(), refs.data_ptr(), self.failures.data_ptr())
-        self._ref = C.byref(self._desc)
+        self._at = C.addressof(self._desc)
         size = C.c_size_t()
-        _lib.check(_lib.lib().svsx_cache_workspace(self._ref, 0, C.byref(size)))  # checks the description, too
-        self._space = size.value
+        _lib.check(_lib.lib().svsx_cache_workspace(self._at, _MOST, C.byref(size)))  # checks the description, too
+        # calls that change a cache follow one another, so one workspace serves them all
+        self._space, self._space_bytes = torch.empty(size.value, dtype=torch.uint8, device=keys.device), size.value
+        self._space_at = self._space.data_ptr()
 
-    def _workspace(self, n):
+    def _list(self, x, name):
+        """A vector of int32 on the cache's device; a list on the host is copied there first (and the host waits for that)."""
         import torch
 
-        return torch.empty(self._space + 4 * n, dtype=torch.uint8, device=self.device)
+        if not isinstance(x, torch.Tensor):
+            x = torch.as_tensor(x, dtype=torch.int32).to(self.device)
+        if x.dtype != self._int32 or x.dim() != 1 or not x.is_contiguous():
+            raise _invalid(f"{name} must be a contiguous vector of int32")
+        if x.get_device() != self._index:
+            raise _elsewhere(name, x)
+        return x
 
     def extend(self, sequences, offsets, n_tokens: int):
         """Sequence ``sequences[i]`` grows by ``offsets[i + 1] - offsets[i]`` rows; returns the slot of each of the ``n_tokens`` new rows (int64, for
         ``write``; -1 where an entry was refused or no entry has the row)."""
-        import torch
-
-        sequences, offsets = _list(sequences, self.device, "sequences"), _list(offsets, self.device, "offsets")
+        sequences, offsets = self._list(sequences, "sequences"), self._list(offsets, "offsets")
         n = sequences.shape[0]
         if offsets.shape[0] != n + 1:
             raise _invalid(f"{n} sequences need {n + 1} offsets, got {offsets.shape[0]}")
         if n_tokens < 0:
             raise _invalid("n_tokens must not be negative")
-        slots = torch.empty(n_tokens, dtype=torch.int64, device=self.device)
-        ws = self._workspace(n)
-        _lib.check(_lib.lib().svsx_cache_extend_device(self._ref, sequences.data_ptr(), offsets.data_ptr(), n, n_tokens, slots.data_ptr(), ws.data_ptr(), ws.shape[0],
-                                                       _stream(self.device)))
+        slots = sequences.new_empty(n_tokens, dtype=self._int64)
+        rc = _lib.lib().svsx_cache_extend_device(self._at, sequences.data_ptr(), offsets.data_ptr(), n, n_tokens, slots.data_ptr(), self._space_at, self._space_bytes,
+                                                 _stream(self._index))
+        if rc:
+            _lib.check(rc)
         return slots
 
     def write(self, slots, keys, values=None, layer: int = 0) -> None:
         """Rows ``keys`` [tokens, heads, key_dim] (and ``values``) of one layer to their slots.  Slots of one call differ; those outside the cache (-1) are skipped."""
-        import torch
-
-        if slots.dtype != torch.int64 or slots.dim() != 1 or not slots.is_contiguous():
+        if slots.dtype != self._int64 or slots.dim() != 1 or not slots.is_contiguous():
             raise _invalid("slots must be a contiguous vector of int64")
-        _on_device("slots", slots, self.device)
+        if slots.get_device() != self._index:
+            raise _elsewhere("slots", slots)
         if (values is None) != (self.values is None):
             raise _invalid("values are given exactly where the cache holds values")
         if not 0 <= layer < self.keys.shape[0]:
             raise _invalid(f"layer {layer} of a cache of {self.keys.shape[0]} layers")
-        n, heads = slots.shape[0], self.keys.shape[2]
-        for name, x, pool in (("keys", keys, self.keys), ("values", values, self.values)):
-            if x is None:
-                continue
-            if x.dtype != pool.dtype or x.shape != (n, heads, pool.shape[4]):
-                raise _invalid(f"{name} must be {pool.dtype} [{n}, {heads}, {pool.shape[4]}], got {x.dtype} {list(x.shape)}")
-            if x.stride(2) != 1 and x.shape[2] > 1:
-                raise _invalid(f"rows of {name} must be contiguous")
-            _on_device(name, x, self.device)
-        _lib.check(_lib.lib().svsx_cache_write_device(self._ref, layer, slots.data_ptr(), n, keys.data_ptr(), keys.stride(0), keys.stride(1),
-                                                      values.data_ptr() if values is not None else None, values.stride(0) if values is not None else 0,
-                                                      values.stride(1) if values is not None else 0, _stream(self.device)))
+        n = slots.shape[0]
+        ks = self._check_rows("keys", keys, n, self._rows[0])
+        vs = self._check_rows("values", values, n, self._rows[1]) if values is not None else (0, 0)
+        rc = _lib.lib().svsx_cache_write_device(self._at, layer, slots.data_ptr(), n, keys.data_ptr(), ks[0], ks[1], values.data_ptr() if values is not None else 0, vs[0], vs[1],
+                                                _stream(self._index))
+        if rc:
+            _lib.check(rc)
+
+    def _check_rows(self, name, x, n, row):
+        if x.dtype != self.keys.dtype or x.shape != (n, *row):
+            raise _invalid(f"{name} must be {self.keys.dtype} {[n, *row]}, got {x.dtype} {list(x.shape)}")
+        strides = x.stride()
+        if strides[2] != 1 and row[1] > 1:
+            raise _invalid(f"rows of {name} must be contiguous")
+        if x.get_device() != self._index:
+            raise _elsewhere(name, x)
+        return strides
 
     def _copy(self, sources, targets, share):
-        sources, targets = _list(sources, self.device, "sources"), _list(targets, self.device, "targets")
+        sources, targets = self._list(sources, "sources"), self._list(targets, "targets")
         n = sources.shape[0]
         if targets.shape[0] != n:
             raise _invalid(f"{n} sources and {targets.shape[0]} targets")
-        ws = self._workspace(n)
-        _lib.check(_lib.lib().svsx_cache_copy_device(self._ref, sources.data_ptr(), targets.data_ptr(), n, share, ws.data_ptr(), ws.shape[0], _stream(self.device)))
+        rc = _lib.lib().svsx_cache_copy_device(self._at, sources.data_ptr(), targets.data_ptr(), n, share, self._space_at, self._space_bytes, _stream(self._index))
+        if rc:
+            _lib.check(rc)
 
     def copy(self, sources, targets) -> None:
         """Each target, an empty sequence, becomes a copy of its source, in pages of its own."""
@@ -142,16 +148,17 @@ class PagedCache:
 
     def free(self, sequences) -> None:
         """The sequences become empty; pages nobody holds any more are free."""
-        sequences = _list(sequences, self.device, "sequences")
-        _lib.check(_lib.lib().svsx_cache_free_device(self._ref, sequences.data_ptr(), sequences.shape[0], _stream(self.device)))
+        sequences = self._list(sequences, "sequences")
+        rc = _lib.lib().svsx_cache_free_device(self._at, sequences.data_ptr(), sequences.shape[0], _stream(self._index))
+        if rc:
+            _lib.check(rc)
 
     def compact(self):
         """Used pages move to the front of the pool; returns each page's new place (int32 [pages], -1 for a page that was free)."""
-        import torch
-
-        moved = torch.empty(self.refs.shape[0], dtype=torch.int32, device=self.device)
-        ws = self._workspace(0)
-        _lib.check(_lib.lib().svsx_cache_compact_device(self._ref, moved.data_ptr(), ws.data_ptr(), ws.shape[0], _stream(self.device)))
+        moved = self.refs.new_empty(self.refs.shape[0])
+        rc = _lib.lib().svsx_cache_compact_device(self._at, moved.data_ptr(), self._space_at, self._space_bytes, _stream(self._index))
+        if rc:
+            _lib.check(rc)
         return moved
 
     def attend(self, queries, sequences=None, layer: int = 0, value_dim: int | None = None, scale: float | None = None, return_lse: bool = False):

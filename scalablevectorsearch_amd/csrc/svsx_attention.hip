@@ -911,9 +911,8 @@ Route route_of(const AttentionArgs& a, size_t es) {
 
 template <typename T, int KS, int HT> hipError_t launch_rows(const AttentionArgs& a, const Plan& plan, const Route& r, hipStream_t stream) {
     typedef RowsLayout<T, KS, HT> L;
-    // more than 64 KB of LDS has to be asked for; asking is cheap and the same every time
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(attend_rows_kernel<T, KS, HT>), hipFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
-    if (e != hipSuccess) return e;
+    static std::atomic<uint64_t> granted{0};
+    if (const hipError_t e = grant_lds(reinterpret_cast<const void*>(attend_rows_kernel<T, KS, HT>), L::kBytes, &granted); e != hipSuccess) return e;
     hipLaunchKernelGGL((attend_rows_kernel<T, KS, HT>), dim3(r.workers ? r.workers : a.n_queries, r.y), dim3(L::kThreads), L::kBytes, stream, a, plan, divider(a.page_size));
     return hipGetLastError();
 }

@@ -594,8 +594,8 @@ PromptRoute route_of(const ExpandedArgs& a, size_t es) {
 
 template <typename T, int DK, int DV, int NW> hipError_t launch_prompt(const ExpandedArgs& a, const Space& w, hipStream_t stream) {
     typedef PromptLayout<T, DK, DV, NW> L;
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(prompt_kernel<T, DK, DV, NW>), hipFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
-    if (e != hipSuccess) return e;
+    static std::atomic<uint64_t> granted{0};
+    if (const hipError_t e = grant_lds(reinterpret_cast<const void*>(prompt_kernel<T, DK, DV, NW>), L::kBytes, &granted); e != hipSuccess) return e;
     hipLaunchKernelGGL((prompt_kernel<T, DK, DV, NW>), dim3(w.most_tiles * a.n_heads), dim3(NW * 64), L::kBytes, stream, a, w);
     return hipGetLastError();
 }

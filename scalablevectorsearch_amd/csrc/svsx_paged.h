@@ -3,7 +3,9 @@
 
 #include "../../include/svsx.h"
 #include <hip/hip_runtime.h>
+#include <atomic>
 #include <stddef.h>
+#include <stdint.h>
 
 namespace svsx {
 
@@ -25,6 +27,17 @@ struct DeviceScope {
     DeviceScope(const DeviceScope&) = delete;
     DeviceScope& operator=(const DeviceScope&) = delete;
 };
+
+// A kernel that uses more than 64 KB of LDS asks for it, once on each device (bit d of *granted: device d).
+inline hipError_t grant_lds(const void* kernel, int bytes, std::atomic<uint64_t>* granted) {
+    int device = 0;
+    hipError_t e = hipGetDevice(&device);
+    const uint64_t bit = device >= 0 && device < 64 ? 1ull << device : 0;
+    if (e != hipSuccess || (granted->load(std::memory_order_relaxed) & bit)) return e;
+    e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == hipSuccess) granted->fetch_or(bit, std::memory_order_relaxed);
+    return e;
+}
 
 // 16-bit and 32-bit row elements; sums are float32 everywhere
 typedef __bf16 bf16_t;
