@@ -17,6 +17,7 @@ namespace {
 constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
 constexpr int kMaxSequences = 4096;                      // one claim and one running count per sequence in the planner's LDS (32 KB)
 constexpr int kPerThread = kMaxSequences / kPlanThreads; // entries a planner thread scans
+constexpr int kNear = 2048;                              // pages by rank that stay in LDS; what is beyond goes through the workspace
 constexpr int kPagesPerThread = 16;                      // reference counts a planner thread reads per step (four 16-byte loads in flight)
 
 struct CacheArgs {
@@ -87,11 +88,13 @@ __device__ __forceinline__ void load_refs(const CacheArgs& a, uint32_t first, in
 struct PlanShared {
     int claim[kMaxSequences]; // which entry of the call has this sequence for its own (the first that names it)
     int incl[kMaxSequences];  // running count of the pages that the entries up to this one need
+    int length[kMaxSequences]; // of an entry's sequence before the call; -1 = refused
+    int list[kNear];          // the first pages by rank
     int waves[kPlanWaves];
     int bad, refused;
 };
 
-// the `want` lowest free pages to list[]; returns how many there are (at most want)
+// the `want` lowest free pages to sh.list[], from kNear on to list[]; returns how many there are (at most want)
 __device__ __forceinline__ int lowest_free(const CacheArgs& a, int want, int32_t* list, PlanShared& sh) {
     int found = 0;
     for (uint32_t base = 0; base < a.n_pages && found < want; base += kPlanThreads * kPagesPerThread) {
@@ -104,7 +107,10 @@ __device__ __forceinline__ int lowest_free(const CacheArgs& a, int want, int32_t
 #pragma unroll
         for (int i = 0; i < kPagesPerThread; ++i) {
             if (r[i] == 0) {
-                if (rank < want) list[rank] = static_cast<int32_t>(first + i);
+                if (rank < want) {
+                    if (rank < kNear) sh.list[rank] = static_cast<int32_t>(first + i);
+                    else list[rank] = static_cast<int32_t>(first + i);
+                }
                 ++rank;
             }
         }
@@ -151,8 +157,24 @@ __device__ __forceinline__ void claim_sequences(const CacheArgs& a, PlanShared& 
     __syncthreads();
 }
 
+// The slot (page * page_size + row in page) of new row t; -1 where its sequence was refused (start -1) or no entry has it.
+__device__ __forceinline__ int64_t slot_of(const CacheArgs& a, const int32_t* seqs, const int32_t* offsets, int n, int t, const int32_t* start) {
+    if (n == 0) return -1;
+    int lo = 0, hi = n; // the last entry whose rows begin at or before t
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (offsets[mid] <= t) lo = mid;
+        else hi = mid;
+    }
+    const int32_t old = start[lo];
+    if (old < 0 || t < offsets[lo] || t >= offsets[lo + 1]) return -1;
+    const uint32_t at = static_cast<uint32_t>(old) + static_cast<uint32_t>(t - offsets[lo]);
+    const int32_t page = a.table[static_cast<size_t>(seqs[lo]) * a.columns + at / a.page_size];
+    return page >= 0 && static_cast<uint32_t>(page) < a.n_pages ? static_cast<int64_t>(page) * a.page_size + at % a.page_size : -1;
+}
+
 // Sequence seqs[i] grows by offsets[i + 1] - offsets[i] rows.
-__global__ __launch_bounds__(kPlanThreads) void extend_plan_kernel(const CacheArgs a, const int32_t* seqs, const int32_t* offsets, int n, int n_tokens, PlanSpace ws) {
+__global__ __launch_bounds__(kPlanThreads) void extend_plan_kernel(const CacheArgs a, const int32_t* seqs, const int32_t* offsets, int n, int n_tokens, PlanSpace ws, int64_t* slots) {
     __shared__ PlanShared sh;
     claim_sequences(a, sh, seqs, n);
     // offsets that run backwards or out of the call's rows refuse the call: no entry could be told from another's rows
@@ -176,15 +198,16 @@ __global__ __launch_bounds__(kPlanThreads) void extend_plan_kernel(const CacheAr
         need[e] = static_cast<int>(pages) - static_cast<int>((len + a.page_size - 1) / a.page_size);
         old[e] = static_cast<int>(len);
         grown[e] = static_cast<int>(len + count);
+        sh.length[i] = old[e];
     }
     const int total = scan_needs(sh, need);
     const int have = lowest_free(a, total, ws.to, sh);
     for (int rank = threadIdx.x; rank < have; rank += kPlanThreads) {
         const int i = entry_of(sh, n, rank);
         if (sh.incl[i] > have) continue; // the first entry that does not fit
-        const int32_t s = seqs[i], page = ws.to[rank];
+        const int32_t s = seqs[i], page = rank < kNear ? sh.list[rank] : ws.to[rank];
         const int first = i == 0 ? 0 : sh.incl[i - 1];
-        const uint32_t column = (static_cast<uint32_t>(a.lengths[s]) + a.page_size - 1) / a.page_size + (rank - first);
+        const uint32_t column = (static_cast<uint32_t>(sh.length[i]) + a.page_size - 1) / a.page_size + (rank - first);
         a.table[static_cast<size_t>(s) * a.columns + column] = page;
         a.refs[page] = 1;
     }
@@ -194,32 +217,21 @@ __global__ __launch_bounds__(kPlanThreads) void extend_plan_kernel(const CacheAr
         const int i = threadIdx.x * kPerThread + e;
         if (i >= n) continue;
         const bool served = old[e] >= 0 && (need[e] == 0 || sh.incl[i] <= have);
-        ws.start[i] = served ? old[e] : -1;
+        sh.length[i] = served ? old[e] : -1;
+        if (!slots) ws.start[i] = sh.length[i];
         if (served) a.lengths[seqs[i]] = grown[e];
         else atomicAdd(&sh.refused, 1);
     }
     __syncthreads();
     if (threadIdx.x == 0 && sh.refused) atomicAdd(a.failures, sh.refused);
+    if (slots)
+        for (int t = threadIdx.x; t < n_tokens; t += kPlanThreads) slots[t] = slot_of(a, seqs, offsets, n, t, sh.length);
 }
 
-// The slot (page * page_size + row in page) of every new row; -1 where its sequence was refused or no entry has it.
+// The slots of a call of many rows.
 __global__ __launch_bounds__(256) void slots_kernel(const CacheArgs a, const int32_t* seqs, const int32_t* offsets, int n, int n_tokens, const int32_t* start, int64_t* slots) {
     const int t = blockIdx.x * 256 + threadIdx.x;
-    if (t >= n_tokens) return;
-    int lo = 0, hi = n; // the last entry whose rows begin at or before t
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (offsets[mid] <= t) lo = mid;
-        else hi = mid;
-    }
-    int64_t slot = -1;
-    const int32_t old = n > 0 ? start[lo] : -1;
-    if (old >= 0 && t >= offsets[lo] && t < offsets[lo + 1]) {
-        const uint32_t at = static_cast<uint32_t>(old) + static_cast<uint32_t>(t - offsets[lo]);
-        const int32_t page = a.table[static_cast<size_t>(seqs[lo]) * a.columns + at / a.page_size];
-        if (page >= 0 && static_cast<uint32_t>(page) < a.n_pages) slot = static_cast<int64_t>(page) * a.page_size + at % a.page_size;
-    }
-    slots[t] = slot;
+    if (t < n_tokens) slots[t] = slot_of(a, seqs, offsets, n, t, start);
 }
 
 // Sequence targets[i], empty until now, becomes sources[i]: sharing its full pages (share) or with pages of its own.
@@ -243,6 +255,7 @@ __global__ __launch_bounds__(kPlanThreads) void copy_plan_kernel(const CacheArgs
             continue;
         }
         need[e] = static_cast<int>(share ? (l % a.page_size != 0) : (l + a.page_size - 1) / a.page_size);
+        sh.length[i] = len[e];
     }
     const int total = scan_needs(sh, need);
     const int have = lowest_free(a, total, ws.to, sh);
@@ -250,8 +263,9 @@ __global__ __launch_bounds__(kPlanThreads) void copy_plan_kernel(const CacheArgs
         const int i = entry_of(sh, n, rank);
         int32_t from = -1;
         if (sh.incl[i] <= have) {
-            const int32_t s = sources[i], page = ws.to[rank];
-            const uint32_t l = static_cast<uint32_t>(a.lengths[s]), first = i == 0 ? 0 : sh.incl[i - 1];
+            const int32_t s = sources[i], page = rank < kNear ? sh.list[rank] : ws.to[rank];
+            if (rank < kNear) ws.to[rank] = page;
+            const uint32_t l = static_cast<uint32_t>(sh.length[i]), first = i == 0 ? 0 : sh.incl[i - 1];
             const uint32_t column = (share ? l / a.page_size : 0) + (rank - first);
             from = a.table[static_cast<size_t>(s) * a.columns + column];
             a.table[static_cast<size_t>(targets[i]) * a.columns + column] = page;
@@ -519,8 +533,12 @@ int svsx_cache_extend_device(const svsx_cache_desc* desc, const int32_t* d_seque
     DeviceScope on(desc->device);
     if (on.error != hipSuccess) return fail(SVSX_RUNTIME_ERROR, "hipSetDevice(%d) failed: %s", desc->device, hipGetErrorString(on.error));
     const hipStream_t s = static_cast<hipStream_t>(hip_stream);
-    if (n > 0) hipLaunchKernelGGL(extend_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, a, d_sequences, d_offsets, static_cast<int>(n), static_cast<int>(n_tokens), ws);
-    if (n_tokens > 0)
+    // up to four rows a thread the planner gives out the slots itself: a second launch costs more
+    const bool near = n > 0 && n_tokens <= 4 * kPlanThreads;
+    if (n > 0)
+        hipLaunchKernelGGL(extend_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, a, d_sequences, d_offsets, static_cast<int>(n), static_cast<int>(n_tokens), ws,
+                           near && n_tokens > 0 ? d_slots : nullptr);
+    if (n_tokens > 0 && !near)
         hipLaunchKernelGGL(slots_kernel, dim3(static_cast<uint32_t>((n_tokens + 255) / 256)), dim3(256), 0, s, a, d_sequences, d_offsets, static_cast<int>(n), static_cast<int>(n_tokens),
                            ws.start, d_slots);
     return launched("cache extend");
