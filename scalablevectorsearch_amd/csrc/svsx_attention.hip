@@ -392,6 +392,124 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && VB == 1 ? 3 : 2) void attend
     } while (walk.next(a, plan, &c));
 }
 
+// ---- few rows, few heads ---------------------------------------------------------------------------------------------------------------------------
+//
+// Attention over the answers of a search: at most a few hundred rows, each somewhere else, for one to four heads.  There is nothing to split and nothing for the matrix
+// units to share; what counts is how many rows are on their way at once.  One wave takes a query (of one key head): 16 lanes a row, 8 or 16 columns a lane, so four rows
+// at a time; 64 table entries are looked up by the 64 lanes at once; each 16 lanes keep a softmax of their own, joined at the end.
+// 2048 queries of 100 rows of 96 float32 columns: 21 us (78 MB of rows, from a set larger than one L2), and 48 us through attend_group_kernel, whose four waves a query have one tile each.
+
+constexpr uint32_t kFewRows = 256; // rows up to which a query is one wave's
+
+// sum over the 16 lanes of a row of the wave, for each of them
+__device__ __forceinline__ float sum16(float x) {
+    x += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x128, 0xF, 0xF, false)); // rotated by 8, 4, 2, 1
+    x += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x124, 0xF, 0xF, false));
+    x += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x122, 0xF, 0xF, false));
+    x += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x121, 0xF, 0xF, false));
+    return x;
+}
+
+template <typename T, int E, int G, bool Wide> __global__ __launch_bounds__(256) void attend_few_kernel(const AttentionArgs a, const Divider by_page) {
+    constexpr int kBatch = E == 8 ? 8 : 4, kFrags = E / 8; // rows that each 16 lanes have on their way
+    const uint32_t lane = threadIdx.x & 63, item = blockIdx.x * 4 + (threadIdx.x >> 6), quarter = lane >> 4, n16 = lane & 15;
+    if (item >= a.n_queries * a.n_key_heads) return;
+    const uint32_t i = item / a.n_key_heads, g = item % a.n_key_heads;
+    const int32_t* table = nullptr;
+    const uint32_t n = __builtin_amdgcn_readfirstlane(rows_of(a, i, &table));
+    const T* keys = static_cast<const T*>(a.keys) + g * a.key_head_stride;
+    const T* values = static_cast<const T*>(a.values) + g * a.value_head_stride;
+    const float scale = a.scale * kLog2e;
+    float q[G][E], o[G][E], top[G], sum[G];
+#pragma unroll
+    for (int h = 0; h < G; ++h) {
+        const uint32_t head = g * a.group + min(static_cast<uint32_t>(h), a.group - 1);
+        const T* row = static_cast<const T*>(a.queries) + i * a.query_stride + head * a.query_head_stride;
+#pragma unroll
+        for (int f = 0; f < kFrags; ++f) {
+            const Frag<T> x = a.wide_queries ? load_frag<T, true>(row, n16 * E + f * 8, a.dk) : load_frag<T, false>(row, n16 * E + f * 8, a.dk);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                q[h][f * 8 + e] = to_f32(x[e]);
+                o[h][f * 8 + e] = 0.0f;
+            }
+        }
+        top[h] = -INFINITY;
+        sum[h] = 0.0f;
+    }
+    for (uint32_t base = 0; base < n; base += 64) {
+        uint32_t at;
+        const int32_t mine = table[by_page(min(base + lane, n - 1), &at)];
+        const bool is = base + lane < n && static_cast<uint32_t>(mine) < a.n_pages;
+        const int32_t page = is ? mine : -1;
+        for (uint32_t first = 0; first < 16 && base + first * 4 < n; first += kBatch) {
+            Frag<T> k[kBatch][kFrags], v[kBatch][kFrags];
+            bool there[kBatch];
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j) {
+                const int from = static_cast<int>((first + j) * 4 + quarter);
+                const int32_t p = __shfl(page, from);
+                const uint32_t r = __shfl(at, from);
+                there[j] = p >= 0;
+                const T* row = keys + (p >= 0 ? static_cast<size_t>(p) : 0) * a.key_page_stride + r * a.key_row_stride;
+#pragma unroll
+                for (int f = 0; f < kFrags; ++f) k[j][f] = load_frag<T, Wide>(row, n16 * E + f * 8, a.dk);
+                if (!a.shared) {
+                    const T* vrow = values + (p >= 0 ? static_cast<size_t>(p) : 0) * a.value_page_stride + r * a.value_row_stride;
+#pragma unroll
+                    for (int f = 0; f < kFrags; ++f) v[j][f] = load_frag<T, Wide>(vrow, n16 * E + f * 8, a.dv);
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < G; ++h) {
+                float s[kBatch], most = top[h];
+#pragma unroll
+                for (int j = 0; j < kBatch; ++j) {
+                    float x = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < E; ++e) x = fmaf(to_f32(k[j][e >> 3][e & 7]), q[h][e], x);
+                    s[j] = there[j] ? sum16(x) * scale : -INFINITY;
+                    most = fmaxf(most, s[j]);
+                }
+                const float ref = most == -INFINITY ? 0.0f : most, was = exp2_fast(top[h] - ref);
+                top[h] = most;
+                sum[h] *= was;
+#pragma unroll
+                for (int e = 0; e < E; ++e) o[h][e] *= was;
+#pragma unroll
+                for (int j = 0; j < kBatch; ++j) {
+                    const float p = exp2_fast(s[j] - ref);
+                    sum[h] += p;
+                    if (there[j]) { // what a row that is not there would be read from is not defined
+#pragma unroll
+                        for (int e = 0; e < E; ++e) o[h][e] = fmaf(p, to_f32(a.shared ? k[j][e >> 3][e & 7] : v[j][e >> 3][e & 7]), o[h][e]);
+                    }
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int h = 0; h < G; ++h) {
+#pragma unroll
+        for (int off = 16; off <= 32; off <<= 1) {
+            const float other = __shfl_xor(top[h], off), all = fmaxf(top[h], other);
+            const float mine = top[h] == -INFINITY ? 0.0f : exp2_fast(top[h] - all), theirs = other == -INFINITY ? 0.0f : exp2_fast(other - all);
+            sum[h] = sum[h] * mine + __shfl_xor(sum[h], off) * theirs;
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[h][e] = o[h][e] * mine + __shfl_xor(o[h][e], off) * theirs;
+            top[h] = all;
+        }
+        if (static_cast<uint32_t>(h) >= a.group || quarter != 0) continue;
+        const size_t at = static_cast<size_t>(i) * a.n_heads + g * a.group + h;
+        const float inv = sum[h] == 0.0f ? 0.0f : 1.0f / sum[h];
+        T* out = static_cast<T*>(a.out) + at * a.dv;
+#pragma unroll
+        for (uint32_t e = 0; e < E; ++e)
+            if (n16 * E + e < a.dv) out[n16 * E + e] = from_f32<T>(o[h][e] * inv);
+        if (a.lse && n16 == 0) a.lse[at] = sum[h] == 0.0f ? -INFINITY : (top[h] + log2f(sum[h])) * kLn2;
+    }
+}
+
 // ---- rows that are key and value at once, for many heads ------------------------------------------------------------------------------------------
 //
 // Latent rows: every head reads the same row, as key and (its first columns) as value, so 64 heads make 240 operations of each byte and the rows have to be
@@ -861,7 +979,7 @@ int check_attention(const svsx_attention_desc* d, AttentionArgs* a) {
 
 // How a call is answered; decided from sizes, types, strides and addresses alone.
 struct Route {
-    bool rows, group; // many heads over shared rows, or heads that share a key head, on the matrix units; else one workgroup per head
+    bool rows, group, few; // many heads over shared rows, or heads that share a key head, on the matrix units; few rows and heads; else one workgroup per head
     bool wide, page8;
     int ks, vb, ht;
     uint32_t workers, unit, y;
@@ -882,6 +1000,12 @@ Route route_of(const AttentionArgs& a, size_t es) {
              aligned({a.value_page_stride, a.value_head_stride, a.value_row_stride}, a.values);
     // Shared rows go through LDS where more than 16 heads read them, and where they are too long for the registers of the other kernel
     r.rows = a.shared && r.wide && a.dk <= 576 && a.dv <= 512 && (a.group > 16 || a.dk > 256);
+    const uint64_t most = static_cast<uint64_t>(a.max_pages) * a.page_size; // rows that a query can have
+    r.few = most <= kFewRows && a.group <= 4 && a.dk <= 256 && a.dv <= 256;
+    if (r.few) {
+        r.rows = false;
+        return r;
+    }
     r.group = !r.rows && a.dk <= 256 && a.dv <= 256;
     if (!r.rows && !r.group) return r;
     if (r.rows) {
@@ -899,7 +1023,7 @@ Route route_of(const AttentionArgs& a, size_t es) {
     // One workgroup a query where queries alone fill the machine several times over, where no query can have more rows than one unit, or where the sum of all units
     // might not fit 32 bits.
     const uint32_t resident = kUnits * (r.rows ? 1 : r.vb == 2 || es == 4 ? 2 : 3);
-    const uint64_t groups = static_cast<uint64_t>(a.n_queries) * r.y, units = (static_cast<uint64_t>(a.max_pages) * a.page_size + r.unit - 1) / r.unit;
+    const uint64_t groups = static_cast<uint64_t>(a.n_queries) * r.y, units = (most + r.unit - 1) / r.unit;
     if (groups >= 8 * resident || units <= 1 || units * a.n_queries >= (1ull << 32)) return r;
     r.workers = static_cast<uint32_t>(std::min<uint64_t>(std::max(1u, resident / r.y), a.n_queries * units));
     const size_t parts = (static_cast<size_t>(r.workers) + a.n_queries) * a.n_heads;
@@ -962,6 +1086,18 @@ template <typename T> hipError_t launch_split(const AttentionArgs& a, const Rout
 }
 
 template <typename T> hipError_t launch_attention(const AttentionArgs& a, const Route& r, void* workspace, hipStream_t stream) {
+    if (r.few) {
+        const bool narrow = a.dk <= 128 && a.dv <= 128;
+        typedef void (*Kernel)(const AttentionArgs, const Divider);
+        Kernel kernel;
+#define SVSX_FEW(E, G) (r.wide ? attend_few_kernel<T, E, G, true> : attend_few_kernel<T, E, G, false>)
+        if (a.group == 1) kernel = narrow ? SVSX_FEW(8, 1) : SVSX_FEW(16, 1);
+        else if (a.group == 2) kernel = narrow ? SVSX_FEW(8, 2) : SVSX_FEW(16, 2);
+        else kernel = narrow ? SVSX_FEW(8, 4) : SVSX_FEW(16, 4);
+#undef SVSX_FEW
+        hipLaunchKernelGGL(kernel, dim3((a.n_queries * a.n_key_heads + 3) / 4), dim3(256), 0, stream, a, divider(a.page_size));
+        return hipGetLastError();
+    }
     if (r.rows || r.group) return launch_split<T>(a, r, workspace, stream);
     hipLaunchKernelGGL(attend_head_kernel<T>, dim3(a.n_heads, a.n_queries), dim3(256), 0, stream, a);
     return hipGetLastError();
