@@ -465,7 +465,7 @@ int svsx_cache_compact_device(const svsx_cache_desc* desc, int32_t* d_moved, voi
  *   values    d_values = NULL: the first value_dim (<= key_dim) columns of a key row are its value (latent attention, absorbed: n_key_heads = 1).
  *   d_out     [n_queries][n_heads][value_dim] of dtype; a query without rows (or all of whose products are -inf) gives zeros
  *   d_lse     [n_queries][n_heads] float32 or NULL: log sum_r p_r; -inf where there is nothing
- * Strides are in elements; rows are contiguous.  key_dim and value_dim are at most 1024.
+ * Strides are in elements; rows are contiguous.  key_dim and value_dim are at most 1024; n_queries and n_heads at most 65535; scale is finite.
  * The workspace (svsx_paged_attention_workspace bytes, possibly 0) belongs to the call until it has run.  Device pointers, enqueued on hip_stream, no waiting. */
 typedef struct {
     size_t struct_size; /* sizeof(svsx_attention_desc) */
@@ -495,7 +495,7 @@ int svsx_paged_attention_device(const svsx_attention_desc* desc, void* d_workspa
  *   d_queries  [n_tokens][n_heads][nope_dim + rope_dim]     d_rows     [n_rows][rank + rope_dim]
  *   d_w_key    [n_heads][nope_dim][rank], contiguous        d_w_value  [n_heads][value_dim][rank], contiguous
  *   d_out      [n_tokens][n_heads][value_dim], contiguous; a query that sees no row gives zeros.  Queries in no sequence: zeros, or with keep_rest left alone.
- * nope_dim + rope_dim <= 1024, value_dim <= 1024, rank + rope_dim <= 1024.  For the 16-bit types the expanded keys and values are rounded to dtype. */
+ * nope_dim + rope_dim, value_dim and rank + rope_dim are at most 1024; n_rows < 2^27 - 128, n_tokens * n_heads < 2^29, n_sequences * n_heads < 2^22; scale is finite.  For the 16-bit types the expanded keys and values are rounded to dtype. */
 typedef struct {
     size_t struct_size; /* sizeof(svsx_expanded_desc) */
     int device;

@@ -1,7 +1,8 @@
 """Attention over rows that live in HBM, over svsx_paged_attention_device and svsx_latent_expanded_device (include/svsx.h): the exhaustive inner
 products of ``FlatIndex`` with a softmax over them in the place of the k best.
 
-Calls are enqueued on torch's current stream of the queries' device, never wait for the GPU, and may be captured into a graph."""
+Calls are enqueued on torch's current stream of the queries' device, never wait for the GPU, and may be captured into a graph.  They are for serving:
+no gradient flows through them."""
 from __future__ import annotations
 
 import ctypes as C
@@ -72,6 +73,8 @@ def paged_attention(queries, keys, values, table, lengths, sequences=None, value
     code = _dtypes().get(dtype)
     if code is None:
         raise _invalid(f"unsupported row type {dtype} (float32, float16, bfloat16)")
+    if dim < 1:
+        raise _invalid("queries have no columns")
     if keys.dtype != dtype or key_dim != dim:
         raise _invalid(f"keys must be {dtype} rows of {dim}, are {keys.dtype} rows of {key_dim}")
     if (qs[2] != 1 or ks[3] != 1) and dim > 1:
@@ -117,10 +120,13 @@ def paged_attention(queries, keys, values, table, lengths, sequences=None, value
         raise _invalid("value_dim must be positive")
     out = queries.new_empty((n, heads, value_dim))
     lse = queries.new_empty((n, heads), dtype=torch.float32) if return_lse else None
-    desc = _ATTENTION.pack(
-        _ATTENTION.size, device, code, n, heads, key_heads, dim, value_dim, pages, page_size, table_sequences, max_pages, ts[0], queries.data_ptr(), qs[0], qs[1],
-        keys.data_ptr(), ks[0], ks[1], ks[2], value_ptr, vs[0], vs[1], vs[2], table.data_ptr(), lengths.data_ptr(), sequence_ptr, dim**-0.5 if scale is None else scale,
-        out.data_ptr(), lse.data_ptr() if return_lse else 0)
+    try:
+        desc = _ATTENTION.pack(
+            _ATTENTION.size, device, code, n, heads, key_heads, dim, value_dim, pages, page_size, table_sequences, max_pages, ts[0], queries.data_ptr(), qs[0], qs[1],
+            keys.data_ptr(), ks[0], ks[1], ks[2], value_ptr, vs[0], vs[1], vs[2], table.data_ptr(), lengths.data_ptr(), sequence_ptr, dim**-0.5 if scale is None else scale,
+            out.data_ptr(), lse.data_ptr() if return_lse else 0)
+    except OverflowError:
+        raise _invalid("scale must be finite") from None
     L = _lib.lib()
     size = C.c_size_t()
     rc = L.svsx_paged_attention_workspace(desc, C.byref(size))
@@ -164,6 +170,8 @@ def latent_attention_expanded(queries, rows, w_key, w_value, query_offsets, row_
     if any(x.dtype != dtype for x in (rows, w_key, w_value)):
         raise _invalid(f"rows, w_key and w_value must be {dtype} like the queries")
     rope = dim - nope
+    if dim < 1:
+        raise _invalid("queries have no columns")
     if w_key.shape[0] != heads or w_value.shape[0] != heads or w_value.shape[2] != rank or rope < 0 or width != rank + rope:
         raise _invalid(f"queries {list(queries.shape)}, rows {list(rows.shape)}, w_key {list(w_key.shape)} and w_value {list(w_value.shape)} do not fit together")
     if query_offsets.dim() != 1 or query_offsets.shape != row_offsets.shape or query_offsets.shape[0] < 1:

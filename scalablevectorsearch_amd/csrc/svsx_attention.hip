@@ -942,6 +942,7 @@ int check_attention(const svsx_attention_desc* d, AttentionArgs* a) {
     if (d->page_size == 0 || d->page_size >= limit || d->n_pages >= limit || d->n_sequences >= limit || d->max_pages >= limit || d->max_pages * d->page_size >= limit)
         return fail(SVSX_INVALID_ARGUMENT, "page_size must be positive; n_pages, n_sequences and max_pages * page_size must be below 2^31");
     if (d->n_queries > 65535) return fail(SVSX_INVALID_ARGUMENT, "too many queries in one call (%zu, at most 65535)", d->n_queries);
+    if (!std::isfinite(d->scale)) return fail(SVSX_INVALID_ARGUMENT, "scale must be finite");
     if (d->n_queries > 0 && (!d->d_queries || !d->d_out)) return fail(SVSX_INVALID_ARGUMENT, "null argument");
     if (d->n_queries > 0 && d->n_sequences > 0 && (!d->d_lengths || (d->max_pages > 0 && (!d->d_table || (d->n_pages > 0 && !d->d_keys)))))
         return fail(SVSX_INVALID_ARGUMENT, "null argument");
@@ -1004,7 +1005,7 @@ Route route_of(const AttentionArgs& a, size_t es) {
     // Shared rows go through LDS where more than 16 heads read them, and where they are too long for the registers of the other kernel
     r.rows = a.shared && r.wide && a.dk <= 576 && a.dv <= 512 && (a.group > 16 || a.dk > 256);
     const uint64_t most = static_cast<uint64_t>(a.max_pages) * a.page_size; // rows that a query can have
-    r.few = most <= kFewRows && a.group <= 4 && a.dk <= 256 && a.dv <= 256;
+    r.few = most <= kFewRows && a.group <= 4 && a.dk <= 256 && a.dv <= 256 && static_cast<uint64_t>(a.n_queries) * a.n_key_heads <= 1u << 25; // a grid has fewer than 2^32 threads
     if (r.few) {
         r.rows = false;
         return r;

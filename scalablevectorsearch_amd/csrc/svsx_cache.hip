@@ -428,8 +428,8 @@ struct WriteArgs {
 template <typename W> __global__ __launch_bounds__(256) void write_kernel(const WriteArgs a) {
     const uint32_t kind = blockIdx.y, words = a.row_words[kind], per_token = words * a.n_heads;
     const uint64_t at = static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (at >= static_cast<uint64_t>(a.n_tokens) * per_token) return;
     const uint32_t token = static_cast<uint32_t>(at / per_token), in_token = static_cast<uint32_t>(at % per_token);
-    if (token >= a.n_tokens) return;
     const int64_t slot = a.slots[token];
     if (slot < 0 || slot >= static_cast<int64_t>(a.n_pages) * a.page_size) return;
     const uint32_t head = in_token / words, word = in_token % words;

@@ -25,10 +25,8 @@ struct ExpandedArgs {
     int wide_queries, wide_out; // rows begin at 16-byte boundaries and are whole 16-byte words
 };
 
-// One workgroup per query and head, in the latent space: w_key applied to the query, w_value to the result.  For heads of more than 256 columns.
-template <typename T> __global__ __launch_bounds__(256) void expanded_head_kernel(const ExpandedArgs a) {
-    __shared__ RowsShared sm;
-    const uint32_t h = blockIdx.x % a.n_heads, t = blockIdx.x / a.n_heads;
+// One query and head of a workgroup at a time, in the latent space: w_key applied to the query, w_value to the result.  For heads of more than 256 columns.
+template <typename T> __device__ __forceinline__ void one_query(const ExpandedArgs& a, uint32_t h, uint32_t t, RowsShared& sm) {
     T* out = static_cast<T*>(a.out) + (static_cast<size_t>(t) * a.n_heads + h) * a.dv;
     int lo = 0, hi = static_cast<int>(a.n_sequences); // the last sequence whose queries begin at or before t
     while (hi - lo > 1) {
@@ -63,6 +61,14 @@ template <typename T> __global__ __launch_bounds__(256) void expanded_head_kerne
         float x = 0.0f;
         for (uint32_t d = 0; d < a.rank; ++d) x = fmaf(sm.out[0][d], to_f32(wv[static_cast<size_t>(c) * a.rank + d]), x);
         out[c] = from_f32<T>(x);
+    }
+}
+
+template <typename T> __global__ __launch_bounds__(256) void expanded_head_kernel(const ExpandedArgs a) {
+    __shared__ RowsShared sm;
+    for (uint32_t item = blockIdx.x; item < a.n_heads * a.n_tokens; item += gridDim.x) {
+        one_query<T>(a, item % a.n_heads, item / a.n_heads, sm);
+        __syncthreads(); // what the next query's threads write to has been read
     }
 }
 
@@ -543,9 +549,11 @@ int check_expanded(const svsx_expanded_desc* d, ExpandedArgs* a) {
         d->nope_dim + d->rope_dim > kMaxDim || d->nope_dim + d->rope_dim == 0)
         return fail(SVSX_INVALID_ARGUMENT, "rank (%zu) + rope_dim (%zu), nope_dim (%zu) + rope_dim and value_dim (%zu) must be in [1, %d]", d->rank, d->rope_dim, d->nope_dim,
                     d->value_dim, kMaxDim);
-    const size_t limit = size_t(1) << 31;
-    if (d->n_tokens >= limit || d->n_rows >= (size_t(1) << 27) - 128 || d->n_sequences >= limit || d->n_tokens * d->n_heads >= limit || d->n_sequences * d->n_heads >= limit ||
-        d->n_heads * (d->nope_dim + kMaxDim) >= limit) return fail(SVSX_INVALID_ARGUMENT, "too many queries, rows or sequences in one call");
+    // grids have fewer than 2^32 threads: with these limits, and rows that fit the machine's memory once they are expanded, all of them do
+    if (d->n_rows >= (size_t(1) << 27) - 128 || d->n_tokens >= size_t(1) << 29 || d->n_tokens * d->n_heads >= size_t(1) << 29 || d->n_sequences >= size_t(1) << 22 ||
+        d->n_sequences * d->n_heads >= size_t(1) << 22)
+        return fail(SVSX_INVALID_ARGUMENT, "too many queries, rows or sequences in one call (n_rows %zu, n_tokens %zu, n_sequences %zu, n_heads %zu)", d->n_rows, d->n_tokens, d->n_sequences, d->n_heads);
+    if (!std::isfinite(d->scale)) return fail(SVSX_INVALID_ARGUMENT, "scale must be finite");
     if (d->n_tokens > 0 && (!d->d_queries || !d->d_out || !d->d_w_value || (d->nope_dim > 0 && !d->d_w_key))) return fail(SVSX_INVALID_ARGUMENT, "null argument");
     if (d->n_tokens > 0 && d->n_sequences > 0 && (!d->d_query_offsets || !d->d_row_offsets || (d->n_rows > 0 && !d->d_rows))) return fail(SVSX_INVALID_ARGUMENT, "null argument");
     *a = ExpandedArgs{d->d_queries, d->d_rows, d->d_w_key, d->d_w_value, d->d_query_offsets, d->d_row_offsets, d->d_out, d->query_stride, d->query_head_stride, d->row_stride,
@@ -602,7 +610,7 @@ template <typename T, int DK, int DV, int NW> hipError_t launch_prompt(const Exp
 
 template <typename T> hipError_t launch_expanded(const ExpandedArgs& a, PromptRoute& r, void* workspace, hipStream_t stream) {
     if (!r.tiles) {
-        hipLaunchKernelGGL(expanded_head_kernel<T>, dim3(a.n_heads * a.n_tokens), dim3(256), 0, stream, a);
+        hipLaunchKernelGGL(expanded_head_kernel<T>, dim3(std::min(a.n_heads * a.n_tokens, 1u << 20)), dim3(256), 0, stream, a); // a grid has fewer than 2^32 threads
         return hipGetLastError();
     }
     char* base = static_cast<char*>(workspace);
@@ -617,8 +625,6 @@ template <typename T> hipError_t launch_expanded(const ExpandedArgs& a, PromptRo
     g.value_i = static_cast<uint32_t>((w.value_rows + 127) / 128);
     g.values = g.value_i * ((a.n_heads * r.dv + 127) / 128);
     g.copies = 1024;
-    if (static_cast<uint64_t>(g.key_i) * ((a.n_rows + 127) / 128) + static_cast<uint64_t>(g.value_i) * ((a.n_heads * r.dv + 127) / 128) >= (1ull << 31) - 2048) return hipErrorInvalidValue;
-    if (static_cast<uint64_t>(w.most_tiles) * a.n_heads >= (1ull << 31)) return hipErrorInvalidValue;
     auto expand = r.wide ? expand_kernel<T, true> : expand_kernel<T, false>;
     hipLaunchKernelGGL(expand, dim3(g.keys + g.values + g.copies + 1), dim3(256), 0, stream, a, w, g);
     hipError_t e = hipGetLastError();

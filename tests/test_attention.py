@@ -118,6 +118,7 @@ DTYPES = ["float32", "float16", "bfloat16"]
     ([40, 0, 1000], 6, 2, 96, 96, 32), ([70, 33], 14, 2, 80, 80, 5), ([500, 3], 16, 1, 100, 36, 7), ([257, 64], 34, 2, 256, 256, 64),
     ([90, 1], 20, 1, 33, 128, 3), ([45], 5, 5, 192, 128, 128), ([130, 20], 3, 1, 200, 200, 1), ([77], 2, 1, 768, 768, 16), ([35], 4, 2, 1024, 1000, 4),
     ([2100, 1500], 4, 4, 128, 128, 16), ([64, 200], 12, 1, 128, 64, 256),
+    ([256, 0, 1, 65], 3, 1, 96, 40, 1), ([257, 3], 3, 1, 96, 40, 1), ([200, 60], 8, 2, 256, 256, 8), ([31, 255], 4, 4, 100, 250, 5), ([240, 9], 10, 2, 64, 64, 16),
 ])
 def test_paged_attention_is_its_formula(dtype, lengths, heads, kv, dim, value_dim, page):
     _run(*_case(dtype, lengths, heads, kv, dim, value_dim, page))
@@ -359,10 +360,26 @@ def test_a_run_of_the_operators_together():
     assert cache.failures.item() == 0 and cache.lengths.tolist() == [0, 27, 27]
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads, kv, dim, value_dim, page, shared", [(2, 2, 64, 64, 4, False), (1, 1, 64, 64, 16, False), (1, 1, 288, 256, 16, True), (1, 1, 260, 20, 2, False)])
+def test_as_many_queries_as_a_call_takes(heads, kv, dim, value_dim, page, shared):
+    import torch
+
+    import scalablevectorsearch_amd as svs
+
+    q, keys, values, table, n = _case("float16", [200, 0, 70], heads, kv, dim, value_dim, page, shared=shared)
+    table = torch.cat([table, table.new_zeros(3, 512 // page - table.shape[1] if page > 4 else 0)], 1)
+    q, sequences = q.repeat_interleave(3, 0), torch.arange(3, dtype=torch.int32, device="cuda").repeat(3)
+    want = _reference(q, keys, values, table, n, sequences, value_dim, dim**-0.5)
+    which = torch.arange(65535, device="cuda") * 7 % 9
+    out, lse = svs.paged_attention(q[which], keys, values, table, n, sequences=sequences[which], value_dim=value_dim, return_lse=True)
+    _check(out, lse, [x[which.cpu()] for x in want])
+
+
 # ---- the expanded form -----------------------------------------------------------------------------------------------------------------------------
 
 
-def _expanded(q, rows, wk, wv, qo, ro, scale, causal):
+def _expanded(q, rows, wk, wv, qo, ro, scale, causal, only=None):
     import torch
 
     u, e = torch.finfo(q.dtype).eps / 2, 2.0**-24
@@ -373,7 +390,7 @@ def _expanded(q, rows, wk, wv, qo, ro, scale, causal):
     for i in range(len(qo) - 1):
         c = rows[ro[i]:ro[i + 1]]
         nq, nr = qo[i + 1] - qo[i], ro[i + 1] - ro[i]
-        for h in range(heads):
+        for h in only or range(heads):
             k, v = torch.cat([c[:, :rank] @ wk[h].T, c[:, rank:]], 1), c[:, :rank] @ wv[h].T
             ka, va = torch.cat([c[:, :rank].abs() @ wk[h].abs().T, c[:, rank:].abs()], 1), c[:, :rank].abs() @ wv[h].abs().T  # bounds of the sums' roundings
             for j in range(nq):
@@ -396,7 +413,7 @@ def _expanded(q, rows, wk, wv, qo, ro, scale, causal):
 @pytest.mark.parametrize("counts, before, heads, nope, rope, rank, dv", [
     ([1], [0], 1, 1, 0, 1, 1), ([1], [40], 16, 128, 64, 512, 128), ([33, 1, 0, 70], [0, 5, 3, 129], 2, 64, 32, 128, 64), ([200], [0], 2, 128, 64, 256, 128),
     ([65, 130], [300, 0], 3, 64, 64, 96, 128), ([17, 3], [2, 90], 2, 100, 20, 60, 36), ([40], [7], 1, 33, 31, 65, 77), ([129], [128], 1, 192, 64, 512, 192),
-    ([5, 64, 63, 128], [0, 64, 1, 0], 4, 32, 16, 64, 32), ([3], [0], 2, 0, 64, 32, 16),
+    ([5, 64, 63, 128], [0, 64, 1, 0], 4, 32, 16, 64, 32), ([3], [0], 2, 0, 64, 32, 16), ([3, 70], [2, 0], 2, 300, 20, 64, 32), ([4, 9], [3, 80], 2, 32, 16, 64, 300),
 ])
 @pytest.mark.parametrize("causal", [True, False])
 def test_expanded_latent_attention_is_its_formula(dtype, counts, before, heads, nope, rope, rank, dv, causal):
@@ -453,6 +470,84 @@ def test_expanded_prompts_with_ragged_edges(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nope, rope, rank, dv", [(128, 64, 128, 128), (64, 64, 64, 64), (100, 60, 72, 40), (64, 32, 96, 100)])
+def test_expanded_prompts_of_many_heads(dtype, nope, rope, rank, dv):
+    """prompts that fill the machine: 66048 queries and heads, some heads of which are checked"""
+    import torch
+
+    import scalablevectorsearch_amd as svs
+
+    g = torch.Generator().manual_seed(8)
+    t = getattr(torch, dtype)
+    qo, ro = [0, 300, 301, 301, 516], [0, 333, 400, 400, 700]
+    q, rows = torch.randn(516, 128, nope + rope, generator=g).to(t).cuda(), torch.randn(700, rank + rope, generator=g).to(t).cuda()
+    wk, wv = (torch.randn(128, nope, rank, generator=g) * rank**-0.5).to(t).cuda(), (torch.randn(128, dv, rank, generator=g) * rank**-0.5).to(t).cuda()
+    off = [torch.tensor(x, dtype=torch.int32).cuda() for x in (qo, ro)]
+    some = [0, 77, 127]
+    for causal in (True, False):
+        got = svs.latent_attention_expanded(q, rows, wk, wv, *off, causal=causal)
+        out, bound = _expanded(q, rows, wk, wv, qo, ro, (nope + rope) ** -0.5, causal, some)
+        assert ((got.cpu().double() - out).abs() - bound)[:, some].max() <= 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 2.0])
+def test_expanded_prompts_of_any_scale(dtype, scale):
+    import torch
+
+    import scalablevectorsearch_amd as svs
+
+    g = torch.Generator().manual_seed(9)
+    t = getattr(torch, dtype)
+    q, rows = torch.randn(90, 2, 96, generator=g).to(t).cuda(), torch.randn(150, 128, generator=g).to(t).cuda()
+    wk, wv = (torch.randn(2, 64, 96, generator=g) / 10).to(t).cuda(), (torch.randn(2, 64, 96, generator=g) / 10).to(t).cuda()
+    off = [torch.tensor(x, dtype=torch.int32).cuda() for x in ([0, 90], [0, 150])]
+    out, bound = _expanded(q, rows, wk, wv, [0, 90], [0, 150], scale, True)
+    assert ((svs.latent_attention_expanded(q, rows, wk, wv, *off, scale=scale).cpu().double() - out).abs() - bound).max() <= 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads", [2, 256])
+def test_expanded_rows_that_are_not_finite(dtype, heads):
+    """A row concerns the queries that see it: NaN in its latent vector makes their results NaN, an infinite rotary column does where the product is +inf, and where it is
+    -inf the row has no weight.  Earlier queries and other sequences are as if it were not there."""
+    import torch
+
+    import scalablevectorsearch_amd as svs
+
+    g = torch.Generator().manual_seed(10)
+    t = getattr(torch, dtype)
+    nope, rope, rank, dv = 64, 32, 96, 64
+    qo, ro = [0, 21, 200, 256], [0, 30, 259, 330]
+    q, clean = torch.randn(256, heads, nope + rope, generator=g).to(t), torch.randn(330, rank + rope, generator=g).to(t)
+    wk, wv = (torch.randn(heads, nope, rank, generator=g) / 10).to(t).cuda(), (torch.randn(heads, dv, rank, generator=g) / 10).to(t).cuda()
+    off = [torch.tensor(x, dtype=torch.int32).cuda() for x in (qo, ro)]
+    some, scale = [0, heads - 1], (nope + rope) ** -0.5
+    out, bound = _expanded(q, clean, wk, wv, qo, ro, scale, True, some)
+    for row in (30, 100, 163, 258):  # the first of its sequence, two inside, the last
+        sees = torch.zeros(256, dtype=torch.bool)
+        sees[21:200] = torch.arange(179) + 259 - 179 >= row
+        sick = clean.clone()
+        sick[row, 7] = math.nan
+        got = svs.latent_attention_expanded(q.cuda(), sick.cuda(), wk, wv, *off).cpu().double()
+        assert got[sees].isnan().all() and not got[~sees].isnan().any()
+        assert ((got - out).abs() - bound)[~sees][:, some].max() <= 0
+        sick = clean.clone()
+        sick[row, rank + 5] = math.inf
+        got = svs.latent_attention_expanded(q.cuda(), sick.cuda(), wk, wv, *off).cpu().double()
+        up = q[:, :, nope + 5] > 0
+        assert torch.equal(got.isnan().all(2), sees[:, None] & up) and torch.equal(got.isnan().any(2), sees[:, None] & up)
+        assert ((got - out).abs() - bound)[~sees][:, some].max() <= 0
+        less = [0, 30, 258, 329]  # without the row, for those that would see it: they are counted from the end
+        without, wide = _expanded(q, torch.cat([clean[:row], clean[row + 1:]]), wk, wv, qo, less, scale, True, some)
+        here = (sees[:, None] & ~up)[:, some]
+        assert (((got - without).abs() - wide)[:, some][here] <= 0).all()  # of the last row's one query possibly nothing
+
+
+@pytest.mark.gpu
 def test_expanded_prompts_in_a_graph():
     import torch
 
@@ -480,7 +575,8 @@ def test_expanded_prompts_in_a_graph():
 @pytest.mark.parametrize("changes, message", [
     (dict(struct_size=4), "struct_size"), (dict(dtype=2), "row dtype"), (dict(n_heads=3), "multiple"), (dict(n_key_heads=0), "multiple"), (dict(n_heads=0), "multiple"),
     (dict(key_dim=0), "key_dim"), (dict(key_dim=1025), "key_dim"), (dict(value_dim=1025), "value_dim"), (dict(d_values=None, value_dim=9), "value_dim"), (dict(page_size=0), "page_size"),
-    (dict(page_size=1 << 20, max_pages=1 << 20), "page_size"), (dict(n_queries=1 << 32), "queries"), (dict(d_queries=None), "null"), (dict(d_out=None), "null"),
+    (dict(page_size=1 << 20, max_pages=1 << 20), "page_size"), (dict(n_queries=1 << 32), "queries"), (dict(n_queries=65536), "queries"), (dict(n_heads=1 << 16), "65536"),
+    (dict(scale=math.inf), "scale"), (dict(scale=math.nan), "scale"), (dict(d_queries=None), "null"), (dict(d_out=None), "null"),
     (dict(d_table=None), "null"), (dict(d_lengths=None), "null"), (dict(d_keys=None), "null"),
 ])
 def test_paged_attention_refuses_before_any_device_work(changes, message):
@@ -498,7 +594,8 @@ def test_paged_attention_refuses_before_any_device_work(changes, message):
 
 @pytest.mark.parametrize("changes, message", [
     (dict(struct_size=4), "struct_size"), (dict(dtype=3), "row dtype"), (dict(n_heads=0), "n_heads"), (dict(rank=0), "rank"), (dict(rank=1000), "rank"), (dict(value_dim=0), "value_dim"),
-    (dict(nope_dim=1000), "nope_dim"), (dict(n_rows=1 << 31), "too many"), (dict(n_tokens=1 << 31), "too many"), (dict(d_queries=None), "null"), (dict(d_w_key=None), "null"),
+    (dict(nope_dim=1000), "nope_dim"), (dict(n_rows=1 << 31), "too many"), (dict(n_tokens=1 << 31), "too many"), (dict(n_tokens=1 << 28), "too many"),
+    (dict(n_sequences=1 << 21), "too many"), (dict(n_rows=(1 << 27) - 128), "too many"), (dict(scale=-math.inf), "scale"), (dict(d_queries=None), "null"), (dict(d_w_key=None), "null"),
     (dict(d_row_offsets=None), "null"), (dict(d_rows=None), "null"), (dict(d_out=None), "null"),
 ])
 def test_expanded_attention_refuses_before_any_device_work(changes, message):
@@ -512,6 +609,16 @@ def test_expanded_attention_refuses_before_any_device_work(changes, message):
     assert message in L.svsx_last_error().decode()
     assert L.svsx_latent_expanded_device(C.byref(d), 256, 1 << 40, None) == _lib.INVALID_ARGUMENT
     assert L.svsx_latent_expanded_device(None, None, 0, None) == _lib.INVALID_ARGUMENT
+
+
+def test_the_packed_description_is_the_structure():
+    from scalablevectorsearch_amd.attention import _ATTENTION
+
+    fields = [(C.sizeof(_lib.AttentionDesc), 1, 2), range(3, 13), (1 << 40,), (13, 14), (1 << 41,), (15, 16, 17), (1 << 42,), (18, 19, 20), (21, 22, 23), (0.5,), (24, 25)]
+    values = [x for part in fields for x in part]
+    assert _ATTENTION.size == C.sizeof(_lib.AttentionDesc) and len(values) == len(_lib.AttentionDesc._fields_)
+    back = _lib.AttentionDesc.from_buffer_copy(_ATTENTION.pack(*values))
+    assert [getattr(back, name) for name, _ in _lib.AttentionDesc._fields_] == values
 
 
 def test_arrays_on_the_host_are_refused():
@@ -545,6 +652,8 @@ def test_wrong_arguments_are_refused():
         lambda: att(q, keys, values, table.long(), n), lambda: att(q, keys, values, table, n.long()), lambda: att(q, keys, values, table, n[:1]),
         lambda: att(q[:1], keys, values, table, n), lambda: att(q, keys, values, table.cpu(), n), lambda: att(q, keys, values, table, n, sequences=n[:1]),
         lambda: att(q, keys, values, table, n, value_dim=32), lambda: att(q, keys, None, table, n, value_dim=65), lambda: att(q, keys, None, table, n, value_dim=0),
+        lambda: att(q, keys, values, table, n, scale=1e300), lambda: att(q, keys, values, table, n, scale=math.inf), lambda: att(q[..., :0], keys[..., :0], values, table, n),
+        lambda: exp(qe, rows, wk, wv, off, off, scale=1e300), lambda: exp(qe[..., :0], rows[:, :48], wk[:, :0], wv, off, off),
         lambda: att(q[0], keys, values, table, n), lambda: att(q, keys.transpose(2, 3).contiguous().transpose(2, 3), values, table, n),
         lambda: att(torch.zeros(2, 2, 2000, device="cuda"), torch.zeros(3, 1, 4, 2000, device="cuda"), None, table, n),
         lambda: exp(qe, rows.float(), wk, wv, off, off), lambda: exp(qe[:, :3], rows, wk, wv, off, off), lambda: exp(qe, rows[:, :60], wk, wv, off, off),
