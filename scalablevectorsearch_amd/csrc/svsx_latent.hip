@@ -72,10 +72,17 @@ template <typename T> __global__ __launch_bounds__(256) void expanded_head_kerne
     }
 }
 
+struct __align__(16) Tile { // of queries: all that the second launch needs to know of its sequence
+    int32_t first, end;      // queries [first, end): the tile's first one, the sequence's last + 1
+    int32_t begin, rows_end; // its rows, inside the array
+    int32_t shift;           // query t's own row is t + shift
+    int32_t unused[3];
+};
+
 struct Space { // the first launch's results
     void* keys;      // [head][key_rows][DK]
     void* values;    // [head][DV][value_rows]
-    int2* tiles;     // {sequence, first query}
+    Tile* tiles;
     uint32_t* count; // of tiles
     size_t key_rows, value_rows; // at least n_rows + 64: a tile of rows may begin at the last one
     uint32_t dk, dv, most_tiles, tile_queries;
@@ -208,8 +215,14 @@ template <typename T> __device__ __forceinline__ void list_tiles(const ExpandedA
             at += k < wave ? sh[k] : 0;
             base += sh[k];
         }
-        for (uint32_t k = 0; k < n; ++k)
-            if (at + k < w.most_tiles) w.tiles[at + k] = make_int2(static_cast<int>(first + t), static_cast<int>(b + k * w.tile_queries));
+        if (n > 0) {
+            const int32_t rb = a.row_offsets[first + t], re = a.row_offsets[first + t + 1], n_rows = static_cast<int32_t>(a.n_rows);
+            Tile tile = {0, static_cast<int32_t>(e), rb < 0 ? 0 : rb, re < n_rows ? re : n_rows, re - a.query_offsets[first + t + 1], {}};
+            for (uint32_t k = 0; k < n; ++k) {
+                tile.first = static_cast<int32_t>(b + k * w.tile_queries);
+                if (at + k < w.most_tiles) w.tiles[at + k] = tile;
+            }
+        }
     }
     if (t == 0) *w.count = base < w.most_tiles ? base : w.most_tiles;
 }
@@ -301,17 +314,14 @@ template <typename T, int DK, int DV, int NW> struct PromptLayout {
     static constexpr uint32_t kBytes = (kAhead + 1) * kKeyBytes + 2 * kValueBytes;
     static_assert(kBytes <= 160 * 1024 && kGroups % 4 == 0 && DV % 32 == 0, "LDS; loads of four waves");
 };
-template <typename T> __device__ __forceinline__ bool all_finite(const Frag<T>& f) { // no exponent of all ones
-    constexpr uint32_t kExponent = sizeof(T) == 4 ? 0x7F800000u : std::is_same<T, _Float16>::value ? 0x7C00u : 0x7F80u;
-    bool fine = true;
+// Highest bits (of each 16 for the 16-bit types) that are set where an element's exponent is all ones: one more at the exponent's lowest bit carries into the sign's place.
+template <typename T> __device__ __forceinline__ uint32_t not_finite(const Frag<T>& f) {
+    constexpr uint32_t kOne = sizeof(T) == 4 ? 0x00800000u : std::is_same<T, _Float16>::value ? 0x04000400u : 0x00800080u, kSign = sizeof(T) == 4 ? 0x80000000u : 0x80008000u;
+    uint32_t word[sizeof(Frag<T>) / 4], bits = 0;
+    __builtin_memcpy(word, &f, sizeof(f));
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        uint32_t bits;
-        if constexpr (sizeof(T) == 4) bits = __builtin_bit_cast(uint32_t, static_cast<float>(f[e]));
-        else bits = __builtin_bit_cast(uint16_t, static_cast<T>(f[e]));
-        fine = fine && (bits & kExponent) != kExponent;
-    }
-    return fine;
+    for (uint32_t x : word) bits |= (x & ~kSign) + kOne;
+    return bits & kSign;
 }
 
 // One query by one wave, over the expanded rows [begin, last] alone: its lanes across the columns.
@@ -351,15 +361,10 @@ template <typename T, int DK, int DV, int NW> __global__ __launch_bounds__(NW * 
     extern __shared__ __align__(16) unsigned char lds[];
     const uint32_t count = *w.count, turn = blockIdx.x / a.n_heads, h = blockIdx.x % a.n_heads; // a head's tiles on one of the eight L2s where heads are a multiple of 8
     if (turn >= count) return;
-    const int2 tile = w.tiles[count - 1 - turn]; // a sequence's last queries see the most rows: they go first
-    const uint32_t seq = __builtin_amdgcn_readfirstlane(tile.x), q0 = __builtin_amdgcn_readfirstlane(tile.y);
-    uint32_t qb, qe;
-    queries_of(a, seq, &qb, &qe);
-    qe = __builtin_amdgcn_readfirstlane(qe);
+    const Tile tile = w.tiles[count - 1 - turn]; // a sequence's last queries see the most rows: they go first
+    const uint32_t q0 = __builtin_amdgcn_readfirstlane(tile.first), qe = __builtin_amdgcn_readfirstlane(tile.end);
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, r = row32(lane);
-    // rows [begin, end) of the sequence, inside the array; a query at t sees those up to t + shift
-    const int32_t rb = a.row_offsets[seq], re = a.row_offsets[seq + 1], shift = re - a.query_offsets[seq + 1];
-    const int32_t begin = __builtin_amdgcn_readfirstlane(rb < 0 ? 0 : rb), end = __builtin_amdgcn_readfirstlane(re < static_cast<int32_t>(a.n_rows) ? re : static_cast<int32_t>(a.n_rows));
+    const int32_t begin = __builtin_amdgcn_readfirstlane(tile.begin), end = __builtin_amdgcn_readfirstlane(tile.rows_end), shift = __builtin_amdgcn_readfirstlane(tile.shift);
     auto sees = [&](uint32_t t) { // the last row that query t sees; less than begin: none
         const int32_t own = static_cast<int32_t>(t) + shift;
         return a.causal && own < end - 1 ? own : end - 1;
@@ -428,10 +433,12 @@ template <typename T, int DK, int DV, int NW> __global__ __launch_bounds__(NW * 
     auto add_values = [&](uint32_t buffer) {
         const unsigned char* vt = value_buffers + buffer * L::kValueBytes;
         if (pending_edge) { // values of rows that some query does not see: a weight of zero does not take away what is infinite or not a number
+            uint32_t bits = 0;
 #pragma unroll
             for (int d = 0; d < DV / 32; ++d)
 #pragma unroll
-                for (int k = 0; k < 2 * L::kTiles; ++k) odd |= __any(!all_finite<T>(plane_frag<T>(vt, d * 32 + r, k, half)));
+                for (int k = 0; k < 2 * L::kTiles; ++k) bits |= not_finite<T>(plane_frag<T>(vt, d * 32 + r, k, half));
+            odd |= __any(bits != 0);
         }
 #pragma unroll
         for (int k = 0; k < 2 * L::kTiles; ++k)
@@ -595,7 +602,7 @@ PromptRoute route_of(const ExpandedArgs& a, size_t es) {
     w.value_rows = (static_cast<size_t>(a.n_rows) + 63) / 64 * 64 + 64;
     r.values_at = a.n_heads * w.key_rows * r.dk * es;
     r.tiles_at = r.values_at + a.n_heads * w.value_rows * r.dv * es;
-    r.count_at = r.tiles_at + static_cast<size_t>(w.most_tiles) * 8;
+    r.count_at = r.tiles_at + static_cast<size_t>(w.most_tiles) * sizeof(Tile);
     r.bytes = r.count_at + 4;
     return r;
 }
@@ -617,7 +624,7 @@ template <typename T> hipError_t launch_expanded(const ExpandedArgs& a, PromptRo
     Space& w = r.space;
     w.keys = base;
     w.values = base + r.values_at;
-    w.tiles = reinterpret_cast<int2*>(base + r.tiles_at);
+    w.tiles = reinterpret_cast<Tile*>(base + r.tiles_at);
     w.count = reinterpret_cast<uint32_t*>(base + r.count_at);
     ExpandGrid g = {};
     g.key_i = (a.n_heads * a.nope + 127) / 128;
