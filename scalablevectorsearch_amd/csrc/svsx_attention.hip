@@ -64,6 +64,7 @@ template <typename T> __global__ __launch_bounds__(256) void attend_head_kernel(
 //                  (16 bytes) of each of them and transposes that 8 x 8 block in its registers: lane l's columns are 8 (l % 16) .. + 7, the d-th product
 //                  takes the d-th of them.
 // Bound by HBM: 16 heads' products are half the matrix units' time per byte, and 32 rows' keys (of the next 32) and values are in flight per wave, three waves per SIMD.
+// 4 sequences of 131071 rows, 64 heads on 8 (2.15 GB, bfloat16): 383 us, 5.6 TB/s; 64 of up to 8191 rows, 32 heads on 8 (1.07 GB): 220 us, 4.9 TB/s; a kernel that only reads reached 6.3 TB/s.
 // The running maximum of a head is raised only when a score exceeds it by more than 2^kSlack (the accumulators are rescaled then), so the usual 32 rows cost
 // no rescaling; sums are kept per lane and joined at the end.
 //
@@ -392,14 +393,16 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && VB == 1 ? 3 : 2) void attend
     } while (walk.next(a, plan, &c));
 }
 
-// ---- few rows, few heads ---------------------------------------------------------------------------------------------------------------------------
+// ---- few rows, a head a key head ------------------------------------------------------------------------------------------------------------------
 //
-// Attention over the answers of a search: at most a few hundred rows, each somewhere else, for one to four heads.  There is nothing to split and nothing for the matrix
+// Attention over the answers of a search: at most a few hundred rows, each somewhere else, for one head.  There is nothing to split and nothing for the matrix
 // units to share; what counts is how many rows are on their way at once.  One wave takes a query (of one key head): 16 lanes a row, 8 or 16 columns a lane, so four rows
 // at a time; 64 table entries are looked up by the 64 lanes at once; each 16 lanes keep a softmax of their own, joined at the end.
-// 2048 queries of 100 rows of 96 float32 columns: 21 us (78 MB of rows, from a set larger than one L2), and 48 us through attend_group_kernel, whose four waves a query have one tile each.
+// 2048 queries of 100 rows of 96 float32 columns: 22 us (78 MB of rows, from a set larger than one L2), and 48 us through attend_group_kernel, whose four waves a query have one tile each.
+// float16, 128 columns, few against group: 512 queries of 64 rows 8.9 and 12.0 us, of 256 rows 24 and 34, of 512 rows 44 and 55, of 1024 rows 84.5 and 83.5; 128 queries of 64 rows 9.0 and 9.0, of
+// 256 rows 21.5 and 17.3.  With two heads a key head and 8 key heads it is the slower one from 4096 waves on.
 
-constexpr uint32_t kFewRows = 256; // rows up to which a query is one wave's
+constexpr uint32_t kFewRows = 512, kFewItems = 512; // at most so many rows a query; at least so many waves
 
 // sum over the 16 lanes of a row of the wave, for each of them
 __device__ __forceinline__ float sum16(float x) {
@@ -410,7 +413,7 @@ __device__ __forceinline__ float sum16(float x) {
     return x;
 }
 
-template <typename T, int E, int G, bool Wide> __global__ __launch_bounds__(256) void attend_few_kernel(const AttentionArgs a, const Divider by_page) {
+template <typename T, int E, bool Wide> __global__ __launch_bounds__(256) void attend_few_kernel(const AttentionArgs a, const Divider by_page) {
     constexpr int kBatch = E == 8 ? 8 : 4, kFrags = E / 8; // rows that each 16 lanes have on their way
     const uint32_t lane = threadIdx.x & 63, item = blockIdx.x * 4 + (threadIdx.x >> 6), quarter = lane >> 4, n16 = lane & 15;
     if (item >= a.n_queries * a.n_key_heads) return;
@@ -420,22 +423,16 @@ template <typename T, int E, int G, bool Wide> __global__ __launch_bounds__(256)
     const T* keys = static_cast<const T*>(a.keys) + g * a.key_head_stride;
     const T* values = static_cast<const T*>(a.values) + g * a.value_head_stride;
     const float scale = a.scale * kLog2e;
-    float q[G][E], o[G][E], top[G], sum[G];
+    float q[E], o[E], top = -INFINITY, sum = 0.0f;
+    const T* const query = static_cast<const T*>(a.queries) + i * a.query_stride + g * a.query_head_stride;
 #pragma unroll
-    for (int h = 0; h < G; ++h) {
-        const uint32_t head = g * a.group + min(static_cast<uint32_t>(h), a.group - 1);
-        const T* row = static_cast<const T*>(a.queries) + i * a.query_stride + head * a.query_head_stride;
+    for (int f = 0; f < kFrags; ++f) {
+        const Frag<T> x = a.wide_queries ? load_frag<T, true>(query, n16 * E + f * 8, a.dk) : load_frag<T, false>(query, n16 * E + f * 8, a.dk);
 #pragma unroll
-        for (int f = 0; f < kFrags; ++f) {
-            const Frag<T> x = a.wide_queries ? load_frag<T, true>(row, n16 * E + f * 8, a.dk) : load_frag<T, false>(row, n16 * E + f * 8, a.dk);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                q[h][f * 8 + e] = to_f32(x[e]);
-                o[h][f * 8 + e] = 0.0f;
-            }
+        for (int e = 0; e < 8; ++e) {
+            q[f * 8 + e] = to_f32(x[e]);
+            o[f * 8 + e] = 0.0f;
         }
-        top[h] = -INFINITY;
-        sum[h] = 0.0f;
     }
     for (uint32_t base = 0; base < n; base += 64) {
         uint32_t at;
@@ -460,54 +457,48 @@ template <typename T, int E, int G, bool Wide> __global__ __launch_bounds__(256)
                     for (int f = 0; f < kFrags; ++f) v[j][f] = load_frag<T, Wide>(vrow, n16 * E + f * 8, a.dv);
                 }
             }
+            float s[kBatch], most = top;
 #pragma unroll
-            for (int h = 0; h < G; ++h) {
-                float s[kBatch], most = top[h];
+            for (int j = 0; j < kBatch; ++j) {
+                float x = 0.0f;
 #pragma unroll
-                for (int j = 0; j < kBatch; ++j) {
-                    float x = 0.0f;
+                for (int e = 0; e < E; ++e) x = fmaf(to_f32(k[j][e >> 3][e & 7]), q[e], x);
+                s[j] = there[j] ? sum16(x) * scale : -INFINITY;
+                most = fmaxf(most, s[j]);
+            }
+            const float ref = most == -INFINITY ? 0.0f : most, was = exp2_fast(top - ref);
+            top = most;
+            sum *= was;
 #pragma unroll
-                    for (int e = 0; e < E; ++e) x = fmaf(to_f32(k[j][e >> 3][e & 7]), q[h][e], x);
-                    s[j] = there[j] ? sum16(x) * scale : -INFINITY;
-                    most = fmaxf(most, s[j]);
-                }
-                const float ref = most == -INFINITY ? 0.0f : most, was = exp2_fast(top[h] - ref);
-                top[h] = most;
-                sum[h] *= was;
+            for (int e = 0; e < E; ++e) o[e] *= was;
 #pragma unroll
-                for (int e = 0; e < E; ++e) o[h][e] *= was;
+            for (int j = 0; j < kBatch; ++j) {
+                const float p = exp2_fast(s[j] - ref);
+                sum += p;
+                if (there[j]) { // what a row that is not there would be read from is not defined
 #pragma unroll
-                for (int j = 0; j < kBatch; ++j) {
-                    const float p = exp2_fast(s[j] - ref);
-                    sum[h] += p;
-                    if (there[j]) { // what a row that is not there would be read from is not defined
-#pragma unroll
-                        for (int e = 0; e < E; ++e) o[h][e] = fmaf(p, to_f32(a.shared ? k[j][e >> 3][e & 7] : v[j][e >> 3][e & 7]), o[h][e]);
-                    }
+                    for (int e = 0; e < E; ++e) o[e] = fmaf(p, to_f32(a.shared ? k[j][e >> 3][e & 7] : v[j][e >> 3][e & 7]), o[e]);
                 }
             }
         }
     }
 #pragma unroll
-    for (int h = 0; h < G; ++h) {
+    for (int off = 16; off <= 32; off <<= 1) {
+        const float other = __shfl_xor(top, off), all = fmaxf(top, other);
+        const float mine = top == -INFINITY ? 0.0f : exp2_fast(top - all), theirs = other == -INFINITY ? 0.0f : exp2_fast(other - all);
+        sum = sum * mine + __shfl_xor(sum, off) * theirs;
 #pragma unroll
-        for (int off = 16; off <= 32; off <<= 1) {
-            const float other = __shfl_xor(top[h], off), all = fmaxf(top[h], other);
-            const float mine = top[h] == -INFINITY ? 0.0f : exp2_fast(top[h] - all), theirs = other == -INFINITY ? 0.0f : exp2_fast(other - all);
-            sum[h] = sum[h] * mine + __shfl_xor(sum[h], off) * theirs;
-#pragma unroll
-            for (int e = 0; e < E; ++e) o[h][e] = o[h][e] * mine + __shfl_xor(o[h][e], off) * theirs;
-            top[h] = all;
-        }
-        if (static_cast<uint32_t>(h) >= a.group || quarter != 0) continue;
-        const size_t at = static_cast<size_t>(i) * a.n_heads + g * a.group + h;
-        const float inv = sum[h] == 0.0f ? 0.0f : 1.0f / sum[h];
-        T* out = static_cast<T*>(a.out) + at * a.dv;
-#pragma unroll
-        for (uint32_t e = 0; e < E; ++e)
-            if (n16 * E + e < a.dv) out[n16 * E + e] = from_f32<T>(o[h][e] * inv);
-        if (a.lse && n16 == 0) a.lse[at] = sum[h] == 0.0f ? -INFINITY : (top[h] + log2f(sum[h])) * kLn2;
+        for (int e = 0; e < E; ++e) o[e] = o[e] * mine + __shfl_xor(o[e], off) * theirs;
+        top = all;
     }
+    if (quarter != 0) return;
+    const size_t at = static_cast<size_t>(i) * a.n_heads + g;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    T* out = static_cast<T*>(a.out) + at * a.dv;
+#pragma unroll
+    for (uint32_t e = 0; e < E; ++e)
+        if (n16 * E + e < a.dv) out[n16 * E + e] = from_f32<T>(o[e] * inv);
+    if (a.lse && n16 == 0) a.lse[at] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
 }
 
 // ---- rows that are key and value at once, for many heads ------------------------------------------------------------------------------------------
@@ -522,8 +513,10 @@ template <typename T, int E, int G, bool Wide> __global__ __launch_bounds__(256)
 // LDS holds a row as 16-byte words in planes of 64 words, rows 32 bytes further apart than they are long, so that neither eight rows of a key fragment nor the 16
 // half-words of a transposed one meet in a bank; and a narrow plane for the rest, which is brought in several rows at a time and has its words exchanged in fours instead.
 // (Exchanging single words of the long rows as well, with no padding, was measured: the loads then cross each 64-byte line out of order and cost twice the time.)
-// At 16 heads HBM bounds it; at 64 the latency of the steps between a tile's barriers (LDS is busy for 2400 cycles of a tile's 8800, the matrix units for 2176).  Two workgroups
-// of 32-row buffers and four waves on a compute unit were measured in place of one of eight waves: their registers spill, 104 -> 127 us (32 sequences, 128 heads).
+// 32 sequences of up to 8192 rows, 128 heads (36.5 GFLOP, 160 MB, bfloat16): 98 us, 373 TFLOP/s; one of 4097 rows, 16 heads: 17 us.
+// At 16 heads HBM bounds it; at 64 the latency of the steps between a tile's barriers (LDS is busy for 2400 cycles of a tile's 8000, the matrix units for 2176, and the loads straight to LDS,
+// which come to 30 bytes a cycle, for 2400).  Measured in place of it, 32 sequences, 128 heads: two workgroups of 32-row buffers and four waves on a compute unit, whose registers spill, 104 -> 127 us; four
+// waves of 512 registers that take 32 rows for 32 heads and read LDS half as often, 98 -> 112 us, since a wave stands still while it gives out loads and no other wave is there.
 
 template <typename T, int KS, int HT> struct RowsLayout { // KS: 32-column steps of a key row; HT: 16-head tiles
     static constexpr uint32_t kRows = 64;                                      // rows of a tile
@@ -983,7 +976,7 @@ int check_attention(const svsx_attention_desc* d, AttentionArgs* a) {
 
 // How a call is answered; decided from sizes, types, strides and addresses alone.
 struct Route {
-    bool rows, group, few; // many heads over shared rows, or heads that share a key head, on the matrix units; few rows and heads; else one workgroup per head
+    bool rows, group, few; // many heads over shared rows, or heads that share a key head, on the matrix units; few rows, one head; else one workgroup per head
     bool wide, page8;
     int ks, vb, ht;
     uint32_t workers, unit, y;
@@ -1002,10 +995,12 @@ Route route_of(const AttentionArgs& a, size_t es) {
     };
     r.wide = a.dk % 8 == 0 && a.dv % 8 == 0 && aligned({a.key_page_stride, a.key_head_stride, a.key_row_stride}, a.keys) &&
              aligned({a.value_page_stride, a.value_head_stride, a.value_row_stride}, a.values);
-    // Shared rows go through LDS where more than 16 heads read them, and where they are too long for the registers of the other kernel
-    r.rows = a.shared && r.wide && a.dk <= 576 && a.dv <= 512 && (a.group > 16 || a.dk > 256);
+    // Shared rows go through LDS where more than 16 heads read them, and where they are so long that the other kernel reads them twice (32 queries of 4096 float16 rows: 16 heads,
+    // 128 columns 25 us either way, 256 columns 26 us against 45; 32 heads 27 against 29, 29 against 52; 8 heads, 128 columns 24 against 22).
+    r.rows = a.shared && r.wide && a.dk <= 576 && a.dv <= 512 && (a.group > 16 || a.dk > 128);
     const uint64_t most = static_cast<uint64_t>(a.max_pages) * a.page_size; // rows that a query can have
-    r.few = most <= kFewRows && a.group <= 4 && a.dk <= 256 && a.dv <= 256 && static_cast<uint64_t>(a.n_queries) * a.n_key_heads <= 1u << 25; // a grid has fewer than 2^32 threads
+    const uint64_t items = static_cast<uint64_t>(a.n_queries) * a.n_key_heads; // one wave each
+    r.few = a.group == 1 && most <= kFewRows && items >= kFewItems && items <= 1u << 25 && a.dk <= 256 && a.dv <= 256; // a grid has fewer than 2^32 threads
     if (r.few) {
         r.rows = false;
         return r;
@@ -1014,7 +1009,9 @@ Route route_of(const AttentionArgs& a, size_t es) {
     if (!r.rows && !r.group) return r;
     if (r.rows) {
         r.ks = a.dk <= 320 && a.dv <= 256 ? 10 : 18;
-        r.ht = a.group <= 16 || es == 4 ? 1 : a.group <= 32 ? 2 : 4; // float32 queries of 16 heads fill the registers
+        // 32 sequences of 4096 bfloat16 rows, 576 columns, by 16, 32 or 64 heads a workgroup: 16 heads 36, 38, 44 us; 32 heads 48, 41, 46; 64 heads 79, 59, 54; 128 heads 136, 94, 79.
+        // float32 queries of 16 heads fill the registers.
+        r.ht = a.group <= 16 || es == 4 ? 1 : a.group <= 32 ? 2 : 4;
         r.unit = 64;
         r.y = a.n_key_heads * ((a.group + r.ht * 16 - 1) / (r.ht * 16));
     } else {
@@ -1025,10 +1022,11 @@ Route route_of(const AttentionArgs& a, size_t es) {
         r.y = a.n_key_heads * ((a.group + 15) / 16);
     }
     // One workgroup a query where queries alone fill the machine several times over, where no query can have more rows than one unit, or where the sum of all units
-    // might not fit 32 bits.
+    // might not fit 32 bits.  32 heads on 8 of 128 float16 columns, one workgroup a query against equal runs: 512 queries of 1000 rows 305 and 385 us, of lengths up to 1000 204 and 231; but 256
+    // queries, two of them of 4000 rows and the others below 500, 149 and 86.
     const uint32_t resident = kUnits * (r.rows ? 1 : r.vb == 2 || es == 4 ? 2 : 3);
     const uint64_t groups = static_cast<uint64_t>(a.n_queries) * r.y, units = (most + r.unit - 1) / r.unit;
-    if (groups >= 8 * resident || units <= 1 || units * a.n_queries >= (1ull << 32)) return r;
+    if (groups >= 4 * resident || units <= 1 || units * a.n_queries >= (1ull << 32)) return r;
     r.workers = static_cast<uint32_t>(std::min<uint64_t>(std::max(1u, resident / r.y), a.n_queries * units));
     const size_t parts = (static_cast<size_t>(r.workers) + a.n_queries) * a.n_heads;
     r.stats_at = (parts * a.dv * 4 + 15) / 16 * 16;
@@ -1094,11 +1092,8 @@ template <typename T> hipError_t launch_attention(const AttentionArgs& a, const 
         const bool narrow = a.dk <= 128 && a.dv <= 128;
         typedef void (*Kernel)(const AttentionArgs, const Divider);
         Kernel kernel;
-#define SVSX_FEW(E, G) (r.wide ? attend_few_kernel<T, E, G, true> : attend_few_kernel<T, E, G, false>)
-        if (a.group == 1) kernel = narrow ? SVSX_FEW(8, 1) : SVSX_FEW(16, 1);
-        else if (a.group == 2) kernel = narrow ? SVSX_FEW(8, 2) : SVSX_FEW(16, 2);
-        else kernel = narrow ? SVSX_FEW(8, 4) : SVSX_FEW(16, 4);
-#undef SVSX_FEW
+        if (narrow) kernel = r.wide ? attend_few_kernel<T, 8, true> : attend_few_kernel<T, 8, false>;
+        else kernel = r.wide ? attend_few_kernel<T, 16, true> : attend_few_kernel<T, 16, false>;
         hipLaunchKernelGGL(kernel, dim3((a.n_queries * a.n_key_heads + 3) / 4), dim3(256), 0, stream, a, divider(a.page_size));
         return hipGetLastError();
     }

@@ -126,7 +126,8 @@ template <typename T, bool Wide> __device__ __forceinline__ Word<T> load_word(co
 }
 
 // C[i][j] = sum_k A[i][k] B[j][k] for one 128 x 128 tile; four waves of 64 x 64.  row_a(i) / row_b(j): the row, NULL = zeros.  put(i, j, v): eight consecutive i of one j.
-// The next 128 bytes of every row are on their way to registers while these are multiplied.
+// The next 128 bytes of every row are on their way to registers while these are multiplied.  8190 rows of rank 512 for 32 heads (68.7 GFLOP): 106 us, half of what a library product reaches; LDS is busy one and a
+// half times as long as the matrix units.  Two buffers and one barrier a step were measured in place of one buffer: 333 tokens 25.4 -> 27.3 us, as fewer workgroups fit a compute unit.
 template <typename T, bool Wide, typename A, typename B, typename P> __device__ __forceinline__ void product_tile(unsigned char* lds, uint32_t depth, A row_a, B row_b, P put) {
     const uint32_t t = threadIdx.x, lane = t & 63, wave = t >> 6, half = lane >> 5, r = row32(lane);
     unsigned char* const plane_a = lds;
@@ -306,6 +307,7 @@ template <typename T, bool Wide> __global__ __launch_bounds__(256) void expand_k
 // A query is a lane's column throughout, so its maximum, sum and rescaling need one exchange between two lanes.  Per 64 rows a wave has 1280 cycles of products
 // (DK 192, DV 128) against 320 of LDS reads, which eight waves share, and about 1000 of softmax on the vector units: so of the two waves on a SIMD, one does its products (a tile's
 // scores and the last tile's values) while the other does its softmax, and they change over at a barrier.
+// 4095 queries on 8190 rows, 32 heads, bfloat16: 437 us, 1.18 PFLOP/s, 87 % of what an 8192^3 library product reaches.
 template <typename T, int DK, int DV, int NW> struct PromptLayout {
     static constexpr uint32_t kRows = kPlaneCols<T>; // of a tile: a plane of V^T
     static constexpr int kKeyPlanes = DK / kPlaneCols<T>, kTiles = kRows / 32;
@@ -591,7 +593,8 @@ PromptRoute route_of(const ExpandedArgs& a, size_t es) {
     r.dv = r.dk == 256 ? 256 : a.dv <= 64 ? 64 : 128;
     const size_t elems = 16 / es;
     r.wide = a.rank % elems == 0 && ((reinterpret_cast<size_t>(a.rows) | reinterpret_cast<size_t>(a.w_key) | reinterpret_cast<size_t>(a.w_value) | a.row_stride * es) & 15) == 0;
-    // Eight waves share a tile's rows where that leaves every compute unit a workgroup; float32 and 256-column heads have no registers for two waves a SIMD.
+    // Eight waves share a tile's rows where that leaves every compute unit a workgroup (causal prompts, 4 and 8 waves: 512 tokens, 16 heads 34 and 38 us; 1000, 32 heads 60 and 60; 2048, 32 heads
+    // 125 and 115; 4096, 32 heads 325 and 243); float32 and 256-column heads have no registers for two waves a SIMD.
     r.waves = es == 2 && r.dk <= 192 && static_cast<uint64_t>(a.n_tokens) * a.n_heads >= 256 * 256 ? 8 : 4;
     Space& w = r.space;
     w.dk = r.dk;

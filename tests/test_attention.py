@@ -361,6 +361,26 @@ def test_a_run_of_the_operators_together():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kv, dim, value_dim, page, shared", [(2, 96, 40, 1, False), (2, 100, 100, 5, False), (3, 256, 200, 8, False), (2, 128, 64, 4, True), (2, 33, 33, 1, True)])
+def test_many_queries_of_few_rows(dtype, kv, dim, value_dim, page, shared):
+    """as the answers of a search are: some missing, some queries without any, rows with NaN that few see"""
+    import torch
+
+    g = torch.Generator().manual_seed(4)
+    lengths = torch.randint(0, 90, (300,), generator=g).tolist()
+    lengths[:4] = [0, 1, 64, 65]
+    q, keys, values, table, n = _case(dtype, lengths, kv, kv, dim, value_dim, page, seed=4, shared=shared)
+    holes = torch.rand(table.shape, generator=g) < 0.05
+    holes[9] = True
+    table[holes.cuda()] = torch.tensor([-1, keys.shape[0]], dtype=torch.int32).cuda()[torch.arange(int(holes.sum())).cuda() % 2]
+    table[11, 0] = table[12, 0]
+    n[11:13] = n[11:13].clamp_min(1)
+    keys[table[12, 0].long().clamp(0, keys.shape[0] - 1), 0, 0, 0] = math.nan
+    _run(q, keys, values, table, n, value_dim=value_dim)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("heads, kv, dim, value_dim, page, shared", [(2, 2, 64, 64, 4, False), (1, 1, 64, 64, 16, False), (1, 1, 288, 256, 16, True), (1, 1, 260, 20, 2, False)])
 def test_as_many_queries_as_a_call_takes(heads, kv, dim, value_dim, page, shared):
     import torch
