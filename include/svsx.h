@@ -495,7 +495,9 @@ int svsx_paged_attention_device(const svsx_attention_desc* desc, void* d_workspa
  *   d_queries  [n_tokens][n_heads][nope_dim + rope_dim]     d_rows     [n_rows][rank + rope_dim]
  *   d_w_key    [n_heads][nope_dim][rank], contiguous        d_w_value  [n_heads][value_dim][rank], contiguous
  *   d_out      [n_tokens][n_heads][value_dim], contiguous; a query that sees no row gives zeros.  Queries in no sequence: zeros, or with keep_rest left alone.
- * nope_dim + rope_dim, value_dim and rank + rope_dim are at most 1024; n_rows < 2^27 - 128, n_tokens * n_heads < 2^29, n_sequences * n_heads < 2^22; scale is finite.  For the 16-bit types the expanded keys and values are rounded to dtype. */
+ * nope_dim + rope_dim, value_dim and rank + rope_dim are at most 1024; n_rows < 2^27 - 128, n_tokens * n_heads < 2^29, n_sequences * n_heads < 2^22; scale is finite.  For the 16-bit types the expanded keys and values, and the
+ * softmax's weights before they meet the values, are rounded to dtype.  Where a float16 key or value would exceed 65504, the queries of that head that see its 128 rows are answered in the
+ * latent space instead, in float32 and row by row. */
 typedef struct {
     size_t struct_size; /* sizeof(svsx_expanded_desc) */
     int device;

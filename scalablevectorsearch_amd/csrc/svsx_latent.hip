@@ -83,9 +83,14 @@ struct Space { // the first launch's results
     void* keys;      // [head][key_rows][DK]
     void* values;    // [head][DV][value_rows]
     Tile* tiles;
-    uint32_t* count; // of tiles
+    uint32_t* count;  // of tiles
+    uint32_t* beyond; // float16: per workgroup that multiplies (keys, then values), whether a finite result of its 128 x 128 is infinite in the row type
     size_t key_rows, value_rows; // at least n_rows + 64: a tile of rows may begin at the last one
     uint32_t dk, dv, most_tiles, tile_queries;
+};
+
+struct ExpandGrid { // workgroups of the first launch: keys, values, rotary parts, then one for the tiles
+    uint32_t key_i, keys, value_i, values, copies;
 };
 
 // A plane in LDS is rows of 128 bytes (8 words of 16), in groups of eight rows that lie 16 bytes further apart than they are long; in the third and fourth
@@ -125,10 +130,24 @@ template <typename T, bool Wide> __device__ __forceinline__ Word<T> load_word(co
     return w;
 }
 
+// Highest bits (of each 16 for the 16-bit types) that are set where an element's exponent is all ones: one more at the exponent's lowest bit carries into the sign's place.
+template <typename T> __device__ __forceinline__ uint32_t not_finite(const Frag<T>& f) {
+    constexpr uint32_t kOne = sizeof(T) == 4 ? 0x00800000u : std::is_same<T, _Float16>::value ? 0x04000400u : 0x00800080u, kSign = sizeof(T) == 4 ? 0x80000000u : 0x80008000u;
+    uint32_t word[sizeof(Frag<T>) / 4], bits = 0;
+    __builtin_memcpy(word, &f, sizeof(f));
+#pragma unroll
+    for (uint32_t x : word) bits |= (x & ~kSign) + kOne;
+    return bits & kSign;
+}
+
+// Float16 holds 65504 at most, and a projected row may be larger although its products with queries, or its weighted mean, are ordinary numbers.  (bfloat16 has float32's range.)
+template <typename T> inline constexpr bool kNarrow = std::is_same<T, _Float16>::value;
+
 // C[i][j] = sum_k A[i][k] B[j][k] for one 128 x 128 tile; four waves of 64 x 64.  row_a(i) / row_b(j): the row, NULL = zeros.  put(i, j, v): eight consecutive i of one j.
+// Returns, to every thread, whether a finite sum of the tile is infinite in a row type of less range (false for the other types, without asking).
 // The next 128 bytes of every row are on their way to registers while these are multiplied.  8190 rows of rank 512 for 32 heads (68.7 GFLOP): 106 us, half of what a library product reaches; LDS is busy one and a
 // half times as long as the matrix units.  Two buffers and one barrier a step were measured in place of one buffer: 333 tokens 25.4 -> 27.3 us, as fewer workgroups fit a compute unit.
-template <typename T, bool Wide, typename A, typename B, typename P> __device__ __forceinline__ void product_tile(unsigned char* lds, uint32_t depth, A row_a, B row_b, P put) {
+template <typename T, bool Wide, typename A, typename B, typename P> __device__ __forceinline__ bool product_tile(unsigned char* lds, uint32_t depth, A row_a, B row_b, P put) {
     const uint32_t t = threadIdx.x, lane = t & 63, wave = t >> 6, half = lane >> 5, r = row32(lane);
     unsigned char* const plane_a = lds;
     unsigned char* const plane_b = lds + 16 * kGroupBytes;
@@ -170,6 +189,7 @@ template <typename T, bool Wide, typename A, typename B, typename P> __device__ 
             for (int i = 0; i < 4; ++i) c[i >> 1][i & 1] = product32(fa[i >> 1], fb[i & 1], c[i >> 1][i & 1]);
         }
     }
+    bool beyond = false;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -179,13 +199,13 @@ template <typename T, bool Wide, typename A, typename B, typename P> __device__ 
                 Frag<T> v;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] = from_f32<T>(c[i][j][8 * k + e]);
+                if (kNarrow<T> && not_finite<T>(v)) // 65520, halfway to 2^16, is the first that is rounded up
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) beyond |= fabsf(c[i][j][8 * k + e]) >= 65520.0f && fabsf(c[i][j][8 * k + e]) < INFINITY;
                 put((wave & 1) * 64 + i * 32 + 16 * k + 8 * half, (wave >> 1) * 64 + j * 32 + r, v);
             }
+    return kNarrow<T> && __syncthreads_or(beyond);
 }
-
-struct ExpandGrid { // workgroups of the first launch: keys, values, rotary parts, then one for the tiles
-    uint32_t key_i, keys, value_i, values, copies;
-};
 
 // the queries of sequence i, inside the array
 __device__ __forceinline__ void queries_of(const ExpandedArgs& a, uint32_t i, uint32_t* begin, uint32_t* end) {
@@ -237,7 +257,7 @@ template <typename T, bool Wide> __global__ __launch_bounds__(256) void expand_k
     if (block < grid.keys) { // i: (head, column), j: row
         const uint32_t i0 = block % grid.key_i * 128, j0 = block / grid.key_i * 128, n = a.n_heads * a.nope;
         const T* wk = static_cast<const T*>(a.w_key);
-        product_tile<T, Wide>(
+        const bool beyond = product_tile<T, Wide>(
             lds, a.rank, [&](uint32_t i) { return i0 + i < n ? wk + static_cast<size_t>(i0 + i) * a.rank : nullptr; },
             [&](uint32_t j) { return j0 + j < a.n_rows ? rows + static_cast<size_t>(j0 + j) * a.row_stride : nullptr; },
             [&](uint32_t i, uint32_t j, const Frag<T>& v) {
@@ -252,13 +272,14 @@ template <typename T, bool Wide> __global__ __launch_bounds__(256) void expand_k
                     }
                 }
             });
+        if (kNarrow<T> && threadIdx.x == 0) w.beyond[blockIdx.x] = beyond;
         return;
     }
     block -= grid.keys;
     if (block < grid.values) { // i: row, j: (head, column); zeros in columns beyond the head's and rows beyond the last
         const uint32_t i0 = block % grid.value_i * 128, j0 = block / grid.value_i * 128, n = a.n_heads * w.dv;
         const T* wv = static_cast<const T*>(a.w_value);
-        product_tile<T, Wide>(
+        const bool beyond = product_tile<T, Wide>(
             lds, a.rank, [&](uint32_t i) { return i0 + i < a.n_rows ? rows + static_cast<size_t>(i0 + i) * a.row_stride : nullptr; },
             [&](uint32_t j) {
                 const uint32_t h = (j0 + j) / w.dv, col = (j0 + j) % w.dv;
@@ -267,6 +288,7 @@ template <typename T, bool Wide> __global__ __launch_bounds__(256) void expand_k
             [&](uint32_t i, uint32_t j, const Frag<T>& v) {
                 if (i0 + i < w.value_rows && j0 + j < n) *reinterpret_cast<Frag<T>*>(values + static_cast<size_t>(j0 + j) * w.value_rows + i0 + i) = v;
             });
+        if (kNarrow<T> && threadIdx.x == 0) w.beyond[blockIdx.x] = beyond;
         return;
     }
     block -= grid.values;
@@ -315,17 +337,8 @@ template <typename T, int DK, int DV, int NW> struct PromptLayout {
     static constexpr uint32_t kAhead = 3 * kKeyBytes + 2 * kValueBytes <= 160 * 1024 ? 2 : 1; // tiles that keys are brought in ahead of their use
     static constexpr uint32_t kBytes = (kAhead + 1) * kKeyBytes + 2 * kValueBytes;
     static_assert(kBytes <= 160 * 1024 && kGroups % 4 == 0 && DV % 32 == 0, "LDS; loads of four waves");
+    static_assert(!kNarrow<T> || kBytes >= NW * 2 * kMaxDim * sizeof(float), "latent_query's LDS");
 };
-// Highest bits (of each 16 for the 16-bit types) that are set where an element's exponent is all ones: one more at the exponent's lowest bit carries into the sign's place.
-template <typename T> __device__ __forceinline__ uint32_t not_finite(const Frag<T>& f) {
-    constexpr uint32_t kOne = sizeof(T) == 4 ? 0x00800000u : std::is_same<T, _Float16>::value ? 0x04000400u : 0x00800080u, kSign = sizeof(T) == 4 ? 0x80000000u : 0x80008000u;
-    uint32_t word[sizeof(Frag<T>) / 4], bits = 0;
-    __builtin_memcpy(word, &f, sizeof(f));
-#pragma unroll
-    for (uint32_t x : word) bits |= (x & ~kSign) + kOne;
-    return bits & kSign;
-}
-
 // One query by one wave, over the expanded rows [begin, last] alone: its lanes across the columns.
 template <typename T, int DK, int DV> __device__ void slow_query(const ExpandedArgs& a, const Space& w, uint32_t t, uint32_t h, int32_t begin, int32_t last) {
     const uint32_t lane = threadIdx.x & 63, dk = a.nope + a.rope;
@@ -358,7 +371,68 @@ template <typename T, int DK, int DV> __device__ void slow_query(const ExpandedA
         if (lane + 64 * i < a.dv) out[lane + 64 * i] = from_f32<T>(o[i] * inv);
 }
 
-template <typename T, int DK, int DV, int NW> __global__ __launch_bounds__(NW * 64) void prompt_kernel(const ExpandedArgs a, const Space w) {
+// Whether an expanded key or value of head h, in rows begin .. last, is infinite only for the row type's range (with what shares its workgroup in the first launch).  For
+// all threads of the workgroup.  Asking takes 333 tokens of 16 heads from 23.2 to 24.4 us; 4095 on 8190 rows, 32 heads, are as they were.
+__device__ __forceinline__ bool any_beyond(const ExpandedArgs& a, const Space& w, const ExpandGrid& grid, uint32_t h, int32_t begin, int32_t last) {
+    bool beyond = false;
+    if (begin <= last) {
+        const uint32_t r0 = static_cast<uint32_t>(begin) / 128, rows = static_cast<uint32_t>(last) / 128 - r0 + 1;
+        const uint32_t k0 = h * a.nope / 128, ks = a.nope ? ((h + 1) * a.nope - 1) / 128 - k0 + 1 : 0; // workgroups across the head's columns
+        const uint32_t v0 = h * w.dv / 128, vs = ((h + 1) * w.dv - 1) / 128 - v0 + 1;
+        for (uint32_t r = threadIdx.x; r < rows; r += blockDim.x) {
+            for (uint32_t k = 0; k < ks; ++k) beyond |= w.beyond[(r0 + r) * grid.key_i + k0 + k] != 0;
+            for (uint32_t v = 0; v < vs; ++v) beyond |= w.beyond[grid.keys + (v0 + v) * grid.value_i + r0 + r] != 0;
+        }
+    }
+    return __syncthreads_or(beyond);
+}
+
+// One query by one wave in the latent space, where nothing is rounded on the way: w_key applied to the query, rows [begin, last], w_value to the result.  Lanes across the
+// columns; the query and the sums are in the wave's own `lds` (2 kMaxDim floats), so that this rare path takes no registers from the usual one.
+template <typename T> __device__ __forceinline__ void latent_query(const ExpandedArgs& a, uint32_t t, uint32_t h, int32_t begin, int32_t last, float* lds) {
+    const uint32_t lane = threadIdx.x & 63, width = a.rank + a.rope;
+    const T* query = static_cast<const T*>(a.queries) + t * a.query_stride + h * a.query_head_stride;
+    float *const q = lds, *const o = lds + kMaxDim;
+    float top = -INFINITY, sum = 0.0f;
+#pragma unroll 1
+    for (uint32_t c = lane; c < width; c += 64) {
+        const T* w = static_cast<const T*>(a.w_key) + static_cast<size_t>(h) * a.nope * a.rank + c;
+        float x = c < a.rank ? 0.0f : to_f32(query[a.nope + c - a.rank]);
+#pragma unroll 1
+        for (uint32_t d = 0; c < a.rank && d < a.nope; ++d) x = fmaf(to_f32(query[d]), to_f32(w[static_cast<size_t>(d) * a.rank]), x);
+        q[c] = x;
+        o[c] = 0.0f;
+    }
+#pragma unroll 1
+    for (int32_t r = begin; r <= last; ++r) {
+        const T* row = static_cast<const T*>(a.rows) + static_cast<size_t>(r) * a.row_stride;
+        float s = 0.0f;
+#pragma unroll 1
+        for (uint32_t c = lane; c < width; c += 64) s = fmaf(q[c], to_f32(row[c]), s);
+#pragma unroll
+        for (int off = 32; off >= 1; off >>= 1) s += __shfl_xor(s, off);
+        s *= a.scale;
+        if (s == -INFINITY) continue; // no weight; it must not become the difference of two infinities
+        const float raised = s > top || s != s ? s : top, was = expf(top - raised), p = expf(s - raised);
+        top = raised;
+        sum = fmaf(sum, was, p);
+#pragma unroll 1
+        for (uint32_t c = lane; c < a.rank; c += 64) o[c] = fmaf(p, to_f32(row[c]), o[c] * was);
+    }
+    __threadfence_block(); // each lane reads the others' sums
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll 1
+    for (uint32_t c = lane; c < a.dv; c += 64) {
+        const T* w = static_cast<const T*>(a.w_value) + (static_cast<size_t>(h) * a.dv + c) * a.rank;
+        float y = 0.0f;
+#pragma unroll 1
+        for (uint32_t d = 0; d < a.rank; ++d) y = fmaf(o[d], to_f32(w[d]), y);
+        static_cast<T*>(a.out)[(static_cast<size_t>(t) * a.n_heads + h) * a.dv + c] = from_f32<T>(y * inv);
+    }
+    __threadfence_block(); // the next query's sums go where these were
+}
+
+template <typename T, int DK, int DV, int NW> __global__ __launch_bounds__(NW * 64) void prompt_kernel(const ExpandedArgs a, const Space w, const ExpandGrid grid) {
     typedef PromptLayout<T, DK, DV, NW> L;
     extern __shared__ __align__(16) unsigned char lds[];
     const uint32_t count = *w.count, turn = blockIdx.x / a.n_heads, h = blockIdx.x % a.n_heads; // a head's tiles on one of the eight L2s where heads are a multiple of 8
@@ -388,6 +462,12 @@ template <typename T, int DK, int DV, int NW> __global__ __launch_bounds__(NW * 
 #pragma unroll
                 for (int e = 0; e < 8; ++e) q[s][e] = a.scale < 0.0f ? -q[s][e] : from_f32<T>(0.0f);
             }
+        }
+    }
+    if constexpr (kNarrow<T>) {
+        if (any_beyond(a, w, grid, h, begin, group_last)) {
+            for (uint32_t t = q0 + wave * 32; t <= min(q_last, q0 + wave * 32 + 31); ++t) latent_query<T>(a, t, h, begin, sees(t), reinterpret_cast<float*>(lds) + wave * (2 * kMaxDim));
+            return;
         }
     }
     // the compiler is to wait for the queries here: in the loop, where it cannot tell them from the rows on their way, it would wait for both
@@ -581,11 +661,13 @@ struct PromptRoute {
     bool wide;
     int dk, dv, waves;
     Space space;
-    size_t values_at, tiles_at, count_at, bytes;
+    ExpandGrid grid;
+    size_t values_at, tiles_at, count_at, beyond_at, bytes;
 };
 
-PromptRoute route_of(const ExpandedArgs& a, size_t es) {
+PromptRoute route_of(const ExpandedArgs& a, int dtype) {
     PromptRoute r = {};
+    const size_t es = paged_dtype_size(dtype);
     const uint32_t dk = a.nope + a.rope;
     r.tiles = dk <= 256 && a.dv <= 256;
     if (!r.tiles) return r;
@@ -606,15 +688,22 @@ PromptRoute route_of(const ExpandedArgs& a, size_t es) {
     r.values_at = a.n_heads * w.key_rows * r.dk * es;
     r.tiles_at = r.values_at + a.n_heads * w.value_rows * r.dv * es;
     r.count_at = r.tiles_at + static_cast<size_t>(w.most_tiles) * sizeof(Tile);
-    r.bytes = r.count_at + 4;
+    r.beyond_at = r.count_at + 4;
+    ExpandGrid& g = r.grid;
+    g.key_i = (a.n_heads * a.nope + 127) / 128;
+    g.keys = g.key_i * ((a.n_rows + 127) / 128);
+    g.value_i = static_cast<uint32_t>((w.value_rows + 127) / 128);
+    g.values = g.value_i * ((a.n_heads * r.dv + 127) / 128);
+    g.copies = 1024;
+    r.bytes = r.beyond_at + (dtype == SVSX_F16 ? 4 * (static_cast<size_t>(g.keys) + g.values) : 0);
     return r;
 }
 
-template <typename T, int DK, int DV, int NW> hipError_t launch_prompt(const ExpandedArgs& a, const Space& w, hipStream_t stream) {
+template <typename T, int DK, int DV, int NW> hipError_t launch_prompt(const ExpandedArgs& a, const Space& w, const ExpandGrid& g, hipStream_t stream) {
     typedef PromptLayout<T, DK, DV, NW> L;
     static std::atomic<uint64_t> granted{0};
     if (const hipError_t e = grant_lds(reinterpret_cast<const void*>(prompt_kernel<T, DK, DV, NW>), L::kBytes, &granted); e != hipSuccess) return e;
-    hipLaunchKernelGGL((prompt_kernel<T, DK, DV, NW>), dim3(w.most_tiles * a.n_heads), dim3(NW * 64), L::kBytes, stream, a, w);
+    hipLaunchKernelGGL((prompt_kernel<T, DK, DV, NW>), dim3(w.most_tiles * a.n_heads), dim3(NW * 64), L::kBytes, stream, a, w, g);
     return hipGetLastError();
 }
 
@@ -629,25 +718,21 @@ template <typename T> hipError_t launch_expanded(const ExpandedArgs& a, PromptRo
     w.values = base + r.values_at;
     w.tiles = reinterpret_cast<Tile*>(base + r.tiles_at);
     w.count = reinterpret_cast<uint32_t*>(base + r.count_at);
-    ExpandGrid g = {};
-    g.key_i = (a.n_heads * a.nope + 127) / 128;
-    g.keys = g.key_i * ((a.n_rows + 127) / 128);
-    g.value_i = static_cast<uint32_t>((w.value_rows + 127) / 128);
-    g.values = g.value_i * ((a.n_heads * r.dv + 127) / 128);
-    g.copies = 1024;
+    w.beyond = reinterpret_cast<uint32_t*>(base + r.beyond_at);
+    const ExpandGrid& g = r.grid;
     auto expand = r.wide ? expand_kernel<T, true> : expand_kernel<T, false>;
     hipLaunchKernelGGL(expand, dim3(g.keys + g.values + g.copies + 1), dim3(256), 0, stream, a, w, g);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || w.most_tiles == 0) return e;
     if constexpr (sizeof(T) == 2) {
         if (r.waves == 8) {
-            if (r.dk == 128) return r.dv == 64 ? launch_prompt<T, 128, 64, 8>(a, w, stream) : launch_prompt<T, 128, 128, 8>(a, w, stream);
-            return r.dv == 64 ? launch_prompt<T, 192, 64, 8>(a, w, stream) : launch_prompt<T, 192, 128, 8>(a, w, stream);
+            if (r.dk == 128) return r.dv == 64 ? launch_prompt<T, 128, 64, 8>(a, w, g, stream) : launch_prompt<T, 128, 128, 8>(a, w, g, stream);
+            return r.dv == 64 ? launch_prompt<T, 192, 64, 8>(a, w, g, stream) : launch_prompt<T, 192, 128, 8>(a, w, g, stream);
         }
     }
-    if (r.dk == 128) return r.dv == 64 ? launch_prompt<T, 128, 64, 4>(a, w, stream) : launch_prompt<T, 128, 128, 4>(a, w, stream);
-    if (r.dk == 192) return r.dv == 64 ? launch_prompt<T, 192, 64, 4>(a, w, stream) : launch_prompt<T, 192, 128, 4>(a, w, stream);
-    return launch_prompt<T, 256, 256, 4>(a, w, stream);
+    if (r.dk == 128) return r.dv == 64 ? launch_prompt<T, 128, 64, 4>(a, w, g, stream) : launch_prompt<T, 128, 128, 4>(a, w, g, stream);
+    if (r.dk == 192) return r.dv == 64 ? launch_prompt<T, 192, 64, 4>(a, w, g, stream) : launch_prompt<T, 192, 128, 4>(a, w, g, stream);
+    return launch_prompt<T, 256, 256, 4>(a, w, g, stream);
 }
 
 } // namespace
@@ -659,7 +744,7 @@ int svsx_latent_expanded_workspace(const svsx_expanded_desc* desc, size_t* bytes
     ExpandedArgs a;
     if (const int rc = check_expanded(desc, &a)) return rc;
     if (!bytes) return fail(SVSX_INVALID_ARGUMENT, "null argument");
-    *bytes = a.n_tokens ? route_of(a, paged_dtype_size(desc->dtype)).bytes : 0;
+    *bytes = a.n_tokens ? route_of(a, desc->dtype).bytes : 0;
     return SVSX_SUCCESS;
 }
 
@@ -667,7 +752,7 @@ int svsx_latent_expanded_device(const svsx_expanded_desc* desc, void* d_workspac
     ExpandedArgs a;
     if (const int rc = check_expanded(desc, &a)) return rc;
     if (a.n_tokens == 0) return SVSX_SUCCESS;
-    PromptRoute r = route_of(a, paged_dtype_size(desc->dtype));
+    PromptRoute r = route_of(a, desc->dtype);
     if (r.bytes > 0 && (!d_workspace || workspace_bytes < r.bytes || reinterpret_cast<uintptr_t>(d_workspace) % 16 != 0))
         return fail(SVSX_INVALID_ARGUMENT, "a workspace of %zu bytes, aligned to 16, is needed", r.bytes);
     DeviceScope on(desc->device);

@@ -568,6 +568,46 @@ def test_expanded_rows_that_are_not_finite(dtype, heads):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads, nope, rope, rank, dv, what", [
+    (3, 64, 32, 96, 64, "keys"), (3, 64, 32, 96, 64, "values"), (3, 64, 32, 96, 64, "both"), (300, 128, 64, 64, 128, "both"), (2, 100, 20, 72, 77, "both"), (2, 200, 56, 520, 192, "both"),
+])
+@pytest.mark.parametrize("causal", [True, False])
+def test_expanded_keys_and_values_beyond_float16(dtype, heads, nope, rope, rank, dv, what, causal):
+    """A projected key or value may exceed the row type's largest number (float16: 65504) where products of queries and keys, and weighted means of values, are ordinary
+    numbers: rows 140 .. 169 of one sequence have such ones, of either sign.  Queries that see none of them, and heads without them, are as ever."""
+    import torch
+
+    import scalablevectorsearch_amd as svs
+
+    g = torch.Generator().manual_seed(12)
+    t = getattr(torch, dtype)
+    qo, ro = [0, 21, 230], [0, 30, 250]
+    big, scale = (torch.arange(heads) % 3 != 1)[:, None, None], 2.0**-10
+    rows = torch.randn(250, rank + rope, generator=g)
+    rows[140:170, :rank] *= 1000.0
+    # keys and values of those rows: 300, or 60000, in the mean; scores of 2 in the mean
+    large = [torch.where(big, 60.0, 0.3) if what in (x, "both") else torch.full((heads, 1, 1), 0.3) for x in ("keys", "values")]
+    wk, wv = (torch.randn(heads, n, rank, generator=g) * x * rank**-0.5 for n, x in ((nope, large[0]), (dv, large[1])))
+    q = torch.randn(230, heads, nope + rope, generator=g) * 2 / (large[0].reshape(1, heads, 1) * 1000 * nope**0.5 * scale)
+    q, rows, wk, wv = (x.to(t).cuda() for x in (q, rows, wk, wv))
+    off = [torch.tensor(x, dtype=torch.int32).cuda() for x in (qo, ro)]
+    some = sorted({0, 1, heads - 1})
+    out, bound = _expanded(q, rows, wk, wv, qo, ro, scale, causal, some)
+    got = svs.latent_attention_expanded(q, rows, wk, wv, *off, scale=scale, causal=causal).cpu().double()
+    largest = max(float((rows[140:170, :rank].double() @ (wk if what == "keys" else wv)[h].double().T).abs().max()) for h in some)
+    assert largest > 130000
+    # a result beyond the type is infinite, as any rounding to the type makes it; those within its last step may be either
+    top = torch.finfo(t).max
+    got, out, bound = got[:, some], out[:, some], bound[:, some]
+    inside = out.abs() + bound < top
+    assert inside.float().mean() > 0.8
+    off64 = (got - out).abs() - bound
+    assert got[inside].isfinite().all() and off64[inside].max() <= 0, f"worst excess {off64[inside].max().item()}"
+    assert not got.isnan().any()
+
+
+@pytest.mark.gpu
 def test_expanded_prompts_in_a_graph():
     import torch
 
