@@ -250,7 +250,7 @@ __global__ __launch_bounds__(kPlanThreads) void copy_plan_kernel(const CacheArgs
         if (sh.claim[t] != i || sh.claim[s] != n || a.lengths[t] != 0) continue; // a target twice, a source that is a target too, a target that holds rows
         len[e] = a.lengths[s];
         const uint32_t l = static_cast<uint32_t>(len[e]);
-        if ((l + a.page_size - 1) / a.page_size > a.columns) { // no length that this cache can hold
+        if (len[e] < 0 || static_cast<uint64_t>(l) > static_cast<uint64_t>(a.columns) * a.page_size) { // no length that this cache can hold
             len[e] = -1;
             continue;
         }

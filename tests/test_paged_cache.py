@@ -321,6 +321,31 @@ def test_a_step_is_captured_and_replayed():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("length", [-1, -3, -4, -(2**31), 37, 2**31 - 1])
+def test_a_length_that_no_sequence_has_is_refused(length):
+    """lengths below zero and beyond the table (9 pages of 4 rows) in an adopted cache: the sequence neither grows nor is copied, nothing else changes, and the entries beside it are
+    served"""
+    import torch
+
+    import scalablevectorsearch_amd as svs
+
+    cache = svs.PagedCache(30, 4, 1, 2, 0, dtype=torch.float32, n_sequences=6, max_pages=9)
+    cache.extend([0, 1], torch.tensor([0, 6, 15], dtype=torch.int32).cuda(), 15)
+    cache.lengths[0] = length
+    table, refs = cache.table.tolist(), cache.refs.tolist()
+    for share in (False, True):
+        (cache.fork if share else cache.copy)([0, 1], [2, 3])
+        assert cache.failures.item() == 1 and cache.lengths.tolist() == [length, 9, 0, 9, 0, 0]
+        assert cache.table[0].tolist() == table[0] and cache.table[2].tolist() == table[2] and cache.table[4:].tolist() == table[4:]
+        assert sum(cache.refs.tolist()) == sum(refs) + 3
+        cache.free([3])
+        assert cache.refs.tolist() == refs and cache.table.tolist() == table
+        cache.failures.zero_()
+    slots = cache.extend([0, 4], torch.tensor([0, 1, 2], dtype=torch.int32).cuda(), 2).tolist()
+    assert cache.failures.item() == 1 and cache.lengths.tolist() == [length, 9, 0, 0, 1, 0] and slots[0] == -1 and slots[1] >= 0
+
+
+@pytest.mark.gpu
 def test_pages_beyond_two_to_the_31_elements():
     import torch
 
