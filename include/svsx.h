@@ -404,7 +404,8 @@ int svsx_index_build_bound_codes(svsx_index* index, int mode);
 /* ---- paged cache of rows ----------------------------------------------------------------------------------------------------------------
  * Rows that a model stores token by token (keys and values of attention; no reference counterpart), in pages that sequences take, share and give back.
  * The cache is the caller's arrays, all resident in HBM on `device`; a call reads and changes them in stream order, never waits, allocates nothing and may be captured
- * into a graph.  Calls that change one cache must be ordered among each other and with the calls that read it (one stream, or events).
+ * into a graph.  Calls that change one cache must be ordered among each other and with the calls that read it (one stream, or events).  A call may be two launches: threads that
+ * share a stream call one after another.
  *   d_keys     [n_layers][n_pages][n_heads][page_size][key_dim]    of `dtype` (SVSX_F32, SVSX_F16, SVSX_BF16)
  *   d_values   [n_layers][n_pages][n_heads][page_size][value_dim]  NULL with value_dim = 0: the rows are keys and values at once (latent rows)
  *   d_table    [n_sequences][max_pages]  row r of a sequence is row r % page_size of page table[r / page_size]; -1 behind the sequence's last page

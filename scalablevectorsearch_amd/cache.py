@@ -2,10 +2,12 @@
 pages that sequences take, share and give back.
 
 Every call is enqueued on torch's current stream of the cache's device, never waits for the GPU, and may be captured into a graph.  Calls
-that change a cache must be ordered among each other and with its readers, as one stream does."""
+that change a cache must be ordered among each other and with its readers, as one stream does; calls of one PagedCache from several threads on one
+stream are (a call is up to two launches, which follow one another)."""
 from __future__ import annotations
 
 import ctypes as C
+import threading
 
 from . import _lib
 from .attention import _dtypes, _elsewhere, _invalid, _on_device, _stream, paged_attention
@@ -69,7 +71,9 @@ class PagedCache:
         self._at = C.addressof(self._desc)
         size = C.c_size_t()
         _lib.check(_lib.lib().svsx_cache_workspace(self._at, _MOST, C.byref(size)))  # checks the description, too
-        # calls that change a cache follow one another, so one workspace serves them all
+        # calls that change a cache follow one another, so one workspace serves them all.  A call is two launches and the interpreter lets other threads run meanwhile: the lock
+        # keeps their launches from coming between
+        self._lock = threading.Lock()
         self._space, self._space_bytes = torch.empty(size.value, dtype=torch.uint8, device=keys.device), size.value
         self._space_at = self._space.data_ptr()
 
@@ -95,8 +99,9 @@ class PagedCache:
         if n_tokens < 0:
             raise _invalid("n_tokens must not be negative")
         slots = sequences.new_empty(n_tokens, dtype=self._int64)
-        rc = _lib.lib().svsx_cache_extend_device(self._at, sequences.data_ptr(), offsets.data_ptr(), n, n_tokens, slots.data_ptr(), self._space_at, self._space_bytes,
-                                                 _stream(self._index))
+        with self._lock:
+            rc = _lib.lib().svsx_cache_extend_device(self._at, sequences.data_ptr(), offsets.data_ptr(), n, n_tokens, slots.data_ptr(), self._space_at, self._space_bytes,
+                                                     _stream(self._index))
         if rc:
             _lib.check(rc)
         return slots
@@ -114,8 +119,9 @@ class PagedCache:
         n = slots.shape[0]
         ks = self._check_rows("keys", keys, n, self._rows[0])
         vs = self._check_rows("values", values, n, self._rows[1]) if values is not None else (0, 0)
-        rc = _lib.lib().svsx_cache_write_device(self._at, layer, slots.data_ptr(), n, keys.data_ptr(), ks[0], ks[1], values.data_ptr() if values is not None else 0, vs[0], vs[1],
-                                                _stream(self._index))
+        with self._lock:
+            rc = _lib.lib().svsx_cache_write_device(self._at, layer, slots.data_ptr(), n, keys.data_ptr(), ks[0], ks[1], values.data_ptr() if values is not None else 0, vs[0], vs[1],
+                                                    _stream(self._index))
         if rc:
             _lib.check(rc)
 
@@ -134,7 +140,8 @@ class PagedCache:
         n = sources.shape[0]
         if targets.shape[0] != n:
             raise _invalid(f"{n} sources and {targets.shape[0]} targets")
-        rc = _lib.lib().svsx_cache_copy_device(self._at, sources.data_ptr(), targets.data_ptr(), n, share, self._space_at, self._space_bytes, _stream(self._index))
+        with self._lock:
+            rc = _lib.lib().svsx_cache_copy_device(self._at, sources.data_ptr(), targets.data_ptr(), n, share, self._space_at, self._space_bytes, _stream(self._index))
         if rc:
             _lib.check(rc)
 
@@ -149,14 +156,16 @@ class PagedCache:
     def free(self, sequences) -> None:
         """The sequences become empty; pages nobody holds any more are free."""
         sequences = self._list(sequences, "sequences")
-        rc = _lib.lib().svsx_cache_free_device(self._at, sequences.data_ptr(), sequences.shape[0], _stream(self._index))
+        with self._lock:
+            rc = _lib.lib().svsx_cache_free_device(self._at, sequences.data_ptr(), sequences.shape[0], _stream(self._index))
         if rc:
             _lib.check(rc)
 
     def compact(self):
         """Used pages move to the front of the pool; returns each page's new place (int32 [pages], -1 for a page that was free)."""
         moved = self.refs.new_empty(self.refs.shape[0])
-        rc = _lib.lib().svsx_cache_compact_device(self._at, moved.data_ptr(), self._space_at, self._space_bytes, _stream(self._index))
+        with self._lock:
+            rc = _lib.lib().svsx_cache_compact_device(self._at, moved.data_ptr(), self._space_at, self._space_bytes, _stream(self._index))
         if rc:
             _lib.check(rc)
         return moved
@@ -165,5 +174,6 @@ class PagedCache:
         """``paged_attention`` of ``queries`` [n, heads, key_dim] over one layer; row i belongs to ``sequences[i]`` (default: sequence i)."""
         if not 0 <= layer < self.keys.shape[0]:
             raise _invalid(f"layer {layer} of a cache of {self.keys.shape[0]} layers")
-        return paged_attention(queries, self.keys[layer], self.values[layer] if self.values is not None else None, self.table, self.lengths, sequences=sequences,
-                               value_dim=value_dim, scale=scale, return_lse=return_lse)
+        with self._lock:
+            return paged_attention(queries, self.keys[layer], self.values[layer] if self.values is not None else None, self.table, self.lengths, sequences=sequences,
+                                   value_dim=value_dim, scale=scale, return_lse=return_lse)

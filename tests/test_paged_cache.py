@@ -56,6 +56,61 @@ def test_calls_check_their_arguments_before_any_device_work():
     assert L.svsx_cache_write_device(d, 0, None, 0, None, 0, 0, None, 0, 0, None) == _lib.SUCCESS
 
 
+def test_threads_call_one_after_another(monkeypatch):
+    """two calls of one cache are never in the library at once, where the launches of one could come between those of the other; two caches' may be"""
+    import threading
+    import time
+
+    import torch
+
+    from scalablevectorsearch_amd import cache as module
+
+    class Library:
+        """stands in for libsvsx.so and notes, per cache, calls that overlap"""
+
+        inside, calls, overlaps = {}, 0, 0
+
+        def svsx_cache_workspace(self, at, n, size):
+            size._obj.value = 64
+            return _lib.SUCCESS
+
+        def call(self, at, *args):
+            self.inside[at] = self.inside.get(at, 0) + 1
+            self.overlaps += self.inside[at] > 1
+            self.calls += 1
+            time.sleep(0.002)
+            self.inside[at] -= 1
+            return _lib.SUCCESS
+
+        svsx_cache_extend_device = svsx_cache_write_device = svsx_cache_copy_device = svsx_cache_free_device = svsx_cache_compact_device = call
+
+    library = Library()
+    monkeypatch.setattr(_lib, "lib", lambda: library)
+    monkeypatch.setattr(module, "_on_device", lambda *a: None)
+    monkeypatch.setattr(module, "_stream", lambda index: 0)
+    zeros = lambda *s: torch.zeros(*s, dtype=torch.int32)  # noqa: E731
+    caches = [module.PagedCache.from_device(torch.zeros(1, 4, 1, 2, 3), None, zeros(2, 2), zeros(2), zeros(4)) for _ in range(2)]
+    monkeypatch.setattr(module, "paged_attention", lambda q, keys, *a, **k: library.call(next(c._at for c in caches if c.keys.data_ptr() == keys.data_ptr())))
+    one, two, slots = zeros(1), zeros(2), torch.zeros(1, dtype=torch.int64)
+
+    def work(c):
+        for _ in range(3):
+            c.extend(one, two, 1)
+            c.write(slots, torch.zeros(1, 1, 3))
+            c.fork(one, one)
+            c.copy(one, one)
+            c.free(one)
+            c.compact()
+            c.attend(torch.zeros(1, 1, 3))
+
+    threads = [threading.Thread(target=work, args=(caches[i % 2],)) for i in range(6)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert library.calls == 6 * 21 and library.overlaps == 0
+
+
 # ---- the model ---------------------------------------------------------------------------------------------------------------------------------
 
 
@@ -318,6 +373,53 @@ def test_a_step_is_captured_and_replayed():
         assert torch.equal(moved, want)
         for name in ("keys", "values", "table", "lengths", "refs", "failures"):
             assert torch.equal(getattr(cache, name), getattr(eager, name)), (k, name)
+
+
+@pytest.mark.gpu
+def test_threads_on_one_stream():
+    """four threads fork, grow, write and free sequences of their own, a fifth compacts: in the end every sequence has its parent's rows and its own, and counts are the table's"""
+    import threading
+
+    import torch
+
+    import scalablevectorsearch_amd as svs
+
+    cache = svs.PagedCache(200, 4, 1, 2, 0, dtype=torch.float32, n_sequences=5, max_pages=9)
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32).cuda()  # noqa: E731
+    parent = torch.arange(46, dtype=torch.float32, device="cuda").reshape(23, 1, 2)
+    cache.write(cache.extend(ints(0), ints(0, 23), 23), parent)
+    lists = [(ints(0), ints(k), ints(0, 2), torch.full((2, 1, 2), 100.0 + k, device="cuda")) for k in range(1, 5)]
+    torch.cuda.synchronize()
+    errors = []
+
+    def work(zero, mine, two, rows):
+        try:
+            for _ in range(50):
+                cache.free(mine)
+                cache.fork(zero, mine)
+                cache.extend(mine, two, 2)
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    def compact():
+        for _ in range(50):
+            cache.compact()
+
+    threads = [threading.Thread(target=work, args=x) for x in lists] + [threading.Thread(target=compact)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for _, mine, two, rows in lists:  # slots hold until the next compact: written here, to two more rows
+        cache.write(cache.extend(mine, two, 2), rows)
+    assert not errors and cache.failures.item() == 0 and cache.lengths.tolist() == [23, 27, 27, 27, 27]
+    table, held = cache.table.cpu().long(), torch.zeros(200, dtype=torch.int32)
+    for s in range(5):
+        of = table[s, :-(-int(cache.lengths[s]) // 4)]
+        held[of] += 1
+        rows = cache.keys[0].cpu()[of, 0].reshape(-1, 2)
+        assert torch.equal(rows[:23], parent[:, 0].cpu()) and (s == 0 or (rows[25:27] == 100 + s).all())
+    assert torch.equal(held, cache.refs.cpu())
 
 
 @pytest.mark.gpu
