@@ -19,7 +19,7 @@ struct AttentionArgs {
     uint32_t n_queries, n_heads, group, n_key_heads, dk, dv, n_pages, page_size, n_sequences, max_pages;
     float scale;
     int shared;       // rows are keys and values at once
-    int wide_queries; // heads' queries begin at 16-byte boundaries and are whole 16-byte words
+    int wide_queries, wide_out; // heads' queries, and heads' results, begin at 16-byte boundaries and are whole 16-byte words
 };
 
 // rows of query i: its table row and how many rows there are
@@ -381,7 +381,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && VB == 1 ? 3 : 2) void attend
                 Frag<T> f;
 #pragma unroll
                 for (int d = 0; d < 8; ++d) f[d] = from_f32<T>(o[b * 8 + d][r] * inv);
-                if (a.dv % 8 == 0) {
+                if (a.wide_out) {
                     if (col < a.dv) *reinterpret_cast<Frag<T>*>(out + col) = f;
                 } else {
 #pragma unroll
@@ -840,7 +840,13 @@ template <typename T, int KS, int HT> __global__ __launch_bounds__((RowsLayout<T
                     Four f;
 #pragma unroll
                     for (int r = 0; r < 4; ++r) f[r] = from_f32<T>(o[x][d][r] * factor);
-                    *reinterpret_cast<Four*>(static_cast<T*>(a.out) + at * a.dv + col) = f;
+                    T* out = static_cast<T*>(a.out) + at * a.dv + col;
+                    if (a.wide_out) {
+                        *reinterpret_cast<Four*>(out) = f;
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) out[r] = f[r];
+                    }
                 } else {
                     *reinterpret_cast<f32x4*>(plan.partial + at * a.dv + col) = o[x][d];
                 }
@@ -970,6 +976,7 @@ int check_attention(const svsx_attention_desc* d, AttentionArgs* a) {
     a->scale = d->scale;
     a->shared = d->d_values == nullptr;
     const size_t es = paged_dtype_size(d->dtype);
+    a->wide_out = d->value_dim % 8 == 0 && (reinterpret_cast<size_t>(d->d_out) & 15) == 0;
     a->wide_queries = d->key_dim % 8 == 0 && ((reinterpret_cast<size_t>(d->d_queries) | d->query_stride * es | d->query_head_stride * es) & 15) == 0;
     return SVSX_SUCCESS;
 }

@@ -226,6 +226,32 @@ def test_strides_and_alignment(dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lengths, heads, kv, dim, value_dim, page, shared", [
+    ([100, 0, 5], 8, 2, 128, 128, 16, False), ([60, 3], 20, 1, 576, 512, 16, True), ([64, 1], 40, 1, 64, 64, 8, True), ([700, 40], 4, 2, 256, 256, 16, False), ([2000], 16, 1, 288, 256, 16, True),
+    ([30, 9], 2, 1, 512, 480, 4, False),
+])
+def test_results_that_begin_anywhere(dtype, lengths, heads, kv, dim, value_dim, page, shared):
+    """d_out of the C call need not begin at a word: the same bits at every element, nothing before them or behind"""
+    import torch
+
+    q, keys, values, table, n = _case(dtype, lengths, heads, kv, dim, value_dim, page, seed=5, shared=shared)
+    want, _ = _run(q, keys, values, table, n, value_dim=value_dim)
+    d = _lib.AttentionDesc(C.sizeof(_lib.AttentionDesc), 0, {"float32": 0, "float16": 1, "bfloat16": 4}[dtype], len(lengths), heads, kv, dim, value_dim, keys.shape[0], page, len(lengths),
+                           table.shape[1], table.stride(0), q.data_ptr(), q.stride(0), q.stride(1), keys.data_ptr(), *keys.stride()[:3], None if shared else values.data_ptr(),
+                           *(keys if shared else values).stride()[:3], table.data_ptr(), n.data_ptr(), None, dim**-0.5, None, None)
+    L, size = _lib.lib(), C.c_size_t()
+    for first in (0, 1, 2, 4, 7):
+        out = torch.full((want.numel() + 16,), 3.0, dtype=want.dtype, device="cuda")
+        d.d_out = out[first:].data_ptr()
+        _lib.check(L.svsx_paged_attention_workspace(C.byref(d), C.byref(size)))
+        ws = torch.empty(size.value, dtype=torch.uint8, device="cuda")
+        _lib.check(L.svsx_paged_attention_device(C.byref(d), ws.data_ptr(), size.value, torch.cuda.current_stream().cuda_stream))
+        assert torch.equal(out[first:first + want.numel()].view(want.shape), want), first
+        assert (out[:first] == 3).all() and (out[first + want.numel():] == 3).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_queries_name_their_sequences(dtype):
     """several queries of one sequence, sequences in any order, ones that do not exist, fewer queries than sequences; tables longer than lengths and shorter"""
     import torch
