@@ -424,19 +424,20 @@ struct WriteArgs {
     uint32_t n_tokens, n_heads, page_size, n_pages;
 };
 
-// One thread per word of a row (16 bytes where rows allow it).  16381 rows of 8 heads, keys and values, float32: 4.7 TB/s read and written, as a large copy; 128 rows: 2.8 us.
+// One thread per word of a row (16 bytes where rows allow it), several words a thread where a grid, which has fewer than 2^32 threads, would not hold them.  16381 rows of 8 heads, keys and values, float32: 4.7 TB/s read and written, as a large copy; 128 rows: 2.8 us.
 template <typename W> __global__ __launch_bounds__(256) void write_kernel(const WriteArgs a) {
     const uint32_t kind = blockIdx.y, words = a.row_words[kind], per_token = words * a.n_heads;
-    const uint64_t at = static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x;
-    if (at >= static_cast<uint64_t>(a.n_tokens) * per_token) return;
-    const uint32_t token = static_cast<uint32_t>(at / per_token), in_token = static_cast<uint32_t>(at % per_token);
-    const int64_t slot = a.slots[token];
-    if (slot < 0 || slot >= static_cast<int64_t>(a.n_pages) * a.page_size) return;
-    const uint32_t head = in_token / words, word = in_token % words;
-    const size_t page = static_cast<size_t>(slot) / a.page_size, row = static_cast<size_t>(slot) % a.page_size;
-    const W* s = reinterpret_cast<const W*>(a.src[kind] + token * a.token_bytes[kind] + head * a.head_bytes[kind]);
-    W* d = reinterpret_cast<W*>(a.dst[kind]) + ((page * a.n_heads + head) * a.page_size + row) * words;
-    d[word] = s[word];
+    const uint64_t all = static_cast<uint64_t>(a.n_tokens) * per_token;
+    for (uint64_t at = static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x; at < all; at += static_cast<uint64_t>(gridDim.x) * 256) {
+        const uint32_t token = static_cast<uint32_t>(at / per_token), in_token = static_cast<uint32_t>(at % per_token);
+        const int64_t slot = a.slots[token];
+        if (slot < 0 || slot >= static_cast<int64_t>(a.n_pages) * a.page_size) continue;
+        const uint32_t head = in_token / words, word = in_token % words;
+        const size_t page = static_cast<size_t>(slot) / a.page_size, row = static_cast<size_t>(slot) % a.page_size;
+        const W* s = reinterpret_cast<const W*>(a.src[kind] + token * a.token_bytes[kind] + head * a.head_bytes[kind]);
+        W* d = reinterpret_cast<W*>(a.dst[kind]) + ((page * a.n_heads + head) * a.page_size + row) * words;
+        d[word] = s[word];
+    }
 }
 
 int check_cache(const svsx_cache_desc* d, CacheArgs* a) {
@@ -505,6 +506,7 @@ size_t page_word(const CacheArgs& a) {
     return word_of({reinterpret_cast<size_t>(a.keys), reinterpret_cast<size_t>(a.values), a.key_row_bytes, a.value_row_bytes});
 }
 constexpr int kMoveBlocks = 2048; // eight workgroups per compute unit
+constexpr size_t kWriteBlocks = size_t(1) << 20; // 2^28 threads
 
 } // namespace
 } // namespace svsx
@@ -618,8 +620,9 @@ int svsx_cache_write_device(const svsx_cache_desc* desc, size_t layer, const int
     w.n_heads = a.n_heads;
     w.page_size = a.page_size;
     w.n_pages = a.n_pages;
-    const size_t per_token = static_cast<size_t>(std::max(w.row_words[0], w.row_words[1])) * a.n_heads, blocks = (n_tokens * per_token + 255) / 256;
-    if (per_token >= (size_t(1) << 31) || blocks >= (size_t(1) << 31)) return fail(SVSX_INVALID_ARGUMENT, "too many values in one call");
+    const size_t per_token = static_cast<size_t>(std::max(w.row_words[0], w.row_words[1])) * a.n_heads;
+    if (per_token >= (size_t(1) << 31)) return fail(SVSX_INVALID_ARGUMENT, "a row of all heads has %zu words, 2^31 - 1 at most", per_token);
+    const size_t blocks = std::min((n_tokens * per_token + 255) / 256, kWriteBlocks);
     DeviceScope on(desc->device);
     if (on.error != hipSuccess) return fail(SVSX_RUNTIME_ERROR, "hipSetDevice(%d) failed: %s", desc->device, hipGetErrorString(on.error));
     auto kernel = wide == 16 ? write_kernel<uint4> : wide == 4 ? write_kernel<uint32_t> : write_kernel<uint16_t>;

@@ -467,6 +467,27 @@ def test_pages_beyond_two_to_the_31_elements():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [(1 << 13) - 1, (1 << 16) + 3])
+def test_writing_more_words_than_a_grid_has_threads(tokens):
+    """65537 half-words a row: 2^29 of them, and more than 2^32; most slots are outside the cache, the rows that count are the first, the last and some between"""
+    import torch
+
+    import scalablevectorsearch_amd as svs
+
+    cache = svs.PagedCache(4, 2, 1, 65537, 0, dtype=torch.float16, n_sequences=2, max_pages=2)
+    row = torch.randn(1, 1, 65537, device="cuda").half()
+    rows = row.expand(tokens, 1, 65537)  # every token's row is the same memory
+    slots = torch.full((tokens,), -1, dtype=torch.int64, device="cuda")
+    for slot, token in ((0, 0), (5, tokens // 2), (6, tokens - 4), (7, tokens - 1)):
+        slots[token] = slot
+    slots[3] = 8  # outside, too
+    cache.write(slots, rows)
+    got = cache.keys[0, :, 0].reshape(8, 65537)
+    for slot in range(8):
+        assert torch.equal(got[slot], row[0, 0] if slot in (0, 5, 6, 7) else torch.zeros_like(row[0, 0])), slot
+
+
+@pytest.mark.gpu
 def test_wrong_arguments_are_refused():
     import torch
 
