@@ -2,7 +2,7 @@
 products of ``FlatIndex`` with a softmax over them in the place of the k best.
 
 Calls are enqueued on torch's current stream of the queries' device, never wait for the GPU, and may be captured into a graph.  They are for serving:
-no gradient flows through them."""
+no gradient flows through them, and where torch would record one (an input that requires it, outside torch.no_grad()) they refuse."""
 from __future__ import annotations
 
 import ctypes as C
@@ -31,6 +31,16 @@ def _elsewhere(name, x) -> _lib.SvsxError:
 def _on_device(name, x, device) -> None:
     if x.device != device or device.type != "cuda":
         raise _elsewhere(name, x)
+
+
+def _no_gradient(*arrays) -> None:
+    """A result that is cut off from its inputs' gradients, without a word, would be a wrong one."""
+    for x in arrays:
+        if x is not None and x.requires_grad:
+            import torch
+
+            if torch.is_grad_enabled():
+                raise _invalid("no gradient flows through this call: use torch.no_grad(), or detach the inputs")
 
 
 def _stream(index: int) -> int:
@@ -118,6 +128,7 @@ def paged_attention(queries, keys, values, table, lengths, sequences=None, value
             _on_device(name, x, queries.device)
     if value_dim < 0:
         raise _invalid("value_dim must be positive")
+    _no_gradient(queries, keys, values)
     out = queries.new_empty((n, heads, value_dim))
     lse = queries.new_empty((n, heads), dtype=torch.float32) if return_lse else None
     try:
@@ -182,6 +193,7 @@ def latent_attention_expanded(queries, rows, w_key, w_value, query_offsets, row_
         _on_device(name, x, device)
     for name, x in (("queries", queries), ("rows", rows), ("w_key", w_key), ("w_value", w_value)):
         _on_device(name, x, device)
+    _no_gradient(queries, rows, w_key, w_value, out)
     w_key, w_value = w_key.contiguous(), w_value.contiguous()
     keep = out is not None
     if keep:

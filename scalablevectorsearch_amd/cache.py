@@ -10,7 +10,7 @@ import ctypes as C
 import threading
 
 from . import _lib
-from .attention import _dtypes, _elsewhere, _invalid, _on_device, _stream, paged_attention
+from .attention import _dtypes, _elsewhere, _invalid, _no_gradient, _on_device, _stream, paged_attention
 
 _MOST = 4096  # entries of one call (include/svsx.h)
 
@@ -107,7 +107,8 @@ class PagedCache:
         return slots
 
     def write(self, slots, keys, values=None, layer: int = 0) -> None:
-        """Rows ``keys`` [tokens, heads, key_dim] (and ``values``) of one layer to their slots.  Slots of one call differ; those outside the cache (-1) are skipped."""
+        """Rows ``keys`` [tokens, heads, key_dim] (and ``values``) of one layer to their slots.  Slots of one call differ; those outside the cache (-1) are skipped.
+        No gradient flows into the cache: rows that require one are refused outside torch.no_grad()."""
         if slots.dtype != self._int64 or slots.dim() != 1 or not slots.is_contiguous():
             raise _invalid("slots must be a contiguous vector of int64")
         if slots.get_device() != self._index:
@@ -119,6 +120,7 @@ class PagedCache:
         n = slots.shape[0]
         ks = self._check_rows("keys", keys, n, self._rows[0])
         vs = self._check_rows("values", values, n, self._rows[1]) if values is not None else (0, 0)
+        _no_gradient(keys, values)
         with self._lock:
             rc = _lib.lib().svsx_cache_write_device(self._at, layer, slots.data_ptr(), n, keys.data_ptr(), ks[0], ks[1], values.data_ptr() if values is not None else 0, vs[0], vs[1],
                                                     _stream(self._index))

@@ -722,6 +722,36 @@ def test_arrays_on_the_host_are_refused():
 
 
 @pytest.mark.gpu
+def test_inputs_that_require_a_gradient_are_refused():
+    """each input of each call; under no_grad, and detached, the call runs as ever"""
+    import torch
+
+    import scalablevectorsearch_amd as svs
+
+    q, keys, values, table, n = _case("float32", [20, 3], 4, 2, 16, 16, 4)
+    off = torch.tensor([0, 2], dtype=torch.int32).cuda()
+    qe, rows, wk, wv, out = (torch.randn(*s, device="cuda") for s in ((2, 4, 20), (2, 28), (4, 12, 20), (4, 8, 20), (2, 4, 8)))
+    cache = svs.PagedCache(4, 2, 1, 8, dtype=torch.float32, n_sequences=2)
+    slots, k, v = torch.zeros(1, dtype=torch.int64, device="cuda"), torch.randn(1, 1, 8, device="cuda"), torch.randn(1, 1, 8, device="cuda")
+    qc, of = torch.randn(1, 1, 8, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    calls = [
+        ((q, keys, values), lambda a, b, c: svs.paged_attention(a, b, c, table, n)), ((q, keys), lambda a, b: svs.paged_attention(a, b, None, table, n, value_dim=8)),
+        ((qe, rows, wk, wv, out), lambda a, b, c, d, e: svs.latent_attention_expanded(a, b, c, d, off, off, out=e)), ((qc,), lambda a: cache.attend(a, of)),
+        ((k, v), lambda a, b: cache.write(slots, a, b)),
+    ]
+    for c, (arrays, call) in enumerate(calls):
+        want = call(*arrays)
+        for i in range(len(arrays)):
+            grads = [x.clone().requires_grad_(j == i) for j, x in enumerate(arrays)]
+            with pytest.raises(svs.SvsxError) as e:
+                call(*grads)
+            assert e.value.code == _lib.INVALID_ARGUMENT and "gradient" in e.value.message, (c, i)
+            with torch.no_grad():
+                got = call(*grads)
+            assert want is None or torch.equal(got, want), (c, i)
+
+
+@pytest.mark.gpu
 def test_wrong_arguments_are_refused():
     import torch
 
