@@ -422,6 +422,70 @@ def test_as_many_queries_as_a_call_takes(heads, kv, dim, value_dim, page, shared
     _check(out, lse, [x[which.cpu()] for x in want])
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", ["mixed", "late", "early", "last"])
+@pytest.mark.parametrize("dtype, n, heads, kv, dim, value_dim, page, shared", [
+    ("float16", 300, 4, 2, 64, 64, 16, False), ("bfloat16", 300, 16, 8, 64, 64, 8, False), ("float32", 700, 4, 2, 64, 40, 5, False), ("bfloat16", 1100, 2, 1, 96, 96, 16, False),
+    ("float16", 260, 6, 2, 200, 200, 32, False), ("bfloat16", 300, 16, 1, 576, 512, 16, True), ("float16", 600, 33, 1, 544, 512, 8, True), ("float32", 900, 16, 1, 288, 256, 16, True),
+])
+def test_rows_of_more_queries_than_a_workgroup_has_threads(dtype, n, heads, kv, dim, value_dim, page, shared, which):
+    """The split of all rows over the workgroups is derived from the lengths, a workgroup's threads' worth of them at a time: empty queries at the seams, blocks of empty ones before
+    the first that has rows, behind the last, and one query with nearly all"""
+    import torch
+
+    g = torch.Generator().manual_seed(n)
+    lengths = torch.randint(0, 200, (n,), generator=g)
+    lengths[torch.tensor([0, 255, 256, 511, 512, 767, 768, 1023, 1024, n - 1]).clamp(max=n - 1)] = 0
+    lengths[n // 2] = 400  # more than any unit
+    if which == "late":
+        lengths[:n - 3] = 0
+        lengths[n - 3:] = torch.tensor([1, 333, 130])
+    elif which == "early":
+        lengths[3:] = 0
+        lengths[:3] = torch.tensor([129, 0, 400])
+    elif which == "last":
+        lengths[:] = torch.arange(n) % 97 == 5
+        lengths[n - 1] = 7000
+    q, keys, values, table, n_rows = _case(dtype, lengths.tolist(), heads, kv, dim, value_dim, page, seed=n, shared=shared)
+    d = _lib.AttentionDesc(C.sizeof(_lib.AttentionDesc), 0, {"float32": 0, "float16": 1, "bfloat16": 4}[dtype], n, heads, kv, dim, value_dim, keys.shape[0], page, n, table.shape[1], table.stride(0),
+                           q.data_ptr(), q.stride(0), q.stride(1), keys.data_ptr(), *keys.stride()[:3], None if shared else values.data_ptr(), *(keys if shared else values).stride()[:3],
+                           table.data_ptr(), n_rows.data_ptr(), None, 1.0, 256, None)
+    size = C.c_size_t()
+    _lib.check(_lib.lib().svsx_paged_attention_workspace(C.byref(d), C.byref(size)))
+    assert size.value > 0  # the rows are split
+    _run(q, keys, values, table, n_rows, value_dim=value_dim)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim, value_dim", [(128, 128), (576, 512), (100, 20)])
+def test_the_one_row_that_is_not_as_low_as_the_type_allows(dtype, dim, value_dim):
+    """39 rows whose products are the type's lowest value over four (float32: -1e30, which no sum overflows), and one ordinary row, the last, the first or in the middle: the result is that
+    row's value, rounded, and the logarithm of the sum its score"""
+    import torch
+
+    import scalablevectorsearch_amd as svs
+
+    q, keys, values, table, lengths = _case(dtype, [40, 40, 40], 4, 1, dim, value_dim, 8, seed=4, shared=dim == 576)
+    column, alone = dim - 1, (39, 0, 17)  # the column is no value of the latent rows
+    q[:, :, column] = 1.0
+    for i, mine in enumerate(alone):
+        for r in range(40):
+            if r != mine:
+                keys[table[i, r // 8], 0, r % 8, column] = torch.finfo(keys.dtype).min / 4 if dtype != "float32" else -1e30
+    out, lse = svs.paged_attention(q, keys, values, table, lengths, value_dim=value_dim, return_lse=True)
+    u, e = torch.finfo(q.dtype).eps / 2, 2.0**-24
+    for i, mine in enumerate(alone):
+        page, at = int(table[i, mine // 8]), mine % 8
+        value = (values if values is not None else keys)[page, 0, at, :value_dim].double()
+        k = keys[page, 0, at].double()
+        score, size = (q[i].double() @ k) * dim**-0.5, (q[i].double().abs() @ k.abs()) * dim**-0.5
+        # its weight, 1, is exact, and the others' are zero: what is left is the score's own rounding in the weight (exp of it less the maximum: 1 but for that), and the result's
+        d = (32 + dim / 32) * e * (size + score.abs())
+        assert ((out[i].double() - value).abs() <= (u + 2 * d[:, None] + 64 * e) * value.abs()).all(), i
+        assert ((lse[i].double() - score).abs() <= d + 64 * e + 2 * e * score.abs()).all(), i
+
+
 # ---- the expanded form -----------------------------------------------------------------------------------------------------------------------------
 
 
