@@ -60,6 +60,20 @@ float half_bits_to_float(uint16_t h) {
 }
 
 
+// n rows of row_bytes, `step` bytes apart, side by side; one workgroup a row
+__global__ __launch_bounds__(256) void sample_rows_kernel(const unsigned char* src, size_t step, size_t row_bytes, unsigned char* dst) {
+    for (size_t i = threadIdx.x; i < row_bytes; i += 256) dst[blockIdx.x * row_bytes + i] = src[blockIdx.x * step + i];
+}
+
+// Every step-th row of the index, n of them, packed: on the device, and (host != NULL) on the host.  A kernel and a plain copy: hipMemcpy2D reports success and copies nothing in a process that
+// rocprofv3 (1.1.0, ROCm 7.2.0) traces beside another HIP runtime, and records of a sample of zeros reject nothing.
+hipError_t sample_rows(const svsx_index* ix, size_t step, size_t n, void* device, void* host) {
+    const size_t row = ix->d * dtype_size(ix->data_dtype);
+    hipLaunchKernelGGL(sample_rows_kernel, dim3(static_cast<uint32_t>(n)), dim3(256), 0, nullptr, static_cast<const unsigned char*>(ix->d_data), step * ix->row_bytes, row, static_cast<unsigned char*>(device));
+    const hipError_t e = hipGetLastError();
+    return e != hipSuccess || !host ? e : hipMemcpy(host, device, n * row, hipMemcpyDeviceToHost);
+}
+
 // modified Gram-Schmidt on the m columns of V (d x m, column j at V[i * m + j]); twice for orthogonality to rounding
 void orthonormalize_columns(std::vector<double>& V, uint32_t d, uint32_t m) {
     for (int rep = 0; rep < 2; ++rep)
@@ -99,7 +113,11 @@ int build_fat_rows(svsx_index* ix, uint32_t forced_rb, uint32_t* asked_rb, uint3
     const size_t ns = n < want ? n : want;
     const size_t step = n / ns;
     std::vector<unsigned char> raw(ns * d * es);
-    HIP_TRY(hipMemcpy2D(raw.data(), d * es, ix->d_data, step * ix->row_bytes, d * es, ns, hipMemcpyDeviceToHost));
+    {
+        DeviceBuffer packed;
+        HIP_TRY(packed.alloc(raw.size()));
+        HIP_TRY(sample_rows(ix, step, ns, packed.p, raw.data()));
+    }
     std::vector<double> xs(ns * d);
     for (size_t i = 0; i < ns * d; ++i) {
         float f;
@@ -413,11 +431,11 @@ int records_pay_on_a_sample(svsx_index* ix) {
     DeviceBuffer dq, di, dd;
     if (dq.alloc(nq * d * qes) != hipSuccess || di.alloc(nq * k * 8) != hipSuccess || dd.alloc(nq * k * 4) != hipSuccess) { (void)hipGetLastError(); return 1; }
     if (!ix->sq_enabled) {
-        if (hipMemcpy2D(dq.p, d * es, ix->d_data, step * ix->row_bytes, d * es, nq, hipMemcpyDeviceToDevice) != hipSuccess) return 1;
+        if (sample_rows(ix, step, nq, dq.p, nullptr) != hipSuccess) return 1;
     } else { // the queries of a scalar-quantized index are float vectors: the rows' decompressed values (scalar.h:44-46)
         std::vector<unsigned char> raw(nq * d);
         std::vector<float> qf(nq * d);
-        if (hipMemcpy2D(raw.data(), d, ix->d_data, step * ix->row_bytes, d, nq, hipMemcpyDeviceToHost) != hipSuccess) return 1;
+        if (sample_rows(ix, step, nq, dq.p, raw.data()) != hipSuccess) return 1;
         for (size_t i = 0; i < nq * d; ++i) {
             const float c = ix->data_dtype == DT_I8 ? static_cast<float>(static_cast<int8_t>(raw[i])) : static_cast<float>(raw[i]);
             qf[i] = ix->sq_scale * c + ix->sq_bias;
