@@ -3,7 +3,7 @@
 #   config 2 at both operating points, config 3, the config-4 shape (2 M x 768, the bench's graph parameters, the bench's window), the 12.5 M shard;
 #   "c4full" = BASELINE config 4's own size (10 M x 768: ~6 min for the first build alone).
 # Summaries afterwards, locally:  for t in <prefix>_c2_w128 ...; do python tools/summarize_pmc.py $t; done   (-> profiles/<tag>_pmc.json)
-set -u
+set -eu
 P=$1; shift
 T=${*:-"c2 c2m c3 c4 c5"}
 for t in $T; do
