@@ -161,10 +161,8 @@ template <int E> __device__ __forceinline__ float reduce_slots(float (&v)[E]) {
 
 // float32 rows of a static dimension that is a multiple of 16, slot-cyclic mapping, written on explicit register PAIRS (round 5).  The same
 // operations in the same order as float_row_distance below -- lane-slot e of block i goes through acc_step into s[i & 3][e], then
-// (s0 + s1) + (s2 + s3), the remaining 16-blocks into s0, reduce_slots -- but two adjacent lane-slots share one v_pk_add_f32 / v_pk_fma_f32
-// (each half is the same IEEE operation), and a pair is two CONSECUTIVE registers of the 16-byte row load and of the 16-byte query read.
-// Left to itself the SLP vectorizer paired lane-slot e of block i with lane-slot e of block i + 2 and spent 26 v_mov per 16-row pass
-// gathering the operands (87 vector instructions per pass at d = 96; 49 in this form).
+// (s0 + s1) + (s2 + s3), the remaining 16-blocks into s0, reduce_slots -- but two adjacent lane-slots go together, a pair being two CONSECUTIVE
+// registers of the 16-byte row load and of the 16-byte query read (each half is the same IEEE operation; packed instructions are off, so it is two).
 typedef float f2_t __attribute__((ext_vector_type(2)));
 
 template <int METRIC> __device__ __forceinline__ void acc_step2(f2_t& s, f2_t& n, f2_t q, f2_t x) {

@@ -6,7 +6,7 @@ NAME=$1; shift
 R=$(cd "$(dirname "$0")/.." && pwd)
 OUT=$R/variants/$NAME
 mkdir -p $OUT
-FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -fhip-fp32-correctly-rounded-divide-sqrt -fno-fast-math -Wno-unused-function"
+FLAGS=$(make -s -C $R/scalablevectorsearch_amd/csrc flags) # those of the tree
 cd $R/scalablevectorsearch_amd/csrc
 /opt/rocm/bin/hipcc $FLAGS "$@" -c svsx_flat.hip -o $OUT/svsx_flat.o
 OTHERS=$(ls *.o | grep -v -E '^svsx_flat\.o$')

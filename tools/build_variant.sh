@@ -6,7 +6,7 @@ NAME=$1; shift
 R=$(cd "$(dirname "$0")/.." && pwd)
 OUT=$R/variants/$NAME
 mkdir -p $OUT
-FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -fhip-fp32-correctly-rounded-divide-sqrt -fno-fast-math -Wno-unused-function"
+FLAGS=$(make -s -C $R/scalablevectorsearch_amd/csrc flags) # those of the tree
 cd $R/scalablevectorsearch_amd/csrc
 for f in svsx_search_f32 svsx_search_f16 svsx_search_i8 svsx_search_u8; do /opt/rocm/bin/hipcc $FLAGS "$@" -c $f.hip -o $OUT/$f.o & done
 /opt/rocm/bin/hipcc $FLAGS "$@" -c svsx_api.hip -o $OUT/svsx_api.o &
