@@ -41,6 +41,18 @@ def test_objects_follow_what_they_are_made_from(changed):
             assert any(f"-c {f} " in c for c in commands), f
 
 
+def test_a_changed_makefile_makes_the_library_stale(monkeypatch):
+    from scalablevectorsearch_amd import _lib
+
+    _lib.build()
+    calls = []
+    monkeypatch.setattr(_lib.subprocess, "check_call", lambda c: calls.append(c))
+    real = os.path.getmtime
+    monkeypatch.setattr(_lib.os.path, "getmtime", lambda p: real(p) + (1e9 if os.path.basename(p) == "Makefile" else 0))
+    _lib.build()
+    assert len(calls) == 1
+
+
 def test_variants_are_built_with_the_flags_of_the_tree():
     tools = os.path.join(ROOT, "tools")
     for f in os.listdir(tools):
