@@ -363,6 +363,7 @@ def sharded_c5_point(args, svs, q, k, R, d, rank, world, local_rank, device, reu
             if mode5:
                 index.build_bound_codes(mode5)
             sh = dict(x=x, graph=graph, entry=entry, d_entry=d_entry, index=index, sid=sid, n=n5)
+            log(f"[bench] shard {sid} of {total}: {n5} vectors, graph and records after {time.time() - t0:.0f} s")
         keep.append(sh)
         indexes.append(sh["index"])
     torch.cuda.synchronize()
@@ -588,25 +589,25 @@ def regression_uint8_point(args, svs, device, local_rank, k):
     return point
 
 
+def config4_vectors(asked, left, free_hbm):
+    """(vectors, None) where the config-4 point's graph can be built in `left` seconds (40 us a vector, and 60 s for the rest) and `free_hbm` bytes, else (2 000 000, why not)"""
+    need = asked * (768 + 129 * 4 + 128 * 132 + 2 * 768 + 8) * 1.08  # codes, graph, 128-byte inline records, float16 shadow, row norms
+    if asked > 2_000_000 and (need > free_hbm or left < 60 + 40e-6 * asked * 1.3):
+        return 2_000_000, f"{asked} vectors need {need / 1e9:.0f} GB and ~{40e-6 * asked:.0f} s; {free_hbm / 1e9:.0f} GB free and {left:.0f} s left"
+    return asked, None
+
+
 def config4_point(args, svs, device, local_rank, k, t_run0):
     """BASELINE config 4 inside the default line: synthetic N x 768 scalar-quantized int8 rows (SQDataset-style global scale / bias, scalar.h:454-462),
     float32 queries, cosine, batch 4 096, the reference's regression graph parameters (R = 128, L = 200, prune_to 124, alpha 0.95).  N = --c4-n
-    (10 M) when the GPU has the memory and the run the time (build ~340 s), else 2 M -- the size is in the point.  Smallest window with
+    (10 M) when the GPU has the memory and the run the time (build ~340 s: --budget-s 1500), else 2 M -- the size is in the point.  Smallest window with
     recall@10 >= 0.9 by binary search, timed like the headline; ids of a query sample checked against the CPU oracle."""
     import torch
 
     from scalablevectorsearch_amd.build import VamanaBuildParameters, build_vamana_device, device_graph_to_svs
 
     d4, nq4, R4 = 768, 4096, 128
-    total_hbm = torch.cuda.get_device_properties(device).total_memory
-    free_hbm = torch.cuda.mem_get_info(device)[0]
-    n4 = args.c4_n
-    left = args.budget_s - (time.time() - t_run0)
-    need = lambda n_: n_ * (d4 + 129 * 4 + 128 * 132 + 2 * d4 + 8) * 1.08  # codes, graph, 128-byte inline records, float16 shadow, row norms
-    why = None
-    if n4 > 2_000_000 and (need(n4) > free_hbm or left < 60 + 40e-6 * n4 * 1.3):
-        why = f"{n4} vectors need {need(n4) / 1e9:.0f} GB and ~{40e-6 * n4:.0f} s; {free_hbm / 1e9:.0f} GB free and {left:.0f} s left"
-        n4 = 2_000_000
+    n4, why = config4_vectors(args.c4_n, args.budget_s - (time.time() - t_run0), torch.cuda.mem_get_info(device)[0])
     t0 = time.time()
     fn = svs.DistanceCosineSimilarity()
     mn, mx = None, None
@@ -777,9 +778,7 @@ def config4b_point(args, svs, device, local_rank, k, x4, g4, e4, q4f, sq, n4):
     return out
 
 
-def main():
-    t_run0 = time.time()
-    _claim_stdout()
+def arguments():
     ap = argparse.ArgumentParser()
     ap.add_argument("--gpus", type=int, default=1)
     ap.add_argument("--steps", type=int, default=50)
@@ -800,9 +799,15 @@ def main():
     ap.add_argument("--c5-n", type=int, default=0, help="vectors per shard of the sharded_search point (0 = BASELINE config 5's 12 500 000 at every N; -1 = skip the point)")
     ap.add_argument("--sharded-timeout", type=float, default=0.0, help="watchdog of the sharded_search point in seconds (0 = scaled with shards per GPU x shard size); when it fires the line is printed with sharded_search.failed and the run exits 3")
     ap.add_argument("--c4-n", type=int, default=10_000_000, help="vectors of the config-4 point (10 M = BASELINE config 4; falls back to 2 M when time or memory is short; 0 = skip)")
-    ap.add_argument("--budget-s", type=float, default=1500.0, help="wall-clock budget of the whole run: the long extras (config 4 at 10 M) are sized against what is left")
+    ap.add_argument("--budget-s", type=float, default=540.0, help="wall-clock budget of the whole run: the long extras are sized against what is left (config 4 at 10 M needs --budget-s 1500)")
     ap.add_argument("--no-extras", action="store_true", help="skip the informational points (sharded_c5, other configs, 4x batch)")
-    args = ap.parse_args()
+    return ap
+
+
+def main():
+    t_run0 = time.time()
+    _claim_stdout()
+    args = arguments().parse_args()
 
     import torch
     import torch.distributed as dist
@@ -1181,7 +1186,7 @@ def main():
 
         n5_plan, per_plan = sharded_shard_size(args, world, total_hbm), max(1, 8 // world)
         # builds dominate: ~29 s per 12.5 M-vector shard + generation, records / code rows, exact ground truth; comm set-up and the searches on top
-        dog_s = args.sharded_timeout or (240.0 + 75.0 * per_plan * n5_plan / 12_500_000)
+        dog_s = args.sharded_timeout or min(240.0 + 75.0 * per_plan * n5_plan / 12_500_000, max(120.0, args.budget_s - (time.time() - t_run0)))
 
         def give_up():
             if rank == 0:
