@@ -84,7 +84,7 @@ struct Space { // the first launch's results
     void* values;    // [head][DV][value_rows]
     Tile* tiles;
     uint32_t* count;  // of tiles
-    uint32_t* beyond; // float16: per workgroup that multiplies (keys, then values), whether a finite result of its 128 x 128 is infinite in the row type
+    uint4* beyond;    // float16: per workgroup that multiplies (keys, then values) and wave of it, whether a finite result of its 128 x 128 is infinite in the row type
     size_t key_rows, value_rows; // at least n_rows + 64: a tile of rows may begin at the last one
     uint32_t dk, dv, most_tiles, tile_queries;
 };
@@ -144,7 +144,7 @@ template <typename T> __device__ __forceinline__ uint32_t not_finite(const Frag<
 template <typename T> inline constexpr bool kNarrow = std::is_same<T, _Float16>::value;
 
 // C[i][j] = sum_k A[i][k] B[j][k] for one 128 x 128 tile; four waves of 64 x 64.  row_a(i) / row_b(j): the row, NULL = zeros.  put(i, j, v): eight consecutive i of one j.
-// Returns, to every thread, whether a finite sum of the tile is infinite in a row type of less range (false for the other types, without asking).
+// Returns whether a finite sum of the wave's part is infinite in a row type of less range (false for the other types, without asking).
 // The next 128 bytes of every row are on their way to registers while these are multiplied.  8190 rows of rank 512 for 32 heads (68.7 GFLOP): 106 us, half of what a library product reaches; LDS is busy one and a
 // half times as long as the matrix units.  Two buffers and one barrier a step were measured in place of one buffer: 333 tokens 25.4 -> 27.3 us, as fewer workgroups fit a compute unit.
 template <typename T, bool Wide, typename A, typename B, typename P> __device__ __forceinline__ bool product_tile(unsigned char* lds, uint32_t depth, A row_a, B row_b, P put) {
@@ -204,7 +204,7 @@ template <typename T, bool Wide, typename A, typename B, typename P> __device__ 
                     for (int e = 0; e < 8; ++e) beyond |= fabsf(c[i][j][8 * k + e]) >= 65520.0f && fabsf(c[i][j][8 * k + e]) < INFINITY;
                 put((wave & 1) * 64 + i * 32 + 16 * k + 8 * half, (wave >> 1) * 64 + j * 32 + r, v);
             }
-    return kNarrow<T> && __syncthreads_or(beyond);
+    return kNarrow<T> && __any(beyond);
 }
 
 // the queries of sequence i, inside the array
@@ -272,7 +272,7 @@ template <typename T, bool Wide> __global__ __launch_bounds__(256) void expand_k
                     }
                 }
             });
-        if (kNarrow<T> && threadIdx.x == 0) w.beyond[blockIdx.x] = beyond;
+        if (kNarrow<T> && (threadIdx.x & 63) == 0) reinterpret_cast<uint32_t*>(w.beyond + blockIdx.x)[threadIdx.x >> 6] = beyond;
         return;
     }
     block -= grid.keys;
@@ -288,7 +288,7 @@ template <typename T, bool Wide> __global__ __launch_bounds__(256) void expand_k
             [&](uint32_t i, uint32_t j, const Frag<T>& v) {
                 if (i0 + i < w.value_rows && j0 + j < n) *reinterpret_cast<Frag<T>*>(values + static_cast<size_t>(j0 + j) * w.value_rows + i0 + i) = v;
             });
-        if (kNarrow<T> && threadIdx.x == 0) w.beyond[blockIdx.x] = beyond;
+        if (kNarrow<T> && (threadIdx.x & 63) == 0) reinterpret_cast<uint32_t*>(w.beyond + blockIdx.x)[threadIdx.x >> 6] = beyond;
         return;
     }
     block -= grid.values;
@@ -371,20 +371,24 @@ template <typename T, int DK, int DV> __device__ void slow_query(const ExpandedA
         if (lane + 64 * i < a.dv) out[lane + 64 * i] = from_f32<T>(o[i] * inv);
 }
 
-// Whether an expanded key or value of head h, in rows begin .. last, is infinite only for the row type's range (with what shares its workgroup in the first launch).  For
-// all threads of the workgroup.  Asking takes 333 tokens of 16 heads from 23.2 to 24.4 us; 4095 on 8190 rows, 32 heads, are as they were.
+// Whether an expanded key or value of head h, in rows begin .. last, is infinite only for the row type's range (with what shares its workgroup in the first launch).  Every
+// wave asks for itself, and gets the same answer.  Asking, beside the first rows' loads, takes 333 tokens of 16 heads from 26.4 to 27.5 us; 4095 on 8190 rows, 32 heads, are as they were.
 __device__ __forceinline__ bool any_beyond(const ExpandedArgs& a, const Space& w, const ExpandGrid& grid, uint32_t h, int32_t begin, int32_t last) {
     bool beyond = false;
     if (begin <= last) {
         const uint32_t r0 = static_cast<uint32_t>(begin) / 128, rows = static_cast<uint32_t>(last) / 128 - r0 + 1;
         const uint32_t k0 = h * a.nope / 128, ks = a.nope ? ((h + 1) * a.nope - 1) / 128 - k0 + 1 : 0; // workgroups across the head's columns
         const uint32_t v0 = h * w.dv / 128, vs = ((h + 1) * w.dv - 1) / 128 - v0 + 1;
-        for (uint32_t r = threadIdx.x; r < rows; r += blockDim.x) {
-            for (uint32_t k = 0; k < ks; ++k) beyond |= w.beyond[(r0 + r) * grid.key_i + k0 + k] != 0;
-            for (uint32_t v = 0; v < vs; ++v) beyond |= w.beyond[grid.keys + (v0 + v) * grid.value_i + r0 + r] != 0;
+        auto at = [&](uint32_t block) {
+            const uint4 x = w.beyond[block];
+            beyond |= (x.x | x.y | x.z | x.w) != 0;
+        };
+        for (uint32_t r = threadIdx.x & 63; r < rows; r += 64) {
+            for (uint32_t k = 0; k < ks; ++k) at((r0 + r) * grid.key_i + k0 + k);
+            for (uint32_t v = 0; v < vs; ++v) at(grid.keys + (v0 + v) * grid.value_i + r0 + r);
         }
     }
-    return __syncthreads_or(beyond);
+    return __any(beyond);
 }
 
 // One query by one wave in the latent space, where nothing is rounded on the way: w_key applied to the query, rows [begin, last], w_value to the result.  Lanes across the
@@ -464,12 +468,6 @@ template <typename T, int DK, int DV, int NW> __global__ __launch_bounds__(NW * 
             }
         }
     }
-    if constexpr (kNarrow<T>) {
-        if (any_beyond(a, w, grid, h, begin, group_last)) {
-            for (uint32_t t = q0 + wave * 32; t <= min(q_last, q0 + wave * 32 + 31); ++t) latent_query<T>(a, t, h, begin, sees(t), reinterpret_cast<float*>(lds) + wave * (2 * kMaxDim));
-            return;
-        }
-    }
     // the compiler is to wait for the queries here: in the loop, where it cannot tell them from the rows on their way, it would wait for both
 #pragma unroll
     for (int s = 0; s < DK / 16; ++s) asm volatile("" : "+v"(q[s]));
@@ -533,6 +531,14 @@ template <typename T, int DK, int DV, int NW> __global__ __launch_bounds__(NW * 
             bring_keys(0, base0);
             if (L::kAhead > 1 && base0 + step <= group_last) bring_keys(1, base0 + step);
             bring_values(0, base0);
+        }
+        if constexpr (kNarrow<T>) { // asked while the first rows are on their way
+            if (any_beyond(a, w, grid, h, begin, group_last)) {
+                direct_wait();
+                __syncthreads();
+                for (uint32_t t = q0 + wave * 32; t <= min(q_last, q0 + wave * 32 + 31); ++t) latent_query<T>(a, t, h, begin, sees(t), reinterpret_cast<float*>(lds) + wave * (2 * kMaxDim));
+                return;
+            }
         }
         direct_wait();
         lds_barrier();
@@ -688,14 +694,14 @@ PromptRoute route_of(const ExpandedArgs& a, int dtype) {
     r.values_at = a.n_heads * w.key_rows * r.dk * es;
     r.tiles_at = r.values_at + a.n_heads * w.value_rows * r.dv * es;
     r.count_at = r.tiles_at + static_cast<size_t>(w.most_tiles) * sizeof(Tile);
-    r.beyond_at = r.count_at + 4;
+    r.beyond_at = r.count_at + 16;
     ExpandGrid& g = r.grid;
     g.key_i = (a.n_heads * a.nope + 127) / 128;
     g.keys = g.key_i * ((a.n_rows + 127) / 128);
     g.value_i = static_cast<uint32_t>((w.value_rows + 127) / 128);
     g.values = g.value_i * ((a.n_heads * r.dv + 127) / 128);
     g.copies = 1024;
-    r.bytes = r.beyond_at + (dtype == SVSX_F16 ? 4 * (static_cast<size_t>(g.keys) + g.values) : 0);
+    r.bytes = r.beyond_at + (dtype == SVSX_F16 ? sizeof(uint4) * (static_cast<size_t>(g.keys) + g.values) : 0);
     return r;
 }
 
@@ -718,7 +724,7 @@ template <typename T> hipError_t launch_expanded(const ExpandedArgs& a, PromptRo
     w.values = base + r.values_at;
     w.tiles = reinterpret_cast<Tile*>(base + r.tiles_at);
     w.count = reinterpret_cast<uint32_t*>(base + r.count_at);
-    w.beyond = reinterpret_cast<uint32_t*>(base + r.beyond_at);
+    w.beyond = reinterpret_cast<uint4*>(base + r.beyond_at);
     const ExpandGrid& g = r.grid;
     auto expand = r.wide ? expand_kernel<T, true> : expand_kernel<T, false>;
     hipLaunchKernelGGL(expand, dim3(g.keys + g.values + g.copies + 1), dim3(256), 0, stream, a, w, g);
