@@ -458,7 +458,8 @@ int svsx_cache_compact_device(const svsx_cache_desc* desc, int32_t* d_moved, voi
 
 /* ---- attention over rows in HBM ---------------------------------------------------------------------------------------------------------------
  * out[i][h] = sum_r p_r v_r / sum_r p_r with p_r = exp(scale * <q[i][h], k_r>): one new token's attention (no reference counterpart; svsx_flat_search's
- * exhaustive inner products with a softmax in the place of the k best).  Sums and the softmax are kept in float32.
+ * exhaustive inner products with a softmax in the place of the k best).  Scores, maxima and sums are kept in float32; for the 16-bit types the weights p_r are rounded to dtype before
+ * they meet the values where the matrix units multiply them (half a step of the type each), so that a result is about 1.4 times as far from the exact one as its own rounding alone would leave it.
  *   rows      query i attends to rows 0 .. d_lengths[s] - 1 of sequence s = d_sequences[i] (NULL: s = i); row r is row r % page_size of page
  *             d_table[s * table_stride + r / page_size], at most max_pages of them.  An entry outside [0, n_pages) is a hole: its rows are left out (page_size 1: the
  *             table may be the ids32 of svsx_search_device over the same rows).  A sequence outside [0, n_sequences) has no rows.

@@ -71,7 +71,8 @@ def paged_attention(queries, keys, values, table, lengths, sequences=None, value
     ``table`` may be the int32 ids of a search over these rows, missing neighbours included.
 
     Returns softmax(scale * queries . keys) . values [n, heads, value_dim] (scale: default dim ** -0.5) and with ``return_lse`` the
-    logarithm of each softmax's denominator [n, heads] float32, which joins results over parts of the rows.  A query with no rows gives zeros and -inf."""
+    logarithm of each softmax's denominator [n, heads] float32, which joins results over parts of the rows.  A query with no rows gives zeros and -inf.
+    Sums are float32; 16-bit rows round the softmax's weights to their type before these meet the values (float32 rows: 32 bits throughout)."""
     import torch
 
     if queries.dim() != 3 or keys.dim() != 4:
@@ -165,7 +166,9 @@ def latent_attention_expanded(queries, rows, w_key, w_value, query_offsets, row_
     [heads, value_dim, rank]: head h's key is (w_key[h] latent, rotary key), its value w_value[h] latent.  ``queries`` [n_tokens, heads, nope + rope].
     Sequence i has queries ``query_offsets[i]:query_offsets[i + 1]`` and rows ``row_offsets[i]:row_offsets[i + 1]`` (int32, on the GPU, rising); its last query
     is aligned with its last row, and with ``causal`` a query sees the rows up to its own.  A query that sees no row gives zeros.  Queries behind
-    the last sequence give zeros, or with ``out`` [n_tokens, heads, value_dim] (contiguous) leave their rows as they were."""
+    the last sequence give zeros, or with ``out`` [n_tokens, heads, value_dim] (contiguous) leave their rows as they were.
+    Sums are float32; 16-bit rows round the expanded keys and values, and the softmax's weights, to their type (float32 rows: 32 bits throughout), and where a float16 key or value
+    would exceed 65504, the queries of its head that see it are answered row by row in the latent space, which is right and slow."""
     import torch
 
     _rows("queries", queries, 3)

@@ -56,15 +56,19 @@ template <typename T> __global__ __launch_bounds__(256) void attend_head_kernel(
 
 // ---- heads that share a key head, on the matrix units --------------------------------------------------------------------------------------------
 //
-// One wave takes 32 rows of one key head at a time for up to 16 query heads that share it; what it needs of them goes from HBM to registers once and is never
-// staged:
+// One wave takes 32 rows of one key head at a time for up to 16 query heads that share it; what it needs of them goes from HBM to registers once and is not
+// staged in LDS (variants whose registers do not hold it all spill: below):
 //   S = K Q^T      rows x heads.  Row m of the s-th 16 x 16 product is row (m / 4) * 8 + s * 4 + m % 4 of the 32, so that lane l gets the scores of the EIGHT
 //                  CONSECUTIVE rows 8 (l / 16) .. + 7 for head l % 16.
 //   O^T = V^T P^T  columns x heads.  The lane's eight probabilities are a fragment of P^T as they are; and since it owns eight consecutive rows, it loads 8 columns
 //                  (16 bytes) of each of them and transposes that 8 x 8 block in its registers: lane l's columns are 8 (l % 16) .. + 7, the d-th product
 //                  takes the d-th of them.
 // Bound by HBM: 16 heads' products are half the matrix units' time per byte, and 32 rows' keys (of the next 32) and values are in flight per wave, three waves per SIMD.
-// 4 sequences of 131071 rows, 64 heads on 8 (2.15 GB, bfloat16): 383 us, 5.6 TB/s; 64 of up to 8191 rows, 32 heads on 8 (1.07 GB): 220 us, 4.9 TB/s; a kernel that only reads reached 6.3 TB/s.
+// 4 sequences of 131071 rows, 64 heads on 8 (2.15 GB, bfloat16): 384 us, 5.6 TB/s; 64 of up to 8191 rows, 32 heads on 8 (float16; 1.04 to 1.25 GB by the lengths drawn): 211 to 246 us, 5.0 TB/s; a
+// kernel that only reads reached 6.3 TB/s.
+// Registers: rows of up to 128 aligned 16-bit columns in pages of a multiple of 8 fit, but for 15 spilled at 128 columns.  32 sequences of 4096 rows, 32 heads on 8, spilled registers and rate: bfloat16 128
+// columns 16, 4.6 TB/s; 192 28, 4.3; 256 71, 3.8; pages of 5 rows 100, 3.0; rows that are not aligned, 100 columns 48, 1.0; float32 128 columns 4, 5.5; 192 405, 2.9; 256 521, 2.9; 256 not aligned
+// 1780, 0.9; pages of 5 rows 44, 4.0.
 // The running maximum of a head is raised only when a score exceeds it by more than 2^kSlack (the accumulators are rescaled then), so the usual 32 rows cost
 // no rescaling; sums are kept per lane and joined at the end.
 //
@@ -398,7 +402,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && VB == 1 ? 3 : 2) void attend
 // Attention over the answers of a search: at most a few hundred rows, each somewhere else, for one head.  There is nothing to split and nothing for the matrix
 // units to share; what counts is how many rows are on their way at once.  One wave takes a query (of one key head): 16 lanes a row, 8 or 16 columns a lane, so four rows
 // at a time; 64 table entries are looked up by the 64 lanes at once; each 16 lanes keep a softmax of their own, joined at the end.
-// 2048 queries of 100 rows of 96 float32 columns: 22 us (78 MB of rows, from a set larger than one L2), and 48 us through attend_group_kernel, whose four waves a query have one tile each.
+// 2048 queries of 100 rows of 96 float32 columns, keys and values apart (157 MB read): 22 us from a set of 15 MB, which the caches hold (48 us through attend_group_kernel, whose four waves a query have one
+// tile each); 27 us from a million rows, 45 G lines/s of 128 bytes of the 49 that random reads reach.  Rows that are key and value at once, a million: 18 us, 34 G lines/s; bfloat16 16 us.
 // float16, 128 columns, few against group: 512 queries of 64 rows 8.9 and 12.0 us, of 256 rows 24 and 34, of 512 rows 44 and 55, of 1024 rows 84.5 and 83.5; 128 queries of 64 rows 9.0 and 9.0, of
 // 256 rows 21.5 and 17.3.  With two heads a key head and 8 key heads it is the slower one from 4096 waves on.
 
@@ -513,7 +518,8 @@ template <typename T, int E, bool Wide> __global__ __launch_bounds__(256) void a
 // LDS holds a row as 16-byte words in planes of 64 words, rows 32 bytes further apart than they are long, so that neither eight rows of a key fragment nor the 16
 // half-words of a transposed one meet in a bank; and a narrow plane for the rest, which is brought in several rows at a time and has its words exchanged in fours instead.
 // (Exchanging single words of the long rows as well, with no padding, was measured: the loads then cross each 64-byte line out of order and cost twice the time.)
-// 32 sequences of up to 8192 rows, 128 heads (36.5 GFLOP, 160 MB, bfloat16): 98 us, 373 TFLOP/s; one of 4097 rows, 16 heads: 17 us.
+// 32 sequences of up to 8192 rows, 128 heads (about 37 GFLOP, 160 to 175 MB by the lengths drawn, bfloat16): 90 to 101 us, 390 TFLOP/s; one of 4097 rows, 16 heads: 17.7 us.
+// float32 has one buffer and 16 heads a workgroup, so 128 heads bring the rows in eight times: 32 sequences of 4096 rows 579 us (104 with 16 heads); bfloat16 80 (36).
 // At 16 heads HBM bounds it; at 64 the latency of the steps between a tile's barriers (LDS is busy for 2400 cycles of a tile's 8000, the matrix units for 2176, and the loads straight to LDS,
 // which come to 30 bytes a cycle, for 2400).  Measured in place of it, 32 sequences, 128 heads: two workgroups of 32-row buffers and four waves on a compute unit, whose registers spill, 104 -> 127 us; four
 // waves of 512 registers that take 32 rows for 32 heads and read LDS half as often, 98 -> 112 us, since a wave stands still while it gives out loads and no other wave is there.

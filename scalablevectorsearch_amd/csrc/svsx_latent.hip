@@ -145,8 +145,8 @@ template <typename T> inline constexpr bool kNarrow = std::is_same<T, _Float16>:
 
 // C[i][j] = sum_k A[i][k] B[j][k] for one 128 x 128 tile; four waves of 64 x 64.  row_a(i) / row_b(j): the row, NULL = zeros.  put(i, j, v): eight consecutive i of one j.
 // Returns whether a finite sum of the wave's part is infinite in a row type of less range (false for the other types, without asking).
-// The next 128 bytes of every row are on their way to registers while these are multiplied.  8190 rows of rank 512 for 32 heads (68.7 GFLOP): 106 us, half of what a library product reaches; LDS is busy one and a
-// half times as long as the matrix units.  Two buffers and one barrier a step were measured in place of one buffer: 333 tokens 25.4 -> 27.3 us, as fewer workgroups fit a compute unit.
+// The next 128 bytes of every row are on their way to registers while these are multiplied.  8190 rows of rank 512 for 32 heads (68.7 GFLOP): 114 us, 600 TFLOP/s, less than half of what a library product reaches; LDS is busy one and a
+// half times as long as the matrix units.  Two buffers and one barrier a step were measured in place of one buffer: 333 tokens 25.4 -> 27.3 us then, as fewer workgroups fit a compute unit.
 template <typename T, bool Wide, typename A, typename B, typename P> __device__ __forceinline__ bool product_tile(unsigned char* lds, uint32_t depth, A row_a, B row_b, P put) {
     const uint32_t t = threadIdx.x, lane = t & 63, wave = t >> 6, half = lane >> 5, r = row32(lane);
     unsigned char* const plane_a = lds;
@@ -329,7 +329,8 @@ template <typename T, bool Wide> __global__ __launch_bounds__(256) void expand_k
 // A query is a lane's column throughout, so its maximum, sum and rescaling need one exchange between two lanes.  Per 64 rows a wave has 1280 cycles of products
 // (DK 192, DV 128) against 320 of LDS reads, which eight waves share, and about 1000 of softmax on the vector units: so of the two waves on a SIMD, one does its products (a tile's
 // scores and the last tile's values) while the other does its softmax, and they change over at a barrier.
-// 4095 queries on 8190 rows, 32 heads, bfloat16: 437 us, 1.18 PFLOP/s, 87 % of what an 8192^3 library product reaches.
+// 4095 queries on 8190 rows, 32 heads, bfloat16: 433 us, 1.19 PFLOP/s, 87 % of what an 8192^3 library product reaches.  The call: 547 us; float16 574; float32 4.74 ms, 123 TFLOP/s; bfloat16 with 128 heads
+// 2.36 ms.  (192, 128) with eight waves spills 1 to 3 registers at its start, no other variant any.
 template <typename T, int DK, int DV, int NW> struct PromptLayout {
     static constexpr uint32_t kRows = kPlaneCols<T>; // of a tile: a plane of V^T
     static constexpr int kKeyPlanes = DK / kPlaneCols<T>, kTiles = kRows / 32;
