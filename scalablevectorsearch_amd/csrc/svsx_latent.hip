@@ -276,11 +276,16 @@ template <typename T, bool Wide> __global__ __launch_bounds__(256) void expand_k
         return;
     }
     block -= grid.keys;
-    if (block < grid.values) { // i: row, j: (head, column); zeros in columns beyond the head's and rows beyond the last
+    if (block < grid.values) { // i: row, j: (head, column); zeros in columns beyond the head's, rows beyond the last, and rows of no sequence, which may hold anything
         const uint32_t i0 = block % grid.value_i * 128, j0 = block / grid.value_i * 128, n = a.n_heads * w.dv;
+        const int32_t begin = a.n_sequences ? a.row_offsets[0] : 0, end = a.n_sequences ? a.row_offsets[a.n_sequences] : 0;
         const T* wv = static_cast<const T*>(a.w_value);
         const bool beyond = product_tile<T, Wide>(
-            lds, a.rank, [&](uint32_t i) { return i0 + i < a.n_rows ? rows + static_cast<size_t>(i0 + i) * a.row_stride : nullptr; },
+            lds, a.rank,
+            [&](uint32_t i) {
+                const int32_t r = static_cast<int32_t>(i0 + i);
+                return i0 + i < a.n_rows && r >= begin && r < end ? rows + static_cast<size_t>(r) * a.row_stride : nullptr;
+            },
             [&](uint32_t j) {
                 const uint32_t h = (j0 + j) / w.dv, col = (j0 + j) % w.dv;
                 return j0 + j < n && col < a.dv ? wv + (static_cast<size_t>(h) * a.dv + col) * a.rank : nullptr;
@@ -340,7 +345,7 @@ template <typename T, int DK, int DV, int NW> struct PromptLayout {
     static_assert(kBytes <= 160 * 1024 && kGroups % 4 == 0 && DV % 32 == 0, "LDS; loads of four waves");
     static_assert(!kNarrow<T> || kBytes >= NW * 2 * kMaxDim * sizeof(float), "latent_query's LDS");
 };
-// One query by one wave, over the expanded rows [begin, last] alone: its lanes across the columns.
+// One query by one wave, over the expanded rows [begin, last] alone: its lanes across the columns.  Slow: a NaN in one row of 8190 that only the last of 4095 queries sees takes the call from 0.6 to 157 ms.
 template <typename T, int DK, int DV> __device__ void slow_query(const ExpandedArgs& a, const Space& w, uint32_t t, uint32_t h, int32_t begin, int32_t last) {
     const uint32_t lane = threadIdx.x & 63, dk = a.nope + a.rope;
     const T* row = static_cast<const T*>(a.queries) + t * a.query_stride + h * a.query_head_stride;
