@@ -397,45 +397,89 @@ __device__ __forceinline__ bool any_beyond(const ExpandedArgs& a, const Space& w
     return __any(beyond);
 }
 
-// One query by one wave in the latent space, where nothing is rounded on the way: w_key applied to the query, rows [begin, last], w_value to the result.  Lanes across the
-// columns; the query and the sums are in the wave's own `lds` (2 kMaxDim floats), so that this rare path takes no registers from the usual one.
+// The softmax of one wave's query over rows [begin, last] in the latent space: the query `q` and the weighted sum of rows `o` are in LDS, 8 columns a lane and 512 a chunk; four rows at a time.
+template <typename T, bool Wide> __device__ __forceinline__ void latent_rows(const ExpandedArgs& a, int32_t begin, int32_t last, const float* q, float* o, float* total) {
+    constexpr int kBatch = 4, kChunks = kMaxDim / 512;
+    const uint32_t lane = threadIdx.x & 63, width = a.rank + a.rope;
+    float top = -INFINITY, sum = 0.0f;
+#pragma unroll 1
+    for (int32_t r = begin; r <= last; r += kBatch) {
+        Frag<T> x[kBatch][kChunks];
+        float s[kBatch];
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+            const T* row = static_cast<const T*>(a.rows) + static_cast<size_t>(min(r + b, last)) * a.row_stride;
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) x[b][c] = load_frag<T, Wide>(row, c * 512 + lane * 8, width);
+            s[b] = 0.0f;
+        }
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+            const f32x8 mine = *reinterpret_cast<const f32x8*>(q + c * 512 + lane * 8);
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) s[b] = fmaf(mine[e], to_f32(x[b][c][e]), s[b]);
+        }
+        float raised = top;
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+#pragma unroll
+            for (int off = 32; off >= 1; off >>= 1) s[b] += __shfl_xor(s[b], off);
+            s[b] = r + b <= last ? s[b] * a.scale : -INFINITY;
+            raised = s[b] > raised || s[b] != s[b] ? s[b] : raised;
+        }
+        if (raised == -INFINITY) continue; // no weight yet
+        const float was = top == -INFINITY ? 0.0f : expf(top - raised);
+        top = raised;
+        sum *= was;
+        f32x8 mine[kChunks];
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) mine[c] = *reinterpret_cast<const f32x8*>(o + c * 512 + lane * 8) * was;
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+            if (s[b] == -INFINITY) continue; // no weight; it must not become the difference of two infinities
+            const float p = expf(s[b] - top);
+            sum += p;
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) mine[c][e] = fmaf(p, to_f32(x[b][c][e]), mine[c][e]);
+        }
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) *reinterpret_cast<f32x8*>(o + c * 512 + lane * 8) = mine[c];
+    }
+    *total = sum;
+}
+
+// One query by one wave in the latent space, where nothing is rounded on the way: w_key applied to the query, rows [begin, last], w_value to the result.  The query and the sums are in the
+// wave's own `lds` (2 kMaxDim floats), so that this rare path takes no registers from the usual one.  One row of 8190 whose keys are too large, 4095 queries, 32 heads: 121 ms where the last 126 queries see
+// its 128 rows, 192 ms where 2190 do (a row at a time, a column a lane: 959 and 1438 ms; the usual way 0.57).
 template <typename T> __device__ __forceinline__ void latent_query(const ExpandedArgs& a, uint32_t t, uint32_t h, int32_t begin, int32_t last, float* lds) {
     const uint32_t lane = threadIdx.x & 63, width = a.rank + a.rope;
     const T* query = static_cast<const T*>(a.queries) + t * a.query_stride + h * a.query_head_stride;
     float *const q = lds, *const o = lds + kMaxDim;
-    float top = -INFINITY, sum = 0.0f;
 #pragma unroll 1
-    for (uint32_t c = lane; c < width; c += 64) {
+    for (uint32_t c = lane; c < kMaxDim; c += 64) {
         const T* w = static_cast<const T*>(a.w_key) + static_cast<size_t>(h) * a.nope * a.rank + c;
-        float x = c < a.rank ? 0.0f : to_f32(query[a.nope + c - a.rank]);
-#pragma unroll 1
-        for (uint32_t d = 0; c < a.rank && d < a.nope; ++d) x = fmaf(to_f32(query[d]), to_f32(w[static_cast<size_t>(d) * a.rank]), x);
+        float x = c >= a.rank && c < width ? to_f32(query[a.nope + c - a.rank]) : 0.0f;
+        if (c < a.rank)
+#pragma unroll 8
+            for (uint32_t d = 0; d < a.nope; ++d) x = fmaf(to_f32(query[d]), to_f32(w[static_cast<size_t>(d) * a.rank]), x);
         q[c] = x;
         o[c] = 0.0f;
     }
-#pragma unroll 1
-    for (int32_t r = begin; r <= last; ++r) {
-        const T* row = static_cast<const T*>(a.rows) + static_cast<size_t>(r) * a.row_stride;
-        float s = 0.0f;
-#pragma unroll 1
-        for (uint32_t c = lane; c < width; c += 64) s = fmaf(q[c], to_f32(row[c]), s);
-#pragma unroll
-        for (int off = 32; off >= 1; off >>= 1) s += __shfl_xor(s, off);
-        s *= a.scale;
-        if (s == -INFINITY) continue; // no weight; it must not become the difference of two infinities
-        const float raised = s > top || s != s ? s : top, was = expf(top - raised), p = expf(s - raised);
-        top = raised;
-        sum = fmaf(sum, was, p);
-#pragma unroll 1
-        for (uint32_t c = lane; c < a.rank; c += 64) o[c] = fmaf(p, to_f32(row[c]), o[c] * was);
-    }
-    __threadfence_block(); // each lane reads the others' sums
+    __threadfence_block(); // a lane reads what others wrote
+    float sum;
+    if (width % 8 == 0 && ((reinterpret_cast<size_t>(a.rows) | a.row_stride * sizeof(T)) & 15) == 0) latent_rows<T, true>(a, begin, last, q, o, &sum);
+    else latent_rows<T, false>(a, begin, last, q, o, &sum);
+    __threadfence_block();
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll 1
     for (uint32_t c = lane; c < a.dv; c += 64) {
         const T* w = static_cast<const T*>(a.w_value) + (static_cast<size_t>(h) * a.dv + c) * a.rank;
         float y = 0.0f;
-#pragma unroll 1
+#pragma unroll 8
         for (uint32_t d = 0; d < a.rank; ++d) y = fmaf(o[d], to_f32(w[d]), y);
         static_cast<T*>(a.out)[(static_cast<size_t>(t) * a.n_heads + h) * a.dv + c] = from_f32<T>(y * inv);
     }
