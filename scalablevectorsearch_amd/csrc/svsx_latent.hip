@@ -254,12 +254,16 @@ template <typename T, bool Wide> __global__ __launch_bounds__(256) void expand_k
     const T* rows = static_cast<const T*>(a.rows);
     T* keys = static_cast<T*>(w.keys);
     T* values = static_cast<T*>(w.values);
+    auto row_of = [&](uint32_t r) -> const T* { // NULL, zeros, for rows of no sequence, which may hold anything
+        const int32_t begin = a.n_sequences ? a.row_offsets[0] : 0, end = a.n_sequences ? a.row_offsets[a.n_sequences] : 0;
+        return r < a.n_rows && static_cast<int32_t>(r) >= begin && static_cast<int32_t>(r) < end ? rows + static_cast<size_t>(r) * a.row_stride : nullptr;
+    };
     if (block < grid.keys) { // i: (head, column), j: row
         const uint32_t i0 = block % grid.key_i * 128, j0 = block / grid.key_i * 128, n = a.n_heads * a.nope;
         const T* wk = static_cast<const T*>(a.w_key);
         const bool beyond = product_tile<T, Wide>(
             lds, a.rank, [&](uint32_t i) { return i0 + i < n ? wk + static_cast<size_t>(i0 + i) * a.rank : nullptr; },
-            [&](uint32_t j) { return j0 + j < a.n_rows ? rows + static_cast<size_t>(j0 + j) * a.row_stride : nullptr; },
+            [&](uint32_t j) { return row_of(j0 + j); },
             [&](uint32_t i, uint32_t j, const Frag<T>& v) {
                 if (j0 + j >= a.n_rows) return;
                 if (a.nope % 8 == 0) {
@@ -276,16 +280,11 @@ template <typename T, bool Wide> __global__ __launch_bounds__(256) void expand_k
         return;
     }
     block -= grid.keys;
-    if (block < grid.values) { // i: row, j: (head, column); zeros in columns beyond the head's, rows beyond the last, and rows of no sequence, which may hold anything
+    if (block < grid.values) { // i: row, j: (head, column); zeros in columns beyond the head's and rows beyond the last
         const uint32_t i0 = block % grid.value_i * 128, j0 = block / grid.value_i * 128, n = a.n_heads * w.dv;
-        const int32_t begin = a.n_sequences ? a.row_offsets[0] : 0, end = a.n_sequences ? a.row_offsets[a.n_sequences] : 0;
         const T* wv = static_cast<const T*>(a.w_value);
         const bool beyond = product_tile<T, Wide>(
-            lds, a.rank,
-            [&](uint32_t i) {
-                const int32_t r = static_cast<int32_t>(i0 + i);
-                return i0 + i < a.n_rows && r >= begin && r < end ? rows + static_cast<size_t>(r) * a.row_stride : nullptr;
-            },
+            lds, a.rank, [&](uint32_t i) { return row_of(i0 + i); },
             [&](uint32_t j) {
                 const uint32_t h = (j0 + j) / w.dv, col = (j0 + j) % w.dv;
                 return j0 + j < n && col < a.dv ? wv + (static_cast<size_t>(h) * a.dv + col) * a.rank : nullptr;
